@@ -1,4 +1,5 @@
-"""ctypes binding of the C ABI declared in ``include/w8a8_tp.h``.
+"""ctypes binding of the C ABI declared in ``include/w8a8_tp.h`` and
+``include/mxfp4.h``.
 
 The shared library ``_w8a8_tp.so`` is built in-tree by ``build.py``.  There is
 no fallback: if the library is missing, every op raises.
@@ -85,6 +86,19 @@ SIGNATURES = {
     "w8a8_comm_destroy": (None, [_c_vp]),
 }
 
+# the MXFP4 entry points: the list include/mxfp4.h declares
+MXFP4_SIGNATURES = {
+    "mxfp4_scale_bytes": (_c_i64, [_c_i64, _c_i64]),
+    "mxfp4_quant": (_c_int, [_c_vp, _c_i64, _c_int, _c_vp, _c_vp, _c_i64, _c_i64, _c_vp]),
+    "mxfp4_dequant": (_c_int, [_c_vp, _c_vp, _c_vp, _c_int, _c_i64, _c_i64, _c_vp]),
+    "mxfp4_silu_mul_quant": (_c_int, [_c_vp, _c_i64, _c_int, _c_vp, _c_vp, _c_i64, _c_i64, _c_vp]),
+    "mxfp4_rmsnorm_quant": (_c_int, [_c_vp, _c_i64, _c_vp, _c_i64, _c_vp, ctypes.c_float, _c_int, _c_vp, _c_vp,
+                                     _c_i64, _c_i64, _c_vp]),
+    "mxfp4_gemm": (_c_int, [_c_vp, _c_vp, _c_vp, _c_vp, _c_vp, _c_vp, _c_int, _c_i64, _c_i64, _c_i64, _c_vp]),
+    "mxfp4_gemm_silu_quant": (_c_int, [_c_vp, _c_vp, _c_vp, _c_vp, _c_vp, _c_int, _c_vp, _c_vp, _c_i64, _c_i64,
+                                       _c_i64, _c_vp]),
+}
+
 _lib = None
 _lock = threading.Lock()
 
@@ -100,7 +114,7 @@ def load() -> ctypes.CDLL:
                 raise W8A8Error(ERR_UNSUPPORTED,
                                 f"{LIB_PATH} is not built; run `python mini-sglang-fork_b200/build.py`")
             lib = ctypes.CDLL(LIB_PATH)
-            for name, (res, args) in SIGNATURES.items():
+            for name, (res, args) in {**SIGNATURES, **MXFP4_SIGNATURES}.items():
                 fn = getattr(lib, name)
                 fn.restype = res
                 fn.argtypes = args

@@ -62,7 +62,7 @@ def _stale() -> bool:
         return True
     t = os.path.getmtime(LIB_PATH)
     deps = [os.path.join(CSRC, f) for f in os.listdir(CSRC)]
-    deps.append(os.path.join(REPO, "include", "w8a8_tp.h"))
+    deps += [os.path.join(REPO, "include", h) for h in ("w8a8_tp.h", "mxfp4.h")]
     deps.append(os.path.abspath(__file__))
     return any(os.path.getmtime(d) > t for d in deps)
 

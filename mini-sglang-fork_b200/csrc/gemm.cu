@@ -52,6 +52,23 @@ int encode_operand(CUtensorMap* tm, const void* base, int64_t rows, int64_t K, i
   return W8A8_OK;
 }
 
+// Tensor map over a row-major matrix of 32-bit words [rows, words] read as
+// boxes of one row x box_words; out-of-range rows and words read as zero.
+int encode_words(CUtensorMap* tm, const void* base, int64_t rows, int64_t words, int box_words) {
+  auto enc = tensor_map_encoder();
+  W8A8_REQUIRE(enc != nullptr, W8A8_ERR_CUDA, "cuTensorMapEncodeTiled is unavailable from the driver");
+  cuuint64_t dims[2] = {static_cast<cuuint64_t>(words), static_cast<cuuint64_t>(rows)};
+  cuuint64_t strides[1] = {static_cast<cuuint64_t>(words) * 4};
+  cuuint32_t box[2] = {static_cast<cuuint32_t>(box_words), 1u};
+  cuuint32_t estr[2] = {1u, 1u};
+  CUresult r = enc(tm, CU_TENSOR_MAP_DATA_TYPE_UINT32, 2, const_cast<void*>(base), dims, strides, box, estr,
+                   CU_TENSOR_MAP_INTERLEAVE_NONE, CU_TENSOR_MAP_SWIZZLE_NONE, CU_TENSOR_MAP_L2_PROMOTION_L2_256B,
+                   CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE);
+  W8A8_REQUIRE(r == CUDA_SUCCESS, W8A8_ERR_CUDA, "cuTensorMapEncodeTiled failed (%d) for rows=%lld words=%lld",
+               (int)r, (long long)rows, (long long)words);
+  return W8A8_OK;
+}
+
 namespace {
 
 template <int BN, int STAGES, bool SWAP, bool FUSED>

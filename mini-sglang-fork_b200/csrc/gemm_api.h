@@ -27,6 +27,10 @@ int run_gemm(const int8_t* A, const int8_t* B, const float* sa, const float* sb,
 // and columns read as zero.
 int encode_operand(CUtensorMap* tm, const void* base, int64_t rows, int64_t K, int box_rows);
 
+// Tensor map over a row-major matrix of 32-bit words [rows, words] (row
+// stride `words`) read as boxes of one row x box_words.
+int encode_words(CUtensorMap* tm, const void* base, int64_t rows, int64_t words, int box_words);
+
 // Host-side checks of a GEMM call (shape limits, null pointers, 16-byte
 // alignment) that run_gemm makes before any launch; 0 or a status code.
 int validate_gemm_args(const int8_t* A, const int8_t* B, const float* sa, const float* sb, const void* C,

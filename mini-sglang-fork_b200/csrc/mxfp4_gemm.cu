@@ -1,0 +1,138 @@
+// Host side of the MXFP4 GEMM: which kernel a shape gets, the tensor maps, the
+// launches.
+#include <algorithm>
+#include <cstring>
+#include <mutex>
+
+#include "gemm_api.h"
+#include "mxfp4_sm100.cuh"
+
+namespace w8a8 {
+namespace mx {
+namespace {
+
+// Allows a kernel its dynamic shared memory, once per device.
+template <auto Kern>
+int allow_smem(int bytes) {
+  static std::mutex mu;
+  static bool done[64] = {false};
+  const int dev = current_device();
+  W8A8_REQUIRE(dev >= 0 && dev < 64, W8A8_ERR_CUDA, "no current device");
+  std::lock_guard<std::mutex> lk(mu);
+  if (!done[dev]) {
+    W8A8_CUDA_TRY(cudaFuncSetAttribute(Kern, cudaFuncAttributeMaxDynamicSharedMemorySize, bytes));
+    done[dev] = true;
+  }
+  return W8A8_OK;
+}
+
+struct Operands {
+  const uint8_t *a, *as, *b, *bs;
+  int64_t b_rows;  // rows of B: N, or 2I
+};
+
+// Shares of K per output tile: enough CTAs to give every SM about two, at least
+// two k blocks each (one for the shortest K), at most a portable cluster's 8.
+int pick_split(int tiles, int kblocks, int nsm) {
+  int s = 1;
+  while (s < 8 && tiles * s * 2 <= 2 * nsm && kblocks >= 2 * (2 * s)) s *= 2;
+  return s;
+}
+
+template <typename O, int T, bool SILU>
+int launch_row(const Operands& o, MxGemmArgs args, cudaStream_t stream) {
+  using P = MxRowTraits<T, SILU>;
+  constexpr auto kern = mx_row_kernel<O, T, SILU>;
+  if (int rc = allow_smem<kern>(P::kSmemBytes)) return rc;
+  args.wtiles = (args.N + 127) / 128;
+  args.ttiles = (args.M + T - 1) / T;
+  CUtensorMap tw, tws, tx, txs;
+  if (int rc = encode_operand(&tw, o.b, o.b_rows, args.K / 2, 128)) return rc;
+  if (int rc = encode_words(&tws, o.bs, row_tiles(o.b_rows), k_tiles(args.K) * kTileBytes / 4, 256)) return rc;
+  if (int rc = encode_operand(&tx, o.a, args.M, args.K / 2, T)) return rc;
+  if (int rc = encode_words(&txs, o.as, row_tiles(args.M), k_tiles(args.K) * kTileBytes / 4, 256)) return rc;
+  const int64_t tiles = static_cast<int64_t>(args.wtiles) * args.ttiles;
+  const int split = tiles > 4096 ? 1 : pick_split(static_cast<int>(tiles), args.kblocks, sm_count());
+  W8A8_REQUIRE(tiles * split <= 0x7fffffffLL, W8A8_ERR_UNSUPPORTED, "mxfp4_gemm: too many output tiles");
+  cudaLaunchConfig_t cfg = {};
+  cfg.gridDim = dim3(static_cast<unsigned>(tiles * split));
+  cfg.blockDim = dim3(kRowThreads);
+  cfg.dynamicSmemBytes = P::kSmemBytes;
+  cfg.stream = stream;
+  cudaLaunchAttribute attr[2];
+  attr[0].id = cudaLaunchAttributeProgrammaticStreamSerialization;
+  attr[0].val.programmaticStreamSerializationAllowed = 1;
+  attr[1].id = cudaLaunchAttributeClusterDimension;
+  attr[1].val.clusterDim.x = static_cast<unsigned>(split);
+  attr[1].val.clusterDim.y = 1;
+  attr[1].val.clusterDim.z = 1;
+  cfg.attrs = attr;
+  cfg.numAttrs = 2;
+  W8A8_CUDA_TRY(cudaLaunchKernelEx(&cfg, kern, tw, tws, tx, txs, args));
+  return W8A8_OK;
+}
+
+template <typename O, bool SILU>
+int dispatch(const Operands& o, const MxGemmArgs& args, cudaStream_t stream) {
+  if (args.M <= 16) return launch_row<O, 16, SILU>(o, args, stream);
+  if (args.M <= 32) return launch_row<O, 32, SILU>(o, args, stream);
+  if (args.M <= 64) return launch_row<O, 64, SILU>(o, args, stream);
+  return launch_row<O, 128, SILU>(o, args, stream);
+}
+
+int run(const char* what, const Operands& o, const void* bias, void* C, uint8_t* q, uint8_t* qs, int dtype, int64_t M,
+        int64_t N, int64_t K, bool silu, cudaStream_t stream) {
+  W8A8_REQUIRE(M >= 0 && N >= 0 && K >= 0, W8A8_ERR_INVALID_ARG, "%s: negative shape", what);
+  if (M == 0 || N == 0) return W8A8_OK;
+  W8A8_REQUIRE(K > 0 && K % kBlock == 0, W8A8_ERR_INVALID_ARG, "%s: K=%lld must be a positive multiple of 32", what,
+               (long long)K);
+  W8A8_REQUIRE(o.a && o.as && o.b && o.bs && (silu ? q && qs : C != nullptr), W8A8_ERR_INVALID_ARG, "%s: null pointer", what);
+  W8A8_REQUIRE(dtype == kBf16 || dtype == kFp16, W8A8_ERR_INVALID_ARG, "%s: bf16 or fp16", what);
+  W8A8_REQUIRE(M <= (1LL << 27) && N <= (1LL << 27) && K <= (1LL << 27), W8A8_ERR_UNSUPPORTED, "%s: shape too large",
+               what);
+  W8A8_REQUIRE(!silu || N % 128 == 0, W8A8_ERR_UNSUPPORTED, "%s: I=%lld must be a multiple of 128", what, (long long)N);
+  W8A8_REQUIRE(W8A8_ALIGNED16(o.a) && W8A8_ALIGNED16(o.as) && W8A8_ALIGNED16(o.b) && W8A8_ALIGNED16(o.bs) &&
+                   W8A8_ALIGNED16(C) && W8A8_ALIGNED16(q) && W8A8_ALIGNED16(qs) &&
+                   (reinterpret_cast<uintptr_t>(bias) & 1u) == 0,
+               W8A8_ERR_ALIGNMENT, "%s: operands and result must be 16-byte aligned", what);
+  W8A8_REQUIRE(device_cc_major() == 10, W8A8_ERR_UNSUPPORTED,
+               "%s: the tcgen05 kernels need an sm_100 (B200) device; found compute capability %d.x", what,
+               device_cc_major());
+  MxGemmArgs args;
+  std::memset(&args, 0, sizeof(args));
+  args.bias = bias;
+  args.out = C;
+  args.q = q;
+  args.qs = qs;
+  args.err = device_error_word();
+  if (!args.err) return W8A8_ERR_CUDA;
+  args.timeout_ns = kDefaultGemmTimeoutNs;
+  args.M = static_cast<int>(M);
+  args.N = static_cast<int>(N);
+  args.K = static_cast<int>(K);
+  args.kblocks = static_cast<int>((K + 255) / 256);
+  if (dtype == kBf16)
+    return silu ? dispatch<__nv_bfloat16, true>(o, args, stream) : dispatch<__nv_bfloat16, false>(o, args, stream);
+  return silu ? dispatch<__half, true>(o, args, stream) : dispatch<__half, false>(o, args, stream);
+}
+
+}  // namespace
+}  // namespace mx
+}  // namespace w8a8
+
+extern "C" {
+
+int mxfp4_gemm(const uint8_t* a_data, const uint8_t* a_scales, const uint8_t* b_data, const uint8_t* b_scales,
+               const void* bias, void* C, int dtype, int64_t M, int64_t N, int64_t K, void* stream) {
+  return w8a8::mx::run("mxfp4_gemm", {a_data, a_scales, b_data, b_scales, N}, bias, C, nullptr, nullptr, dtype, M, N,
+                       K, false, static_cast<cudaStream_t>(stream));
+}
+
+int mxfp4_gemm_silu_quant(const uint8_t* a_data, const uint8_t* a_scales, const uint8_t* b_data,
+                          const uint8_t* b_scales, const void* bias, int dtype, uint8_t* y_data, uint8_t* y_scales,
+                          int64_t M, int64_t I, int64_t K, void* stream) {
+  return w8a8::mx::run("mxfp4_gemm_silu_quant", {a_data, a_scales, b_data, b_scales, 2 * I}, bias, nullptr, y_data,
+                       y_scales, dtype, M, I, K, true, static_cast<cudaStream_t>(stream));
+}
+
+}  // extern "C"

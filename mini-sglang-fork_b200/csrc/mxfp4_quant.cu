@@ -1,0 +1,611 @@
+// MXFP4 quantisers of the linear path's activations: plain, fused with
+// SiLU*mul, fused with residual add + RMSNorm; and the inverse.
+//
+// Thread mapping, shared by the three: a lane holds 8 consecutive values (one
+// 16-byte load), so four lanes share a block of 32 and a warp covers 256
+// values of a row, which is exactly two scale tiles of that row.  The block's
+// largest magnitude takes two shuffles; the 8 codes of a lane are one 4-byte
+// store (128 contiguous bytes per warp); lanes 0 and 16 collect their tile's
+// four scale bytes and store them as one word.  Lanes beyond the row's end
+// hold zeros, whose scale byte is 0, so the padding blocks of the last tiles
+// come out as the format asks without a case of their own.
+//
+// The plain quantiser is exact: the scale is a power of two, so x / s has no
+// rounding and the only rounding is E2M1's own.  The fused ones quantise a
+// computed y, for which they first work in fp32 with a relative error below
+// `d`: if y (1 - d) and y (1 + d) round to the same code and the block's
+// largest magnitude has the same exponent at both ends, that code and scale
+// are those of the exact value.  Where they differ (about one value in 10^5)
+// the values concerned are evaluated in 64 bits, out of line.  Two
+// conversions instead of one per value, and the result does not depend on how
+// exp or the row's sum were evaluated.
+#include "common.cuh"
+#include "mxfp4.cuh"
+#include "sm100.cuh"
+
+namespace w8a8 {
+namespace mx {
+namespace {
+
+constexpr int kThreads = 256;
+
+// max over the four lanes of a block
+__device__ __forceinline__ uint32_t quad_max(uint32_t v) {
+  v = max(v, __shfl_xor_sync(0xffffffffu, v, 1));
+  return max(v, __shfl_xor_sync(0xffffffffu, v, 2));
+}
+
+// Stores a warp's scale bytes (one per block, in every lane of the block):
+// the words of k tiles kt and kt + 1, from lanes 0 and 16.
+__device__ __forceinline__ void store_scales(uint8_t* scales, int64_t row, int64_t kt, int64_t ktiles, int lane,
+                                             int byte) {
+  uint32_t w = static_cast<uint32_t>(byte);
+  w |= __shfl_down_sync(0xffffffffu, w, 4) << 8;
+  w |= __shfl_down_sync(0xffffffffu, w, 8) << 16;
+  if ((lane & 15) == 0)
+    *reinterpret_cast<uint32_t*>(scales + scale_offset(row, kt + (lane >> 4), ktiles)) = w;
+}
+
+__device__ __forceinline__ uint32_t amax8(const float (&v)[8]) {
+  uint32_t m = abs_bits(v[0]);
+#pragma unroll
+  for (int j = 1; j < 8; ++j) m = max(m, abs_bits(v[j]));
+  return m;
+}
+
+// ------------------------------------------------------------------- plain
+// A warp takes VPT consecutive groups of 256 values of one row.
+template <typename T, int VPT>
+__global__ void __launch_bounds__(kThreads) quant_kernel(const T* __restrict__ x, int64_t ldx, uint8_t* __restrict__ data,
+                                                         uint8_t* __restrict__ scales, int64_t M, int K, int segs) {
+  const int lane = threadIdx.x & 31;
+  const int64_t task = static_cast<int64_t>(blockIdx.x) * (kThreads / 32) + (threadIdx.x >> 5);
+  const int64_t row = task / segs;
+  const int g0 = static_cast<int>(task - row * segs) * VPT;  // first 256-value group
+  const int nvec = K >> 3;
+  const int64_t kt = k_tiles(K);
+  dev::griddep_launch();
+  dev::griddep_wait();
+  if (row >= M) return;
+  const uint4* xr = reinterpret_cast<const uint4*>(x + row * ldx);
+  uint32_t* qr = reinterpret_cast<uint32_t*>(data + row * (K >> 1));
+  uint4 raw[VPT];
+#pragma unroll
+  for (int j = 0; j < VPT; ++j) {
+    const int vi = (g0 + j) * 32 + lane;
+    raw[j] = vi < nvec ? __ldcs(xr + vi) : make_uint4(0, 0, 0, 0);
+  }
+#pragma unroll
+  for (int j = 0; j < VPT; ++j) {
+    const int vi = (g0 + j) * 32 + lane;
+    if ((g0 + j) * 32 >= nvec) break;  // the whole warp is beyond the row
+    float v[8];
+    unpack8<T>(raw[j], v);
+    const int byte = scale_byte(quad_max(amax8(v)));
+    const uint32_t w = byte == kNanScale ? 0u : pack8_scaled(v, inv_scale(byte));
+    if (vi < nvec) qr[vi] = w;
+    store_scales(scales, row, 2 * (g0 + j), kt, lane, byte);
+  }
+}
+
+// -------------------------------------------------------------- SiLU * mul
+constexpr float kSiluDelta = 3.814697265625e-6f;  // 2^-18, see silu_mul_fast
+
+__device__ inline double silu_mul_exact(float g, float u) {
+  const double gd = g;
+  return gd / (1.0 + exp(-gd)) * static_cast<double>(u);
+}
+
+template <typename T>
+__device__ __noinline__ double silu_amax_exact(uint4 graw, uint4 uraw) {
+  float g[8], u[8];
+  unpack8<T>(graw, g);
+  unpack8<T>(uraw, u);
+  double m = 0.0;
+  for (int j = 0; j < 8; ++j) {
+    const double a = fabs(silu_mul_exact(g[j], u[j]));
+    m = (a > m || isnan(a)) ? a : m;
+  }
+  return m;
+}
+
+template <typename T>
+__device__ __noinline__ uint32_t silu_codes_exact(uint4 graw, uint4 uraw, int byte, uint32_t lo, uint32_t hi) {
+  float g[8], u[8];
+  unpack8<T>(graw, g);
+  unpack8<T>(uraw, u);
+  const double f = ldexp(1.0, 127 - byte);
+  for (int j = 0; j < 8; ++j) {
+    if (((lo ^ hi) >> (4 * j)) & 15u)
+      lo = (lo & ~(15u << (4 * j))) | (code_of(silu_mul_exact(g[j], u[j]) * f) << (4 * j));
+  }
+  return lo;
+}
+
+// Whether a vector holds a gate outside the fast form's range: below -40,
+// where exp's argument error grows, or (bf16 only) a nonzero one below 2^-100,
+// whose product with the sigmoid would be rounded as a subnormal before a large
+// `up` scales it back.  Taken on the 16-bit pairs: min and min |.| in 8
+// instructions; a zero gate only costs the call.
+template <typename T>
+__device__ __forceinline__ bool far_gate(const uint4& raw);
+
+template <>
+__device__ __forceinline__ bool far_gate<__nv_bfloat16>(const uint4& raw) {
+  const __nv_bfloat162* h = reinterpret_cast<const __nv_bfloat162*>(&raw);
+  const __nv_bfloat162 m = __hmin2(__hmin2(h[0], h[1]), __hmin2(h[2], h[3]));
+  const __nv_bfloat162 a = __hmin2(__hmin2(__habs2(h[0]), __habs2(h[1])), __hmin2(__habs2(h[2]), __habs2(h[3])));
+  return fminf(__low2float(m), __high2float(m)) < -40.0f ||
+         fminf(__low2float(a), __high2float(a)) < 7.888609052210118e-31f;
+}
+
+template <>
+__device__ __forceinline__ bool far_gate<__half>(const uint4& raw) {
+  const __half2* h = reinterpret_cast<const __half2*>(&raw);
+  const __half2 m = __hmin2(__hmin2(h[0], h[1]), __hmin2(h[2], h[3]));
+  return fminf(__low2float(m), __high2float(m)) < -40.0f;
+}
+
+// The exact product, rounded once to fp32, of those gates.  Below -200 it is a
+// zero of the product's sign next to any scale, which the fast form gives.
+template <typename T>
+__device__ __noinline__ void silu_far(uint4 graw, uint4 uraw, float (&y)[8]) {
+  float g[8], u[8];
+  unpack8<T>(graw, g);
+  unpack8<T>(uraw, u);
+  for (int j = 0; j < 8; ++j) {
+    const bool low = g[j] < -40.0f && g[j] > -200.0f;
+    const bool tiny = g[j] != 0.0f && fabsf(g[j]) < 7.888609052210118e-31f;
+    if (low || tiny) y[j] = static_cast<float>(silu_mul_exact(g[j], u[j]));
+  }
+}
+
+template <typename T, int VPT>
+__global__ void __launch_bounds__(kThreads) silu_kernel(const T* __restrict__ gate_up, int64_t ld,
+                                                        uint8_t* __restrict__ data, uint8_t* __restrict__ scales,
+                                                        int64_t M, int I, int segs) {
+  const int lane = threadIdx.x & 31;
+  const int64_t task = static_cast<int64_t>(blockIdx.x) * (kThreads / 32) + (threadIdx.x >> 5);
+  const int64_t row = task / segs;
+  const int g0 = static_cast<int>(task - row * segs) * VPT;
+  const int nvec = I >> 3;
+  const int64_t kt = k_tiles(I);
+  dev::griddep_launch();
+  dev::griddep_wait();
+  if (row >= M) return;
+  const uint4* gr = reinterpret_cast<const uint4*>(gate_up + row * ld);
+  const uint4* ur = gr + nvec;
+  uint32_t* qr = reinterpret_cast<uint32_t*>(data + row * (I >> 1));
+  uint4 graw[VPT], uraw[VPT];
+#pragma unroll
+  for (int j = 0; j < VPT; ++j) {
+    const int vi = (g0 + j) * 32 + lane;
+    graw[j] = vi < nvec ? __ldcs(gr + vi) : make_uint4(0, 0, 0, 0);
+    uraw[j] = vi < nvec ? __ldcs(ur + vi) : make_uint4(0, 0, 0, 0);
+  }
+#pragma unroll
+  for (int j = 0; j < VPT; ++j) {
+    const int vi = (g0 + j) * 32 + lane;
+    if ((g0 + j) * 32 >= nvec) break;
+    float y[8];
+    {
+      float g[8], u[8];
+      unpack8<T>(graw[j], g);
+      unpack8<T>(uraw[j], u);
+#pragma unroll
+      for (int e = 0; e < 8; ++e) y[e] = silu_mul_fast(g[e], u[e]);
+      if (far_gate<T>(graw[j])) silu_far<T>(graw[j], uraw[j], y);
+    }
+    const uint32_t m = quad_max(amax8(y));
+    const float amax = __uint_as_float(m);
+    int byte = scale_byte(abs_bits(amax * (1.0f - kSiluDelta)));
+    if (byte != scale_byte(abs_bits(amax * (1.0f + kSiluDelta)))) {
+      // next to a power of two: all four lanes of the block come here
+      double d = silu_amax_exact<T>(graw[j], uraw[j]);
+      const uint32_t quad = 15u << (lane & 28);
+#pragma unroll
+      for (int o = 1; o <= 2; o *= 2) {
+        const double other = __shfl_xor_sync(quad, d, o);
+        d = (other > d || isnan(other)) ? other : d;
+      }
+      byte = scale_byte(d);
+    }
+    uint32_t w = 0;
+    if (byte != kNanScale) {
+      const float f = inv_scale(byte);
+      w = pack8_scaled(y, f * (1.0f - kSiluDelta));
+      const uint32_t hi = pack8_scaled(y, f * (1.0f + kSiluDelta));
+      if (w != hi) w = silu_codes_exact<T>(graw[j], uraw[j], byte, w, hi);
+    }
+    if (vi < nvec) qr[vi] = w;
+    store_scales(scales, row, 2 * (g0 + j), kt, lane, byte);
+  }
+}
+
+// ----------------------------------------------------------------- RMSNorm
+// One CTA per row, lane t of the CTA holding vectors t + blockDim * j.  The
+// sum of squares is taken in fp32 over four values and in 64 bits from there
+// (one conversion and one add per four values), so r is good to fp32 and the
+// exact path can use the same sum.  y = (v r) w in fp32: errors of r (2.5e-7)
+// and of the two products stay below 2^-20.
+constexpr float kNormDelta = 9.5367431640625e-7f;  // 2^-20
+constexpr int kNormMaxThreads = 1024;
+
+struct NormRow {
+  double ss;  // sum of v^2 over the row
+  int K;
+  float eps;
+};
+
+template <typename T>
+__device__ inline double norm_exact(float x, float res, float w, const NormRow& n) {
+  const double v = static_cast<double>(x) + static_cast<double>(res);
+  return v / sqrt(n.ss / n.K + static_cast<double>(n.eps)) * static_cast<double>(w);
+}
+
+template <typename T>
+__device__ __noinline__ double norm_amax_exact(uint4 xr, uint4 rr, uint4 wr, NormRow n) {
+  float x[8], r[8], w[8];
+  unpack8<T>(xr, x);
+  unpack8<T>(rr, r);
+  unpack8<T>(wr, w);
+  double m = 0.0;
+  for (int j = 0; j < 8; ++j) {
+    const double a = fabs(norm_exact<T>(x[j], r[j], w[j], n));
+    m = (a > m || isnan(a)) ? a : m;
+  }
+  return m;
+}
+
+template <typename T>
+__device__ __noinline__ uint32_t norm_codes_exact(uint4 xr, uint4 rr, uint4 wr, NormRow n, int byte, uint32_t lo,
+                                                  uint32_t hi) {
+  float x[8], r[8], w[8];
+  unpack8<T>(xr, x);
+  unpack8<T>(rr, r);
+  unpack8<T>(wr, w);
+  const double f = ldexp(1.0, 127 - byte);
+  for (int j = 0; j < 8; ++j) {
+    if (((lo ^ hi) >> (4 * j)) & 15u)
+      lo = (lo & ~(15u << (4 * j))) | (code_of(norm_exact<T>(x[j], r[j], w[j], n) * f) << (4 * j));
+  }
+  return lo;
+}
+
+template <typename T>
+__device__ __noinline__ void norm_far(uint4 xr, uint4 rr, uint4 wr, NormRow n, float (&y)[8]) {
+  float x[8], r[8], w[8];
+  unpack8<T>(xr, x);
+  unpack8<T>(rr, r);
+  unpack8<T>(wr, w);
+  for (int j = 0; j < 8; ++j) y[j] = static_cast<float>(norm_exact<T>(x[j], r[j], w[j], n));
+}
+
+template <typename T, int VPT, bool ADD>
+__global__ void __launch_bounds__(kNormMaxThreads)
+    rmsnorm_kernel(const T* __restrict__ x, int64_t ldx, T* residual, int64_t ldr, const T* __restrict__ weight,
+                   float eps, uint8_t* __restrict__ data, uint8_t* __restrict__ scales, int64_t M, int K) {
+  __shared__ double part[32];
+  const int lane = threadIdx.x & 31;
+  const int warps = blockDim.x >> 5;
+  const int nvec = K >> 3;
+  const int64_t kt = k_tiles(K);
+  dev::griddep_launch();
+  dev::griddep_wait();
+  const int64_t row = blockIdx.x;
+  const uint4* xr = reinterpret_cast<const uint4*>(x + row * ldx);
+  uint4* rr = ADD ? reinterpret_cast<uint4*>(residual + row * ldr) : nullptr;
+  const uint4* wr = reinterpret_cast<const uint4*>(weight);
+  const uint4 zero = make_uint4(0, 0, 0, 0);
+  uint4 xa[VPT], ra[VPT];
+#pragma unroll
+  for (int j = 0; j < VPT; ++j) {
+    const int vi = threadIdx.x + j * blockDim.x;
+    xa[j] = vi < nvec ? __ldcs(xr + vi) : zero;
+    ra[j] = ADD && vi < nvec ? rr[vi] : zero;
+  }
+  float v[VPT][8];
+  double ss = 0.0;
+#pragma unroll
+  for (int j = 0; j < VPT; ++j) {
+    const int vi = threadIdx.x + j * blockDim.x;
+    unpack8<T>(xa[j], v[j]);
+    if constexpr (ADD) {
+      float r[8];
+      unpack8<T>(ra[j], r);
+#pragma unroll
+      for (int e = 0; e < 8; ++e) v[j][e] += r[e];
+      if (vi < nvec)
+        rr[vi] = make_uint4(pack2<T>(v[j][0], v[j][1]), pack2<T>(v[j][2], v[j][3]), pack2<T>(v[j][4], v[j][5]),
+                            pack2<T>(v[j][6], v[j][7]));
+    }
+#pragma unroll
+    for (int e = 0; e < 8; e += 4) {
+      // a sum that leaves fp32 (|v| above 1e19) is taken in 64 bits
+      const float s = v[j][e] * v[j][e] + v[j][e + 1] * v[j][e + 1] + v[j][e + 2] * v[j][e + 2] +
+                      v[j][e + 3] * v[j][e + 3];
+      if (s > 1e30f || s < 1e-30f) {
+#pragma unroll
+        for (int i = 0; i < 4; ++i) ss += static_cast<double>(v[j][e + i]) * v[j][e + i];
+      } else {
+        ss += s;
+      }
+    }
+  }
+#pragma unroll
+  for (int o = 16; o > 0; o >>= 1) ss += __shfl_xor_sync(0xffffffffu, ss, o);
+  if (lane == 0) part[threadIdx.x >> 5] = ss;
+  __syncthreads();
+  ss = lane < warps ? part[lane] : 0.0;
+#pragma unroll
+  for (int o = 16; o > 0; o >>= 1) ss += __shfl_xor_sync(0xffffffffu, ss, o);
+  const NormRow n = {ss, K, eps};
+  const double mean = ss * (1.0 / K) + static_cast<double>(eps);
+  // a row whose mean square nears the ends of fp32's range is taken in 64 bits
+  const bool far = !(mean > 1e-30 && mean < 1e30);
+  const float r = 1.0f / sqrtf(static_cast<float>(mean));
+#pragma unroll
+  for (int j = 0; j < VPT; ++j) {
+    const int base = (threadIdx.x & ~31) + j * blockDim.x;
+    if (base >= nvec) break;
+    const int vi = base + lane;
+    const uint4 wraw = vi < nvec ? __ldg(wr + vi) : zero;
+    float w[8], y[8];
+    unpack8<T>(wraw, w);
+#pragma unroll
+    for (int e = 0; e < 8; ++e) y[e] = v[j][e] * r * w[e];
+    if (far) norm_far<T>(xa[j], ra[j], wraw, n, y);
+    // a lane beyond the row holds zeros whatever r is (0 * inf would be NaN)
+    if (vi >= nvec) {
+#pragma unroll
+      for (int e = 0; e < 8; ++e) y[e] = 0.0f;
+    }
+    const float amax = __uint_as_float(quad_max(amax8(y)));
+    int byte = scale_byte(abs_bits(amax * (1.0f - kNormDelta)));
+    if (byte != scale_byte(abs_bits(amax * (1.0f + kNormDelta)))) {
+      double d = norm_amax_exact<T>(xa[j], ra[j], wraw, n);
+      const uint32_t quad = 15u << (lane & 28);
+#pragma unroll
+      for (int o = 1; o <= 2; o *= 2) {
+        const double other = __shfl_xor_sync(quad, d, o);
+        d = (other > d || isnan(other)) ? other : d;
+      }
+      byte = scale_byte(d);
+    }
+    uint32_t code = 0;
+    if (byte != kNanScale) {
+      const float f = inv_scale(byte);
+      code = pack8_scaled(y, f * (1.0f - kNormDelta));
+      const uint32_t hi = pack8_scaled(y, f * (1.0f + kNormDelta));
+      if (code != hi) code = norm_codes_exact<T>(xa[j], ra[j], wraw, n, byte, code, hi);
+    }
+    if (vi < nvec) reinterpret_cast<uint32_t*>(data + row * (K >> 1))[vi] = code;
+    store_scales(scales, row, 2 * (base >> 5), kt, lane, byte);
+  }
+}
+
+// ----------------------------------------------------------------- inverse
+template <typename O>
+__device__ __forceinline__ void store8(O* out, const float (&v)[8]) {
+  if constexpr (sizeof(O) == 4) {
+    reinterpret_cast<float4*>(out)[0] = make_float4(v[0], v[1], v[2], v[3]);
+    reinterpret_cast<float4*>(out)[1] = make_float4(v[4], v[5], v[6], v[7]);
+  } else {
+    *reinterpret_cast<uint4*>(out) = make_uint4(pack2<O>(v[0], v[1]), pack2<O>(v[2], v[3]), pack2<O>(v[4], v[5]),
+                                                pack2<O>(v[6], v[7]));
+  }
+}
+
+template <typename O, int VPT>
+__global__ void __launch_bounds__(kThreads) dequant_kernel(const uint8_t* __restrict__ data,
+                                                           const uint8_t* __restrict__ scales, O* __restrict__ out,
+                                                           int64_t M, int K, int segs) {
+  const int lane = threadIdx.x & 31;
+  const int64_t task = static_cast<int64_t>(blockIdx.x) * (kThreads / 32) + (threadIdx.x >> 5);
+  const int64_t row = task / segs;
+  const int g0 = static_cast<int>(task - row * segs) * VPT;
+  const int nvec = K >> 3;
+  const int64_t kt = k_tiles(K);
+  dev::griddep_launch();
+  dev::griddep_wait();
+  if (row >= M) return;
+  const uint32_t* qr = reinterpret_cast<const uint32_t*>(data + row * (K >> 1));
+  uint32_t w[VPT], s[VPT];
+#pragma unroll
+  for (int j = 0; j < VPT; ++j) {
+    const int vi = (g0 + j) * 32 + lane;
+    w[j] = vi < nvec ? qr[vi] : 0u;
+    s[j] = vi < nvec ? scales[scale_offset(row, vi >> 4, kt) + ((vi >> 2) & 3)] : 0u;
+  }
+#pragma unroll
+  for (int j = 0; j < VPT; ++j) {
+    const int vi = (g0 + j) * 32 + lane;
+    if (vi >= nvec) break;
+    // 2^(s - 127): a subnormal for s = 0, NaN for s = 255
+    const float f = s[j] == kNanScale ? __uint_as_float(0x7fffffffu)
+                    : s[j] == 0       ? __uint_as_float(0x00400000u)
+                                      : __uint_as_float(s[j] << 23);
+    float v[8];
+#pragma unroll
+    for (int b = 0; b < 4; ++b) {
+      uint32_t h;
+      asm("{\n\t.reg .b8 t;\n\tcvt.u8.u32 t, %1;\n\tcvt.rn.f16x2.e2m1x2 %0, t;\n\t}"
+          : "=r"(h)
+          : "r"((w[j] >> (8 * b)) & 255u));
+      const float2 p = __half22float2(reinterpret_cast<const __half2&>(h));
+      v[2 * b] = p.x * f;
+      v[2 * b + 1] = p.y * f;
+    }
+    store8(out + row * K + static_cast<int64_t>(vi) * 8, v);
+  }
+}
+
+// -------------------------------------------------------------------- host
+int check_shape(const char* what, int64_t M, int64_t K) {
+  W8A8_REQUIRE(M >= 0 && K >= 0, W8A8_ERR_INVALID_ARG, "%s: negative shape", what);
+  W8A8_REQUIRE(K > 0 && K % kBlock == 0, W8A8_ERR_INVALID_ARG, "%s: the last dimension (%lld) must be a positive multiple of 32",
+               what, (long long)K);
+  W8A8_REQUIRE(K <= (1LL << 30) && M <= (1LL << 30), W8A8_ERR_UNSUPPORTED, "%s: shape too large", what);
+  return W8A8_OK;
+}
+
+int check_device(const char* what) {
+  W8A8_REQUIRE(device_cc_major() == 10, W8A8_ERR_UNSUPPORTED,
+               "%s: the kernels need an sm_100 (B200) device; found compute capability %d.x", what, device_cc_major());
+  return W8A8_OK;
+}
+
+// Groups of 256 values per warp: 4 (64 bytes in flight per lane) once that
+// still gives every SM 16 warps, else 1.
+int pick_vpt(int64_t M, int64_t K) {
+  const int64_t groups = M * ((K + 255) / 256);
+  return groups >= 4 * 16 * static_cast<int64_t>(sm_count()) ? 4 : 1;
+}
+
+int grid_of(const char* what, int64_t M, int64_t K, int vpt, int* segs, unsigned* grid) {
+  const int64_t groups = (K + 255) / 256;
+  *segs = static_cast<int>((groups + vpt - 1) / vpt);
+  const int64_t ctas = (M * *segs + kThreads / 32 - 1) / (kThreads / 32);
+  W8A8_REQUIRE(ctas <= 0x7fffffffLL, W8A8_ERR_UNSUPPORTED, "%s: %lld x %lld is too large for one launch", what,
+               (long long)M, (long long)K);
+  *grid = static_cast<unsigned>(ctas);
+  return W8A8_OK;
+}
+
+template <typename T>
+int run_quant(const void* x, int64_t ldx, uint8_t* data, uint8_t* scales, int64_t M, int64_t K, cudaStream_t s) {
+  const int vpt = pick_vpt(M, K);
+  int segs;
+  unsigned grid;
+  if (int rc = grid_of("mxfp4_quant", M, K, vpt, &segs, &grid)) return rc;
+  auto kern = vpt == 4 ? quant_kernel<T, 4> : quant_kernel<T, 1>;
+  W8A8_CUDA_TRY(launch_pdl(kern, dim3(grid), dim3(kThreads), 0, s, static_cast<const T*>(x), ldx, data, scales, M,
+                           static_cast<int>(K), segs));
+  return W8A8_OK;
+}
+
+template <typename T>
+int run_silu(const void* gu, int64_t ld, uint8_t* data, uint8_t* scales, int64_t M, int64_t I, cudaStream_t s) {
+  const int vpt = pick_vpt(M, I) == 4 ? 2 : 1;
+  int segs;
+  unsigned grid;
+  if (int rc = grid_of("mxfp4_silu_mul_quant", M, I, vpt, &segs, &grid)) return rc;
+  auto kern = vpt == 2 ? silu_kernel<T, 2> : silu_kernel<T, 1>;
+  W8A8_CUDA_TRY(launch_pdl(kern, dim3(grid), dim3(kThreads), 0, s, static_cast<const T*>(gu), ld, data, scales, M,
+                           static_cast<int>(I), segs));
+  return W8A8_OK;
+}
+
+template <typename T, bool ADD>
+int run_norm(const void* x, int64_t ldx, void* residual, int64_t ldr, const void* weight, float eps, uint8_t* data,
+             uint8_t* scales, int64_t M, int64_t K, cudaStream_t s) {
+  const int nvec = static_cast<int>(K / 8);
+  const int vpt = nvec <= kNormMaxThreads ? 1 : nvec <= 2 * kNormMaxThreads ? 2 : 4;
+  const int threads = ((nvec + vpt - 1) / vpt + 31) / 32 * 32;
+  auto kern = vpt == 1 ? rmsnorm_kernel<T, 1, ADD> : vpt == 2 ? rmsnorm_kernel<T, 2, ADD> : rmsnorm_kernel<T, 4, ADD>;
+  W8A8_CUDA_TRY(launch_pdl(kern, dim3(static_cast<unsigned>(M)), dim3(threads), 0, s, static_cast<const T*>(x), ldx,
+                           static_cast<T*>(residual), ldr, static_cast<const T*>(weight), eps, data, scales, M,
+                           static_cast<int>(K)));
+  return W8A8_OK;
+}
+
+template <typename O>
+int run_dequant(const uint8_t* data, const uint8_t* scales, void* out, int64_t M, int64_t K, cudaStream_t s) {
+  const int vpt = pick_vpt(M, K);
+  int segs;
+  unsigned grid;
+  if (int rc = grid_of("mxfp4_dequant", M, K, vpt, &segs, &grid)) return rc;
+  auto kern = vpt == 4 ? dequant_kernel<O, 4> : dequant_kernel<O, 1>;
+  W8A8_CUDA_TRY(launch_pdl(kern, dim3(grid), dim3(kThreads), 0, s, data, scales, static_cast<O*>(out), M,
+                           static_cast<int>(K), segs));
+  return W8A8_OK;
+}
+
+}  // namespace
+}  // namespace mx
+}  // namespace w8a8
+
+extern "C" {
+
+int64_t mxfp4_scale_bytes(int64_t rows, int64_t K) {
+  if (rows < 0 || K <= 0 || K % w8a8::mx::kBlock) return 0;
+  return w8a8::mx::row_tiles(rows) * w8a8::mx::k_tiles(K) * w8a8::mx::kTileBytes;
+}
+
+int mxfp4_quant(const void* x, int64_t ldx, int dtype, uint8_t* data, uint8_t* scales, int64_t M, int64_t K,
+                void* stream) {
+  using namespace w8a8;
+  if (M == 0) return W8A8_OK;
+  if (int rc = mx::check_shape("mxfp4_quant", M, K)) return rc;
+  W8A8_REQUIRE(x && data && scales, W8A8_ERR_INVALID_ARG, "mxfp4_quant: null pointer");
+  W8A8_REQUIRE(dtype == mx::kBf16 || dtype == mx::kFp16, W8A8_ERR_INVALID_ARG, "mxfp4_quant: bf16 or fp16 input");
+  W8A8_REQUIRE(ldx >= K && ldx % 8 == 0, W8A8_ERR_INVALID_ARG, "mxfp4_quant: the row stride must be a multiple of 8, at least K");
+  W8A8_REQUIRE(W8A8_ALIGNED16(x) && W8A8_ALIGNED16(data) && W8A8_ALIGNED16(scales), W8A8_ERR_ALIGNMENT,
+               "mxfp4_quant: pointers must be 16-byte aligned");
+  if (int rc = mx::check_device("mxfp4_quant")) return rc;
+  auto s = static_cast<cudaStream_t>(stream);
+  return dtype == mx::kBf16 ? mx::run_quant<__nv_bfloat16>(x, ldx, data, scales, M, K, s)
+                            : mx::run_quant<__half>(x, ldx, data, scales, M, K, s);
+}
+
+int mxfp4_dequant(const uint8_t* data, const uint8_t* scales, void* out, int dtype, int64_t M, int64_t K,
+                  void* stream) {
+  using namespace w8a8;
+  if (M == 0) return W8A8_OK;
+  if (int rc = mx::check_shape("mxfp4_dequant", M, K)) return rc;
+  W8A8_REQUIRE(data && scales && out, W8A8_ERR_INVALID_ARG, "mxfp4_dequant: null pointer");
+  W8A8_REQUIRE(dtype >= mx::kBf16 && dtype <= mx::kFp32, W8A8_ERR_INVALID_ARG, "mxfp4_dequant: bf16, fp16 or fp32 output");
+  W8A8_REQUIRE(W8A8_ALIGNED16(data) && W8A8_ALIGNED16(scales) && W8A8_ALIGNED16(out), W8A8_ERR_ALIGNMENT,
+               "mxfp4_dequant: pointers must be 16-byte aligned");
+  if (int rc = mx::check_device("mxfp4_dequant")) return rc;
+  auto s = static_cast<cudaStream_t>(stream);
+  switch (dtype) {
+    case mx::kBf16: return mx::run_dequant<__nv_bfloat16>(data, scales, out, M, K, s);
+    case mx::kFp16: return mx::run_dequant<__half>(data, scales, out, M, K, s);
+    default: return mx::run_dequant<float>(data, scales, out, M, K, s);
+  }
+}
+
+int mxfp4_silu_mul_quant(const void* gate_up, int64_t ld, int dtype, uint8_t* data, uint8_t* scales, int64_t M,
+                         int64_t I, void* stream) {
+  using namespace w8a8;
+  if (M == 0) return W8A8_OK;
+  if (int rc = mx::check_shape("mxfp4_silu_mul_quant", M, I)) return rc;
+  W8A8_REQUIRE(gate_up && data && scales, W8A8_ERR_INVALID_ARG, "mxfp4_silu_mul_quant: null pointer");
+  W8A8_REQUIRE(dtype == mx::kBf16 || dtype == mx::kFp16, W8A8_ERR_INVALID_ARG,
+               "mxfp4_silu_mul_quant: bf16 or fp16 input");
+  W8A8_REQUIRE(ld >= 2 * I && ld % 8 == 0, W8A8_ERR_INVALID_ARG,
+               "mxfp4_silu_mul_quant: the row stride must be a multiple of 8, at least 2I");
+  W8A8_REQUIRE(W8A8_ALIGNED16(gate_up) && W8A8_ALIGNED16(data) && W8A8_ALIGNED16(scales), W8A8_ERR_ALIGNMENT,
+               "mxfp4_silu_mul_quant: pointers must be 16-byte aligned");
+  if (int rc = mx::check_device("mxfp4_silu_mul_quant")) return rc;
+  auto s = static_cast<cudaStream_t>(stream);
+  return dtype == mx::kBf16 ? mx::run_silu<__nv_bfloat16>(gate_up, ld, data, scales, M, I, s)
+                            : mx::run_silu<__half>(gate_up, ld, data, scales, M, I, s);
+}
+
+int mxfp4_rmsnorm_quant(const void* x, int64_t ldx, void* residual, int64_t ldr, const void* weight, float eps,
+                        int dtype, uint8_t* data, uint8_t* scales, int64_t M, int64_t K, void* stream) {
+  using namespace w8a8;
+  if (M == 0) return W8A8_OK;
+  if (int rc = mx::check_shape("mxfp4_rmsnorm_quant", M, K)) return rc;
+  W8A8_REQUIRE(x && weight && data && scales, W8A8_ERR_INVALID_ARG, "mxfp4_rmsnorm_quant: null pointer");
+  W8A8_REQUIRE(dtype == mx::kBf16 || dtype == mx::kFp16, W8A8_ERR_INVALID_ARG,
+               "mxfp4_rmsnorm_quant: bf16 or fp16 input");
+  W8A8_REQUIRE(K <= 32768, W8A8_ERR_UNSUPPORTED, "mxfp4_rmsnorm_quant: K=%lld is above 32768", (long long)K);
+  W8A8_REQUIRE(ldx >= K && ldx % 8 == 0 && (!residual || (ldr >= K && ldr % 8 == 0)), W8A8_ERR_INVALID_ARG,
+               "mxfp4_rmsnorm_quant: row strides must be multiples of 8, at least K");
+  W8A8_REQUIRE(eps >= 0.0f && eps < 1e30f, W8A8_ERR_INVALID_ARG, "mxfp4_rmsnorm_quant: eps must be finite and not negative");
+  W8A8_REQUIRE(W8A8_ALIGNED16(x) && W8A8_ALIGNED16(residual) && W8A8_ALIGNED16(weight) && W8A8_ALIGNED16(data) &&
+                   W8A8_ALIGNED16(scales),
+               W8A8_ERR_ALIGNMENT, "mxfp4_rmsnorm_quant: pointers must be 16-byte aligned");
+  if (int rc = mx::check_device("mxfp4_rmsnorm_quant")) return rc;
+  auto s = static_cast<cudaStream_t>(stream);
+  if (dtype == mx::kBf16)
+    return residual ? mx::run_norm<__nv_bfloat16, true>(x, ldx, residual, ldr, weight, eps, data, scales, M, K, s)
+                    : mx::run_norm<__nv_bfloat16, false>(x, ldx, residual, ldr, weight, eps, data, scales, M, K, s);
+  return residual ? mx::run_norm<__half, true>(x, ldx, residual, ldr, weight, eps, data, scales, M, K, s)
+                  : mx::run_norm<__half, false>(x, ldx, residual, ldr, weight, eps, data, scales, M, K, s);
+}
+
+}  // extern "C"

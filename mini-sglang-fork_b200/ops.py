@@ -1,4 +1,5 @@
-"""Torch-facing wrappers of the C ABI (``include/w8a8_tp.h``).
+"""Torch-facing wrappers of the C ABI (``include/w8a8_tp.h``,
+``include/mxfp4.h``).
 
 Every op launches hand-written sm_100a CUDA through ``_w8a8_tp.so`` on the
 caller's current CUDA stream.  There is no CPU or library fallback: a
@@ -35,6 +36,16 @@ __all__ = [
     "moe_quant_rows",
     "moe_sum",
     "fused_experts_w8a8",
+    "MXFP4Tensor",
+    "mxfp4_scale_shape",
+    "mxfp4_tile_scales",
+    "mxfp4_plain_scales",
+    "mxfp4_quant",
+    "mxfp4_dequant",
+    "mxfp4_silu_and_mul_quant",
+    "mxfp4_rmsnorm_quant",
+    "mxfp4_gemm",
+    "mxfp4_gate_up_silu_quant",
 ]
 
 # Split-K workspace kept per device (zeroed once, left zeroed by every call).
@@ -471,6 +482,238 @@ def fused_experts_w8a8(x: torch.Tensor, w1q: torch.Tensor, sw1: torch.Tensor, w2
     qy = moe_quant_rows(y, amax, routing)
     c3 = moe_gemm(qy.q, qy.s, w2q, sw2, routing, route_w=topk_weights)
     return moe_sum(c3, routing, out)
+
+
+# ---------------------------------------------------------------------------
+# microscaled 4-bit (MXFP4): quantisers, product, gated MLP
+# ---------------------------------------------------------------------------
+_MX_DTYPE = {torch.bfloat16: 0, torch.float16: 1, torch.float32: 2}
+
+
+def mxfp4_scale_shape(rows: int, k: int) -> Tuple[int, int, int]:
+    """Shape of the scale tiles of an MXFP4 ``[rows, k]`` matrix: 512-byte
+    tiles of 128 rows x 4 blocks, K padded to 256 values."""
+    return (rows + 127) // 128, 2 * ((k + 255) // 256), 512
+
+
+class MXFP4Tensor:
+    """A microscaled 4-bit matrix ``[R, K]``: ``data [R, K/2]`` uint8 (two
+    E2M1 codes per byte, even column low) and ``scales``, the E8M0 bytes of its
+    32-value blocks in tiles of :func:`mxfp4_scale_shape` (row r, block c of a
+    tile at ``(r % 32) * 16 + (r // 32) * 4 + c``).  The product of
+    :func:`mxfp4_quant` and its fused forms, an operand of :func:`mxfp4_gemm`,
+    and accepted by the MXFP4 layers in place of a 16-bit activation."""
+
+    __slots__ = ("data", "scales", "shape")
+
+    def __init__(self, data: torch.Tensor, scales: torch.Tensor):
+        if data.dtype != torch.uint8 or data.dim() != 2 or not data.is_contiguous() or data.shape[1] % 16:
+            raise _lib.W8A8Error(_lib.ERR_INVALID_ARG, "MXFP4Tensor: data must be contiguous uint8 [R, K/2], K % 32 == 0")
+        r, half = data.shape
+        if (scales.dtype != torch.uint8 or not scales.is_contiguous()
+                or tuple(scales.shape) != mxfp4_scale_shape(r, 2 * half)):
+            raise _lib.W8A8Error(_lib.ERR_INVALID_ARG, f"MXFP4Tensor: scales must be contiguous uint8 tiles "
+                                 f"{mxfp4_scale_shape(r, 2 * half)}, got {scales.dtype} {tuple(scales.shape)}")
+        if scales.device != data.device:
+            raise _lib.W8A8Error(_lib.ERR_INVALID_ARG, f"MXFP4Tensor: data on {data.device}, scales on {scales.device}")
+        self.data = data
+        self.scales = scales
+        self.shape = torch.Size((r, 2 * half))
+
+    @property
+    def device(self):
+        return self.data.device
+
+
+def mxfp4_tile_scales(scales: torch.Tensor) -> torch.Tensor:
+    """Plain E8M0 bytes ``[R, K/32]`` (a checkpoint's order) to scale tiles."""
+    if scales.dtype != torch.uint8 or scales.dim() != 2:
+        raise _lib.W8A8Error(_lib.ERR_INVALID_ARG, "mxfp4_tile_scales: scales must be uint8 [R, K/32]")
+    r, c = scales.shape
+    rt, kt, _ = mxfp4_scale_shape(r, 32 * c)
+    padded = scales.new_zeros(128 * rt, 4 * kt)
+    padded[:r, :c] = scales
+    return padded.view(rt, 4, 32, kt, 4).permute(0, 3, 2, 1, 4).reshape(rt, kt, 512)
+
+
+def mxfp4_plain_scales(t: MXFP4Tensor) -> torch.Tensor:
+    """The E8M0 bytes ``[R, K/32]`` of an :class:`MXFP4Tensor`, row by row."""
+    rt, kt, _ = t.scales.shape
+    r, k = t.shape
+    plain = t.scales.view(rt, kt, 32, 4, 4).permute(0, 3, 2, 1, 4).reshape(128 * rt, 4 * kt)
+    return plain[:r, :k // 32].contiguous()
+
+
+class _OnDevice:
+    """Makes a tensor's device current around a launch when it is not."""
+
+    __slots__ = ("idx", "prev")
+
+    def __init__(self, t: torch.Tensor):
+        self.idx = t.device.index
+
+    def __enter__(self):
+        self.prev = torch.cuda.current_device()
+        if self.prev != self.idx:
+            torch.cuda.set_device(self.idx)
+
+    def __exit__(self, *exc):
+        if self.prev != self.idx:
+            torch.cuda.set_device(self.prev)
+
+
+def _check_mx_input(name: str, what: str, x: torch.Tensor) -> int:
+    """A 2-D 16-bit CUDA activation with unit column stride; its dtype code.
+    (A row stride of 0 or below K, as an expanded or overlapping view has, is
+    refused: only separate rows are read and, for a residual, written.)"""
+    _require_cuda(name, x)
+    if x.dtype not in (torch.bfloat16, torch.float16) or x.dim() != 2 or (x.shape[1] > 1 and x.stride(1) != 1):
+        raise _lib.W8A8Error(_lib.ERR_INVALID_ARG,
+                             f"{name}: {what} must be a 2-D bf16 or fp16 tensor with unit column stride")
+    return _MX_DTYPE[x.dtype]
+
+
+def _row_stride(x: torch.Tensor) -> int:
+    """Row stride of a 2-D tensor; the width where there is no second row (a
+    single row's stride is arbitrary)."""
+    return x.stride(0) if x.shape[0] > 1 else (x.shape[1] + 7) // 8 * 8
+
+
+def _mx_empty(rows: int, k: int, device: torch.device) -> MXFP4Tensor:
+    if k <= 0 or k % 32:
+        raise _lib.W8A8Error(_lib.ERR_INVALID_ARG, f"MXFP4: the last dimension ({k}) must be a positive multiple of 32")
+    t = MXFP4Tensor.__new__(MXFP4Tensor)
+    t.data = torch.empty(rows, k // 2, dtype=torch.uint8, device=device)
+    t.scales = torch.empty(mxfp4_scale_shape(rows, k), dtype=torch.uint8, device=device)
+    t.shape = torch.Size((rows, k))
+    return t
+
+
+def mxfp4_quant(x: torch.Tensor) -> MXFP4Tensor:
+    """``x [M, K]`` bf16 or fp16 to MXFP4: per 32 values the scale
+    ``2^(floor(log2 amax) - 2)``, values rounded to the nearest E2M1 number
+    (ties to even, saturating at 6).  A block with an infinity or a NaN gets
+    the NaN scale.  Rows may be strided (multiples of 8); K % 32 == 0."""
+    dt = _check_mx_input("mxfp4_quant", "x", x)
+    m, k = x.shape
+    q = _mx_empty(m, k, x.device)
+    with _OnDevice(x):
+        _lib.check(_lib.load().mxfp4_quant(_ptr(x), _row_stride(x), dt, _ptr(q.data), _ptr(q.scales), m, k,
+                                           _stream(x)), "mxfp4_quant")
+    return q
+
+
+def mxfp4_dequant(q: MXFP4Tensor, dtype: torch.dtype = torch.bfloat16) -> torch.Tensor:
+    """The values of an :class:`MXFP4Tensor` as a contiguous bf16, fp16 or fp32
+    tensor (exact in bf16 and fp32; a NaN-scaled block is NaN)."""
+    if dtype not in _MX_DTYPE:
+        raise _lib.W8A8Error(_lib.ERR_INVALID_ARG, f"mxfp4_dequant: bf16, fp16 or fp32, not {dtype}")
+    _require_cuda("mxfp4_dequant", q.data)
+    m, k = q.shape
+    out = torch.empty(m, k, dtype=dtype, device=q.device)
+    with _OnDevice(q.data):
+        _lib.check(_lib.load().mxfp4_dequant(_ptr(q.data), _ptr(q.scales), _ptr(out), _MX_DTYPE[dtype], m, k,
+                                             _stream(out)), "mxfp4_dequant")
+    return out
+
+
+def mxfp4_silu_and_mul_quant(gate_up: torch.Tensor) -> MXFP4Tensor:
+    """``silu(gate) * up`` of ``gate_up [M, 2I]`` bf16 or fp16 to MXFP4 ``[M,
+    I]``, the product not rounded in between (values next to a rounding border
+    are evaluated in 64 bits).  I % 32 == 0."""
+    dt = _check_mx_input("mxfp4_silu_and_mul_quant", "gate_up", gate_up)
+    m, two_i = gate_up.shape
+    if two_i % 2:
+        raise _lib.W8A8Error(_lib.ERR_INVALID_ARG, "mxfp4_silu_and_mul_quant: last dim must be even")
+    q = _mx_empty(m, two_i // 2, gate_up.device)
+    with _OnDevice(gate_up):
+        _lib.check(_lib.load().mxfp4_silu_mul_quant(_ptr(gate_up), _row_stride(gate_up), dt, _ptr(q.data),
+                                                    _ptr(q.scales), m, two_i // 2, _stream(gate_up)),
+                   "mxfp4_silu_and_mul_quant")
+    return q
+
+
+def mxfp4_rmsnorm_quant(x: torch.Tensor, weight: torch.Tensor, eps: float,
+                        residual: Optional[torch.Tensor] = None) -> Tuple[MXFP4Tensor, torch.Tensor]:
+    """RMSNorm (after ``x + residual`` when a residual is given, updating the
+    residual in place, as :func:`rmsnorm_quant` does) to MXFP4, the normalised
+    row not rounded in between.  Returns ``(MXFP4Tensor, residual)``; the
+    residual is ``x`` itself without one.  bf16 or fp16, K % 32 == 0, K <=
+    32768."""
+    dt = _check_mx_input("mxfp4_rmsnorm_quant", "x", x)
+    m, k = x.shape
+    if weight.dtype != x.dtype or weight.shape != (k,) or not weight.is_contiguous():
+        raise _lib.W8A8Error(_lib.ERR_INVALID_ARG, "mxfp4_rmsnorm_quant: weight must be a contiguous [K] vector of x's type")
+    if residual is not None and (residual.dtype != x.dtype or residual.shape != x.shape
+                                 or (k > 1 and residual.stride(1) != 1)):
+        raise _lib.W8A8Error(_lib.ERR_INVALID_ARG,
+                             "mxfp4_rmsnorm_quant: residual must match x (shape, type, unit column stride)")
+    _require_cuda("mxfp4_rmsnorm_quant", weight, residual)
+    _one_device("mxfp4_rmsnorm_quant", x, weight, residual)
+    q = _mx_empty(m, k, x.device)
+    with _OnDevice(x):
+        _lib.check(_lib.load().mxfp4_rmsnorm_quant(
+            _ptr(x), _row_stride(x), _ptr(residual), _row_stride(residual) if residual is not None else k,
+            _ptr(weight), float(eps), dt, _ptr(q.data), _ptr(q.scales), m, k, _stream(x)), "mxfp4_rmsnorm_quant")
+    return q, residual if residual is not None else x
+
+
+def _check_mx_gemm(name: str, a: MXFP4Tensor, w: MXFP4Tensor, bias: Optional[torch.Tensor],
+                   dtype: torch.dtype) -> None:
+    if dtype not in (torch.bfloat16, torch.float16):
+        raise _lib.W8A8Error(_lib.ERR_INVALID_ARG, f"{name}: bf16 or fp16, not {dtype}")
+    if a.shape[1] != w.shape[1]:
+        raise _lib.W8A8Error(_lib.ERR_INVALID_ARG, f"{name}: shape mismatch A{tuple(a.shape)} B{tuple(w.shape)}")
+    if bias is not None and (bias.dtype != dtype or bias.shape != (w.shape[0],) or not bias.is_contiguous()):
+        raise _lib.W8A8Error(_lib.ERR_INVALID_ARG, f"{name}: bias must be contiguous {dtype} [{w.shape[0]}]")
+    _require_cuda(name, a.data, w.data, bias)
+    _one_device(name, a.data, w.data, bias)
+
+
+def mxfp4_gemm(a: MXFP4Tensor, w: MXFP4Tensor, bias: Optional[torch.Tensor] = None,
+               out: Optional[torch.Tensor] = None, out_dtype: torch.dtype = torch.bfloat16) -> torch.Tensor:
+    """``a [M, K] @ w [N, K]^T (+ bias [N])`` on the block-scaled tensor cores,
+    accumulated in fp32 and rounded once to ``out_dtype`` (bf16 or fp16; the
+    bias has it too, and ``out`` when given)."""
+    if out is not None:
+        out_dtype = out.dtype
+    _check_mx_gemm("mxfp4_gemm", a, w, bias, out_dtype)
+    m, k = a.shape
+    n = w.shape[0]
+    if out is None:
+        out = torch.empty(m, n, dtype=out_dtype, device=a.device)
+    else:
+        _require_cuda("mxfp4_gemm", out)
+        _one_device("mxfp4_gemm", a.data, out)
+        _check_2d("mxfp4_gemm out", out, out_dtype, (m, n))
+    with _OnDevice(out):
+        _lib.check(_lib.load().mxfp4_gemm(_ptr(a.data), _ptr(a.scales), _ptr(w.data), _ptr(w.scales), _ptr(bias),
+                                          _ptr(out), _MX_DTYPE[out_dtype], m, n, k, _stream(out)), "mxfp4_gemm")
+    return out
+
+
+def mxfp4_gate_up_silu_quant(a: MXFP4Tensor, w: MXFP4Tensor, bias: Optional[torch.Tensor] = None,
+                             dtype: torch.dtype = torch.bfloat16) -> MXFP4Tensor:
+    """The gated half of an MLP in MXFP4: ``w [2I, K]`` is the merged [gate;
+    up] weight, the result MXFP4 ``silu(a gate^T) * (a up^T)``, ``[M, I]``.
+    With I % 128 == 0 one kernel forms it from the fp32 sums and nothing of the
+    [M, 2I] product reaches memory; otherwise :func:`mxfp4_gemm` (rounding to
+    ``dtype``) and :func:`mxfp4_silu_and_mul_quant` run.  ``dtype`` is also the
+    bias's type.  I % 32 == 0."""
+    _check_mx_gemm("mxfp4_gate_up_silu_quant", a, w, bias, dtype)
+    m, k = a.shape
+    i, odd = divmod(w.shape[0], 2)
+    if odd or i % 32:
+        raise _lib.W8A8Error(_lib.ERR_INVALID_ARG,
+                             f"mxfp4_gate_up_silu_quant: {w.shape[0]} weight rows are not [gate; up] of a multiple of 32")
+    if i % 128:
+        return mxfp4_silu_and_mul_quant(mxfp4_gemm(a, w, bias, out_dtype=dtype))
+    y = _mx_empty(m, i, a.device)
+    with _OnDevice(a.data):
+        _lib.check(_lib.load().mxfp4_gemm_silu_quant(_ptr(a.data), _ptr(a.scales), _ptr(w.data), _ptr(w.scales),
+                                                     _ptr(bias), _MX_DTYPE[dtype], _ptr(y.data), _ptr(y.scales),
+                                                     m, i, k, _stream(a.data)), "mxfp4_gate_up_silu_quant")
+    return y
 
 
 # The stream-K counter region at the head of a GEMM workspace (65536 tile
