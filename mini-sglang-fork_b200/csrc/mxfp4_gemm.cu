@@ -5,7 +5,7 @@
 #include <mutex>
 
 #include "gemm_api.h"
-#include "mxfp4_sm100.cuh"
+#include "mxfp4_pair_sm100.cuh"
 
 namespace w8a8 {
 namespace mx {
@@ -44,14 +44,14 @@ int launch_row(const Operands& o, MxGemmArgs args, cudaStream_t stream) {
   using P = MxRowTraits<T, SILU>;
   constexpr auto kern = mx_row_kernel<O, T, SILU>;
   if (int rc = allow_smem<kern>(P::kSmemBytes)) return rc;
-  args.wtiles = (args.N + 127) / 128;
+  const int64_t wtiles = (args.N + 127) / 128;
   args.ttiles = (args.M + T - 1) / T;
   CUtensorMap tw, tws, tx, txs;
   if (int rc = encode_operand(&tw, o.b, o.b_rows, args.K / 2, 128)) return rc;
   if (int rc = encode_words(&tws, o.bs, row_tiles(o.b_rows), k_tiles(args.K) * kTileBytes / 4, 256)) return rc;
   if (int rc = encode_operand(&tx, o.a, args.M, args.K / 2, T)) return rc;
   if (int rc = encode_words(&txs, o.as, row_tiles(args.M), k_tiles(args.K) * kTileBytes / 4, 256)) return rc;
-  const int64_t tiles = static_cast<int64_t>(args.wtiles) * args.ttiles;
+  const int64_t tiles = wtiles * args.ttiles;
   const int split = tiles > 4096 ? 1 : pick_split(static_cast<int>(tiles), args.kblocks, sm_count());
   W8A8_REQUIRE(tiles * split <= 0x7fffffffLL, W8A8_ERR_UNSUPPORTED, "mxfp4_gemm: too many output tiles");
   cudaLaunchConfig_t cfg = {};
@@ -73,7 +73,31 @@ int launch_row(const Operands& o, MxGemmArgs args, cudaStream_t stream) {
 }
 
 template <typename O, bool SILU>
+int launch_pair(const Operands& o, const MxGemmArgs& g, cudaStream_t stream) {
+  constexpr auto kern = mx_pair_kernel<O, SILU>;
+  if (int rc = allow_smem<kern>(PairTraits::kSmemBytes)) return rc;
+  PairArgs args;
+  args.g = g;
+  args.pairs_m = (g.M + 255) / 256;
+  args.tiles_n = SILU ? g.N / 128 : (g.N + 255) / 256;
+  const int64_t blocks = static_cast<int64_t>(args.pairs_m) * args.tiles_n;
+  // (the block counter runs one grid past the last block)
+  W8A8_REQUIRE(blocks <= 0x7fff0000LL, W8A8_ERR_UNSUPPORTED, "mxfp4_gemm: too many output tiles");
+  CUtensorMap ta, tas, tb, tbs;
+  if (int rc = encode_operand(&ta, o.a, g.M, g.K / 2, 128)) return rc;
+  if (int rc = encode_words(&tas, o.as, row_tiles(g.M), k_tiles(g.K) * kTileBytes / 4, 256)) return rc;
+  if (int rc = encode_operand(&tb, o.b, o.b_rows, g.K / 2, 128)) return rc;
+  if (int rc = encode_words(&tbs, o.bs, row_tiles(o.b_rows), k_tiles(g.K) * kTileBytes / 4, 256)) return rc;
+  const int pairs = static_cast<int>(std::min<int64_t>(blocks, std::max(1, sm_count() / 2)));
+  W8A8_CUDA_TRY(launch_pdl(kern, dim3(2 * pairs), dim3(PairTraits::kThreads), PairTraits::kSmemBytes, stream, ta, tas,
+                           tb, tbs, args));
+  return W8A8_OK;
+}
+
+template <typename O, bool SILU>
 int dispatch(const Operands& o, const MxGemmArgs& args, cudaStream_t stream) {
+  const int64_t blocks = static_cast<int64_t>((args.M + 255) / 256) * (SILU ? args.N / 128 : (args.N + 255) / 256);
+  if (args.M > 128 && 2 * blocks >= sm_count() / 2) return launch_pair<O, SILU>(o, args, stream);
   if (args.M <= 16) return launch_row<O, 16, SILU>(o, args, stream);
   if (args.M <= 32) return launch_row<O, 32, SILU>(o, args, stream);
   if (args.M <= 64) return launch_row<O, 64, SILU>(o, args, stream);

@@ -1,0 +1,372 @@
+// MXFP4 GEMM for prefill: 256 x 256 output blocks on SM pairs.
+//
+// A cluster of two CTAs shares one tcgen05.mma.cta_group::2 (M = 256, N = 256,
+// 64 values of K): CTA h stages rows [128h, 128h + 128) of A and of B and the
+// scales of its A rows and of all 256 B rows, 35 KB per 256-value k block; the
+// even CTA issues the scale copies and the MMAs, which work on both CTAs'
+// shared memory and TMEM.  At the fp4 rate a pair needs 64 operand bytes per
+// clock and SM, which is about what the L2 gives; any smaller block would be
+// bound by that.
+//
+// Two 256-column accumulators and the scales do not fit TMEM's 512 columns, so
+// the accumulators overlap by 64: accumulator 0 is columns [0, 256),
+// accumulator 1 [192, 448), the scales of two k blocks [448, 512).  The
+// epilogue reads the 64 shared columns first and releases them; the next
+// block's MMAs wait for those only, while the rest is still being read.
+#pragma once
+
+#include "mxfp4_sm100.cuh"
+
+namespace w8a8 {
+namespace mx {
+
+struct PairTraits {
+  static constexpr int kStages = 5;
+  static constexpr int kTile = 128 * 128;  // bytes of 128 rows of a k block
+  static constexpr int kSf = 1024;
+  static constexpr int kStageBytes = 2 * kTile + 3 * kSf;
+  static constexpr int kEpiWarps = 8;
+  static constexpr int kThreads = 32 * (2 + kEpiWarps);
+  static constexpr int kAccStep = 192;  // columns from accumulator 0 to accumulator 1
+  static constexpr int kSfCol = 448;    // two buffers of 32 columns (A 8, B 16)
+  static constexpr int kBarrierBytes = 256;
+  static constexpr int kStagingBytes = kEpiWarps * 2048;
+  static constexpr int kSmemBytes = 1024 + kStages * kStageBytes + kBarrierBytes + kStagingBytes;
+  static_assert(kSmemBytes <= 227 * 1024, "shared memory");
+  // 512 TMEM columns: no other CTA with TMEM may share the SM (MxRowTraits)
+  static_assert(kSmemBytes >= 120 * 1024, "one CTA per SM");
+};
+
+__device__ __forceinline__ void cp_scales_pair(uint32_t taddr, uint64_t sdesc) {
+  asm volatile("tcgen05.cp.cta_group::2.32x128b.warpx4 [%0], %1;" ::"r"(taddr), "l"(sdesc) : "memory");
+}
+
+__device__ __forceinline__ void mma_mxf4_pair(uint32_t d_tmem, uint64_t adesc, uint64_t bdesc, uint32_t idesc,
+                                              uint32_t sfa, uint32_t sfb, uint32_t accumulate) {
+  asm volatile(
+      "{\n\t.reg .pred p;\n\t"
+      "setp.ne.b32 p, %6, 0;\n\t"
+      "tcgen05.mma.cta_group::2.kind::mxf4.block_scale.scale_vec::2X [%0], %1, %2, %3, [%4], [%5], p;\n\t}" ::"r"(
+          d_tmem),
+      "l"(adesc), "l"(bdesc), "r"(idesc), "r"(sfa), "r"(sfb), "r"(accumulate)
+      : "memory");
+}
+
+struct PairArgs {
+  MxGemmArgs g;
+  int pairs_m;  // 256-row blocks of the output
+  int tiles_n;  // 256-column blocks (SiLU: 128 features)
+};
+
+// Block p -> (256-row block, column block): groups of up to 16 row blocks, the
+// row block running fastest, so that the pairs at work share a few column
+// blocks and a group's A (16 x 256 rows) stays in L2 while B streams past.
+__device__ __forceinline__ void pair_block(const PairArgs& a, int p, int& pm, int& tn) {
+  constexpr int kGroup = 16;
+  const int group = p / (kGroup * a.tiles_n);
+  const int first = group * kGroup;
+  const int rows = min(kGroup, a.pairs_m - first);
+  const int r = p - group * kGroup * a.tiles_n;
+  pm = first + r % rows;
+  tn = r / rows;
+}
+
+template <typename O, bool SILU>
+__global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(PairTraits::kThreads, 1)
+    mx_pair_kernel(const __grid_constant__ CUtensorMap tm_a, const __grid_constant__ CUtensorMap tm_as,
+                   const __grid_constant__ CUtensorMap tm_b, const __grid_constant__ CUtensorMap tm_bs,
+                   const PairArgs args) {
+  using P = PairTraits;
+  extern __shared__ __align__(1024) uint8_t smem_raw[];
+  uint8_t* smem = reinterpret_cast<uint8_t*>((reinterpret_cast<uintptr_t>(smem_raw) + 1023) & ~uintptr_t(1023));
+  uint8_t* s_a = smem;
+  uint8_t* s_b = s_a + P::kStages * P::kTile;
+  uint8_t* s_as = s_b + P::kStages * P::kTile;
+  uint8_t* s_bs = s_as + P::kStages * P::kSf;
+  uint64_t* bars = reinterpret_cast<uint64_t*>(s_bs + P::kStages * 2 * P::kSf);
+  uint64_t* full = bars;
+  uint64_t* empty = bars + P::kStages;
+  uint64_t* acc_full = bars + 2 * P::kStages;  // [2]
+  uint64_t* acc_free = acc_full + 2;           // the overlap of a block's accumulator has been read
+  uint64_t* drain = acc_free + 1;
+  uint32_t* tmem_slot = reinterpret_cast<uint32_t*>(drain + 1);
+  volatile int* abort_flag = reinterpret_cast<volatile int*>(tmem_slot + 1);
+  uint8_t* staging = reinterpret_cast<uint8_t*>(bars) + P::kBarrierBytes;
+
+  const int warp = threadIdx.x >> 5;
+  const int lane = threadIdx.x & 31;
+  const uint32_t half = dev::cluster_rank();  // 0 = leader
+  const int first = blockIdx.x >> 1;
+  const int step = gridDim.x >> 1;
+  const int blocks = args.pairs_m * args.tiles_n;
+  const MxGemmArgs& g = args.g;
+  const long long tmo = g.timeout_ns;
+
+  if (threadIdx.x == 0) {
+    for (int s = 0; s < P::kStages; ++s) {
+      dev::mbar_init(dev::smem_u32(full + s), 1);
+      dev::mbar_init(dev::smem_u32(empty + s), 1);
+    }
+    dev::mbar_init(dev::smem_u32(acc_full), 1);
+    dev::mbar_init(dev::smem_u32(acc_full + 1), 1);
+    dev::mbar_init(dev::smem_u32(acc_free), 2 * P::kEpiWarps);  // the epilogue warps of both CTAs
+    dev::mbar_init(dev::smem_u32(drain), 1);
+    *abort_flag = 0;
+    dev::fence_mbar_init();
+    dev::prefetch_tmap(&tm_a);
+    dev::prefetch_tmap(&tm_as);
+    dev::prefetch_tmap(&tm_b);
+    dev::prefetch_tmap(&tm_bs);
+  }
+  if (warp == 1) {
+    dev::tmem_alloc2(dev::smem_u32(tmem_slot), 512);
+    dev::tmem_relinquish2();
+  }
+  dev::tc_fence_before();
+  dev::cluster_sync();  // barriers of both CTAs initialised before any cross-CTA use
+  dev::tc_fence_after();
+  const uint32_t tmem = __shfl_sync(0xffffffffu, *tmem_slot, 0);  // (the same in every lane, and known to be)
+  dev::griddep_launch();
+  dev::griddep_wait();  // any operand may be the previous kernel's output
+
+  if (warp == 0) {
+    // ------------------------------------------------------------ producer
+    int stage = 0;
+    uint32_t phase = 0, issued_mask = 0, issued_phase = 0;
+    bool ok = true;
+    for (int p = first; ok && p < blocks; p += step) {
+      int pm, tn;
+      pair_block(args, p, pm, tn);
+      const int ta = 2 * pm + static_cast<int>(half);  // 128-row tile of A
+      // 128-row tiles of B: the block's two, or its gate rows and their up rows
+      const int tb0 = SILU ? tn : 2 * tn;
+      const int tb1 = SILU ? tn + (g.N >> 7) : 2 * tn + 1;
+      const int b_row = (half ? tb1 : tb0) * 128;
+      for (int kb = 0; kb < g.kblocks; ++kb) {
+        ok = warp_wait(dev::smem_u32(empty + stage), phase ^ 1u, abort_flag, g.err, tmo);
+        if (!ok) break;
+        if (elect_one()) {
+          const uint32_t bar = dev::mapa(dev::smem_u32(full + stage), 0);
+          if (half == 0) dev::mbar_expect_tx(dev::smem_u32(full + stage), 2 * P::kStageBytes);
+          dev::tma_load_2d_pair(dev::smem_u32(s_a + stage * P::kTile), &tm_a, bar, kb * 128, ta * 128);
+          dev::tma_load_2d_pair(dev::smem_u32(s_b + stage * P::kTile), &tm_b, bar, kb * 128, b_row);
+          dev::tma_load_2d_pair(dev::smem_u32(s_as + stage * P::kSf), &tm_as, bar, kb * 256, ta);
+          dev::tma_load_2d_pair(dev::smem_u32(s_bs + stage * 2 * P::kSf), &tm_bs, bar, kb * 256, tb0);
+          dev::tma_load_2d_pair(dev::smem_u32(s_bs + (stage * 2 + 1) * P::kSf), &tm_bs, bar, kb * 256, tb1);
+        }
+        __syncwarp();
+        issued_mask |= 1u << stage;
+        issued_phase = (issued_phase & ~(1u << stage)) | (phase << stage);
+        if (++stage == P::kStages) {
+          stage = 0;
+          phase ^= 1u;
+        }
+      }
+    }
+    // The leader's full barriers count both CTAs' bytes: once they have landed,
+    // no copy of either CTA is in flight (the pair then meets at the closing
+    // cluster barrier).
+    if (half == 0 && lane == 0)
+      for (int s = 0; s < P::kStages; ++s)
+        if (issued_mask & (1u << s))
+          if (!dev::mbar_wait_drain(dev::smem_u32(full + s), (issued_phase >> s) & 1u, tmo))
+            if (g.err) atomicOr(g.err, kErrGemmDrain);
+  } else if (warp == 1) {
+    if (half == 0) {
+      // --------------------------------------------- MMA issuer (leader only)
+      int stage = 0, stage2 = 0;  // this k block's stage, the one two k blocks back
+      uint32_t phase = 0, phase2 = 0;
+      uint32_t it = 0, blk = 0;
+      bool ok = true;
+      for (int p = first; ok && p < blocks; p += step, ++blk) {
+        if (blk > 0 && !__all_sync(0xffffffffu, dev::mbar_wait_cluster(dev::smem_u32(acc_free), (blk - 1) & 1u,
+                                                                       abort_flag, g.err, kErrGemmWait, tmo)))
+          break;
+        dev::tc_fence_after();
+        const uint32_t d = tmem + (blk & 1u) * P::kAccStep;
+        for (int kb = 0; kb < g.kblocks; ++kb, ++it) {
+          if (it >= 2) {  // the scale buffer's last readers are done
+            ok = warp_wait(dev::smem_u32(empty + stage2), phase2, abort_flag, g.err, tmo);
+            if (!ok) break;
+            if (++stage2 == P::kStages) {
+              stage2 = 0;
+              phase2 ^= 1u;
+            }
+          }
+          ok = warp_wait(dev::smem_u32(full + stage), phase, abort_flag, g.err, tmo);
+          if (!ok) break;
+          dev::tc_fence_after();
+          if (elect_one()) {
+            const uint32_t sfa = tmem + P::kSfCol + (it & 1u) * 32;
+            const uint32_t sfb = sfa + 8;
+#pragma unroll
+            for (int c = 0; c < 2; ++c) {
+              cp_scales_pair(sfa + 4 * c, sdesc_scales(dev::smem_u32(s_as + stage * P::kSf + c * kTileBytes)));
+              cp_scales_pair(sfb + 8 * c, sdesc_scales(dev::smem_u32(s_bs + stage * 2 * P::kSf + c * kTileBytes)));
+              cp_scales_pair(sfb + 8 * c + 4,
+                             sdesc_scales(dev::smem_u32(s_bs + (stage * 2 + 1) * P::kSf + c * kTileBytes)));
+            }
+            const uint64_t da = dev::sdesc_k_sw128(dev::smem_u32(s_a + stage * P::kTile));
+            const uint64_t db = dev::sdesc_k_sw128(dev::smem_u32(s_b + stage * P::kTile));
+            const int steps = min(4, (g.K - kb * 256 + 63) / 64);  // beyond K: nothing to add
+#pragma unroll
+            for (int k = 0; k < 4; ++k) {
+              if (k >= steps) break;
+              constexpr uint32_t ids[2] = {idesc_mxf4(256, 256, 0), idesc_mxf4(256, 256, 2)};
+              mma_mxf4_pair(d, da + 2 * k, db + 2 * k, ids[k & 1], sfa + 4 * (k >> 1), sfb + 8 * (k >> 1),
+                            (kb > 0 || k > 0) ? 1u : 0u);
+            }
+            dev::tc_commit_pair(dev::smem_u32(empty + stage));
+            dev::tc_commit_pair(dev::mapa(dev::smem_u32(empty + stage), 1));
+          }
+          __syncwarp();
+          if (++stage == P::kStages) {
+            stage = 0;
+            phase ^= 1u;
+          }
+        }
+        if (!ok) break;
+        if (elect_one()) {
+          dev::tc_commit_pair(dev::smem_u32(acc_full + (blk & 1u)));
+          dev::tc_commit_pair(dev::mapa(dev::smem_u32(acc_full + (blk & 1u)), 1));
+        }
+        __syncwarp();
+      }
+      if (elect_one()) dev::tc_commit_pair(dev::smem_u32(drain));
+      if (lane == 0 && !dev::mbar_wait_drain(dev::smem_u32(drain), 0, tmo))
+        if (g.err) atomicOr(g.err, kErrGemmDrain);
+    }
+  } else {
+    // ---------------------------------------------------------------- epilogue
+    const int quarter = warp & 3;      // TMEM lane quarter (warp id mod 4)
+    const int hh = (warp - 2) >> 2;    // which of the two warps of that quarter
+    const uint32_t lanes = static_cast<uint32_t>(quarter * 32) << 16;
+    uint4* stg = reinterpret_cast<uint4*>(staging + (warp - 2) * 2048);
+    const uint32_t free_bar = dev::mapa(dev::smem_u32(acc_free), 0);
+    uint32_t blk = 0;
+    for (int p = first; p < blocks; p += step, ++blk) {
+      int pm, tn;
+      pair_block(args, p, pm, tn);
+      const int row0 = (2 * pm + static_cast<int>(half)) * 128 + quarter * 32;  // this warp's rows
+      const uint32_t acc = blk & 1u;
+      const bool ok =
+          dev::mbar_wait(dev::smem_u32(acc_full + acc), (blk >> 1) & 1u, abort_flag, g.err, kErrGemmWait, tmo);
+      if (!__all_sync(0xffffffffu, ok)) break;
+      dev::tc_fence_after();
+      const uint32_t t = tmem + lanes + acc * P::kAccStep;
+      auto release = [&]() {  // after the loads of the shared columns
+        dev::tc_fence_before();
+        __syncwarp();
+        if (lane == 0) dev::mbar_arrive_cluster(free_bar);
+      };
+      if constexpr (SILU) {
+        // columns [0, 128): gate features, [128, 256): their up features.
+        // Chunks of 32 features, first one with a shared column: 2 + hh (its
+        // up columns) of accumulator 0, hh (its gate columns) of accumulator 1.
+        const int64_t row = row0 + lane;
+        const int64_t kt = k_tiles(g.N);
+#pragma unroll 1
+        for (int i = 0; i < 2; ++i) {
+          const int j = 2 * (acc ^ 1u ^ static_cast<uint32_t>(i)) + hh;
+          uint32_t vg[32], vu[32];
+          dev::tmem_ld32(t + 32 * j, vg);
+          dev::tmem_ld32(t + 128 + 32 * j, vu);
+          dev::tmem_wait_ld(vg);
+          dev::tmem_wait_ld(vu);
+          if (i == 0) release();
+          const int f0 = tn * 128 + 32 * j;
+          float y[32];
+          if (g.bias) {
+            const O* b = static_cast<const O*>(g.bias) + f0;
+#pragma unroll
+            for (int e = 0; e < 32; ++e)
+              y[e] = silu_mul_fast(__uint_as_float(vg[e]) + to_float(b[e]),
+                                   __uint_as_float(vu[e]) + to_float(b[g.N + e]));
+          } else {
+#pragma unroll
+            for (int e = 0; e < 32; ++e) y[e] = silu_mul_fast(__uint_as_float(vg[e]), __uint_as_float(vu[e]));
+          }
+          uint32_t m = 0;
+#pragma unroll
+          for (int e = 0; e < 32; ++e) m = max(m, abs_bits(y[e]));
+          const int byte = scale_byte(m);
+          const float f = inv_scale(byte);
+          uint32_t w[4];
+#pragma unroll
+          for (int e = 0; e < 4; ++e) {
+            const float v[8] = {y[8 * e],     y[8 * e + 1], y[8 * e + 2], y[8 * e + 3],
+                                y[8 * e + 4], y[8 * e + 5], y[8 * e + 6], y[8 * e + 7]};
+            w[e] = byte == kNanScale ? 0u : pack8_scaled(v, f);
+          }
+          if (row < g.M) {
+            *reinterpret_cast<uint4*>(g.q + row * (g.N >> 1) + (f0 >> 1)) = make_uint4(w[0], w[1], w[2], w[3]);
+            uint8_t* s = g.qs + scale_offset(row, tn, kt);
+            s[j] = static_cast<uint8_t>(byte);
+            if (tn + 1 == args.tiles_n && tn + 1 < kt) s[kTileBytes + j] = 0;  // the padding tile
+          }
+        }
+      } else {
+        // chunks of 32 columns: the shared one first (6 + hh of accumulator
+        // 0, hh of accumulator 1), then three of the other six
+#pragma unroll 1
+        for (int i = 0; i < 4; ++i) {
+          const int c = i == 0 ? (acc ? hh : 6 + hh) : (acc ? 2 : 0) + 2 * (i - 1) + hh;
+          uint32_t v[32];
+          dev::tmem_ld32(t + 32 * c, v);
+          dev::tmem_wait_ld(v);
+          if (i == 0) release();
+          const int col0 = tn * 256 + 32 * c;
+          if (g.bias) {
+            const O* b = static_cast<const O*>(g.bias) + col0;
+#pragma unroll
+            for (int e = 0; e < 32; ++e)
+              if (col0 + e < g.N) v[e] = __float_as_uint(__uint_as_float(v[e]) + to_float(b[e]));
+          }
+          // through the warp's 2 KB of shared memory (16-byte pieces, the
+          // piece index XORed with the row pair: no bank conflict either way)
+          // to rows of 64 contiguous bytes
+#pragma unroll
+          for (int e = 0; e < 4; ++e) {
+            uint32_t w[4];
+#pragma unroll
+            for (int k = 0; k < 4; ++k)
+              w[k] = pack2<O>(__uint_as_float(v[8 * e + 2 * k]), __uint_as_float(v[8 * e + 2 * k + 1]));
+            stg[lane * 4 + (e ^ ((lane >> 1) & 3))] = make_uint4(w[0], w[1], w[2], w[3]);
+          }
+          __syncwarp();
+          O* out = static_cast<O*>(g.out);
+#pragma unroll
+          for (int e = 0; e < 4; ++e) {
+            const int r = e * 8 + (lane >> 2), piece = lane & 3;
+            const uint4 w = stg[r * 4 + (piece ^ ((r >> 1) & 3))];
+            const int64_t row = row0 + r;
+            const int col = col0 + piece * 8;
+            if (row >= g.M || col >= g.N) continue;
+            O* dst = out + row * g.N + col;
+            if ((g.N & 7) == 0) {
+              *reinterpret_cast<uint4*>(dst) = w;
+            } else {  // rows that are not 16-byte aligned
+              const uint32_t x[4] = {w.x, w.y, w.z, w.w};
+#pragma unroll
+              for (int k = 0; k < 8; ++k)
+                if (col + k < g.N)
+                  reinterpret_cast<uint16_t*>(dst)[k] = static_cast<uint16_t>(x[k >> 1] >> (16 * (k & 1)));
+            }
+          }
+          __syncwarp();
+        }
+      }
+    }
+    dev::tc_fence_before();
+  }
+
+  __syncthreads();
+  dev::cluster_sync();  // the pair is done with both CTAs' TMEM and shared memory
+  if (warp == 1) {
+    dev::tc_fence_after();
+    dev::tmem_dealloc2(tmem, 512);
+  }
+}
+
+}  // namespace mx
+}  // namespace w8a8

@@ -54,6 +54,29 @@ __device__ __forceinline__ void mma_mxf4(uint32_t d_tmem, uint64_t adesc, uint64
       : "memory");
 }
 
+// One lane of a converged warp.  The producer and MMA roles run their loops
+// with the whole warp and issue under this predicate: the compiler then knows
+// that one lane is active and passes the operands of TMA and tcgen05 (which
+// the hardware takes from uniform registers) directly.  Under a predicate on
+// the lane index it emits a loop over the lanes' values around every such
+// instruction; a k block of four MMAs and six scale copies then took 606 ns to
+// issue, with this 280 ns, which is the MMAs' own time.
+__device__ __forceinline__ bool elect_one() {
+  uint32_t p;
+  asm volatile(
+      "{\n\t.reg .pred q;\n\t"
+      "elect.sync _|q, 0xffffffff;\n\t"
+      "selp.b32 %0, 1, 0, q;\n\t}"
+      : "=r"(p));
+  return p != 0;
+}
+
+// mbar_wait by a whole warp: true for all lanes or for none.
+__device__ __forceinline__ bool warp_wait(uint32_t bar, uint32_t parity, volatile int* abort_flag,
+                                          unsigned int* err, long long tmo) {
+  return __all_sync(0xffffffffu, dev::mbar_wait(bar, parity, abort_flag, err, kErrGemmWait, tmo));
+}
+
 struct MxGemmArgs {
   const void* bias;  // [N] of the output type, or null
   void* out;         // C [M, N]
@@ -63,8 +86,7 @@ struct MxGemmArgs {
   long long timeout_ns;
   int M, N, K;       // N: output columns (I with the SiLU epilogue)
   int kblocks;       // 256-value k blocks
-  int wtiles;        // weight tiles: 128 output columns each
-  int ttiles;        // token tiles
+  int ttiles;        // token tiles of the weight-stationary kernel
 };
 
 // 16 columns of fp32 TMEM
@@ -158,7 +180,12 @@ __device__ __forceinline__ void emit(const MxGemmArgs& a, int t, int col, int la
     const int c0 = col - lane;
     if ((lane & 7) == 0)
       *reinterpret_cast<uint32_t*>(a.q + static_cast<int64_t>(t) * (a.N >> 1) + ((c0 + lane) >> 1)) = w;
-    if (lane == 0) a.qs[scale_offset(t, c0 >> 7, k_tiles(a.N)) + ((c0 >> 5) & 3)] = static_cast<uint8_t>(byte);
+    if (lane == 0) {
+      const int64_t kt = k_tiles(a.N);
+      uint8_t* s = a.qs + scale_offset(t, c0 >> 7, kt) + ((c0 >> 5) & 3);
+      *s = static_cast<uint8_t>(byte);
+      if ((c0 >> 7) + 1 == (a.N >> 7) && ((a.N >> 7) & 1)) s[kTileBytes] = 0;  // the padding tile
+    }
   }
 }
 
@@ -215,17 +242,17 @@ __global__ void __launch_bounds__(kRowThreads) mx_row_kernel(const __grid_consta
   dev::tc_fence_before();
   __syncthreads();
   dev::tc_fence_after();
-  const uint32_t tmem = *tmem_slot;
+  const uint32_t tmem = __shfl_sync(0xffffffffu, *tmem_slot, 0);  // (the same in every lane, and known to be)
   dev::griddep_launch();
   dev::griddep_wait();  // any operand may be the previous kernel's output
 
   if (warp == 0) {
-    if (lane == 0) {
-      // ---------------------------------------------------------- producer
-      int stage = 0;
-      uint32_t phase = 0, issued_mask = 0, issued_phase = 0;
-      for (int kb = kb0; kb < kb1; ++kb) {
-        if (!dev::mbar_wait(dev::smem_u32(empty + stage), phase ^ 1u, abort_flag, args.err, kErrGemmWait, tmo)) break;
+    // ------------------------------------------------------------ producer
+    int stage = 0;
+    uint32_t phase = 0, issued_mask = 0, issued_phase = 0;
+    for (int kb = kb0; kb < kb1; ++kb) {
+      if (!warp_wait(dev::smem_u32(empty + stage), phase ^ 1u, abort_flag, args.err, tmo)) break;
+      if (elect_one()) {
         const uint32_t bar = dev::smem_u32(full + stage);
         dev::mbar_expect_tx(bar, P::kStageBytes);
 #pragma unroll
@@ -236,26 +263,28 @@ __global__ void __launch_bounds__(kRowThreads) mx_row_kernel(const __grid_consta
         }
         dev::tma_load_2d(dev::smem_u32(s_x + stage * P::kX), &tm_x, bar, kb * 128, tt * T);
         dev::tma_load_2d(dev::smem_u32(s_xs + stage * P::kSf), &tm_xs, bar, kb * 256, (tt * T) >> 7);
-        issued_mask |= 1u << stage;
-        issued_phase = (issued_phase & ~(1u << stage)) | (phase << stage);
-        if (++stage == P::kStages) {
-          stage = 0;
-          phase ^= 1u;
-        }
       }
+      __syncwarp();
+      issued_mask |= 1u << stage;
+      issued_phase = (issued_phase & ~(1u << stage)) | (phase << stage);
+      if (++stage == P::kStages) {
+        stage = 0;
+        phase ^= 1u;
+      }
+    }
+    if (lane == 0)
       for (int s = 0; s < P::kStages; ++s)  // no copy in flight when the CTA ends
         if (issued_mask & (1u << s))
           if (!dev::mbar_wait_drain(dev::smem_u32(full + s), (issued_phase >> s) & 1u, tmo))
             if (args.err) atomicOr(args.err, kErrGemmDrain);
-    }
   } else if (warp == 1) {
-    if (lane == 0) {
-      // --------------------------------------------------------------- MMA
-      int stage = 0;
-      uint32_t phase = 0;
-      for (int kb = kb0; kb < kb1; ++kb) {
-        if (!dev::mbar_wait(dev::smem_u32(full + stage), phase, abort_flag, args.err, kErrGemmWait, tmo)) break;
-        dev::tc_fence_after();
+    // ----------------------------------------------------------------- MMA
+    int stage = 0;
+    uint32_t phase = 0;
+    for (int kb = kb0; kb < kb1; ++kb) {
+      if (!warp_wait(dev::smem_u32(full + stage), phase, abort_flag, args.err, tmo)) break;
+      dev::tc_fence_after();
+      if (elect_one()) {
         // each stage has its own scale columns: free again once the MMAs that
         // read them have arrived on `empty`
         const uint32_t sf = tmem + P::kAccCols + stage * P::kSfCols;
@@ -269,26 +298,28 @@ __global__ void __launch_bounds__(kRowThreads) mx_row_kernel(const __grid_consta
         }
         const uint64_t dx = dev::sdesc_k_sw128(dev::smem_u32(s_x + stage * P::kX));
         const int steps = min(4, (args.K - kb * 256 + 63) / 64);  // beyond K: nothing to add
-        for (int k = 0; k < steps; ++k) {
-          const uint32_t id = idesc_mxf4(128, T, 0) | (static_cast<uint32_t>(k & 1) << 5) |
-                              (static_cast<uint32_t>(k & 1) << 30);
+#pragma unroll
+        for (int k = 0; k < 4; ++k) {
+          if (k >= steps) break;
+          constexpr uint32_t ids[2] = {idesc_mxf4(128, T, 0), idesc_mxf4(128, T, 2)};
 #pragma unroll
           for (int h = 0; h < P::kTiles; ++h) {
             const uint64_t dw = dev::sdesc_k_sw128(dev::smem_u32(s_w + (stage * P::kTiles + h) * P::kW));
-            mma_mxf4(tmem + h * T, dw + 2 * k, dx + 2 * k, id, sf + 8 * (h + 1) + 4 * (k >> 1), sf + 4 * (k >> 1),
-                     (kb > kb0 || k > 0) ? 1u : 0u);
+            mma_mxf4(tmem + h * T, dw + 2 * k, dx + 2 * k, ids[k & 1], sf + 8 * (h + 1) + 4 * (k >> 1),
+                     sf + 4 * (k >> 1), (kb > kb0 || k > 0) ? 1u : 0u);
           }
         }
         dev::tc_commit(dev::smem_u32(empty + stage));
-        if (++stage == P::kStages) {
-          stage = 0;
-          phase ^= 1u;
-        }
       }
-      dev::tc_commit(dev::smem_u32(acc_full));
-      if (!dev::mbar_wait_drain(dev::smem_u32(acc_full), 0, tmo))
-        if (args.err) atomicOr(args.err, kErrGemmDrain);
+      __syncwarp();
+      if (++stage == P::kStages) {
+        stage = 0;
+        phase ^= 1u;
+      }
     }
+    if (elect_one()) dev::tc_commit(dev::smem_u32(acc_full));
+    if (lane == 0 && !dev::mbar_wait_drain(dev::smem_u32(acc_full), 0, tmo))
+      if (args.err) atomicOr(args.err, kErrGemmDrain);
   }
   __syncwarp();
   const int tokens = min(T, args.M - tt * T);

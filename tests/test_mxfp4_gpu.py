@@ -54,13 +54,12 @@ def _operand(pkg, r, k, sigma, seed, dev, spread=0):
     return t, O.values(c, b)
 
 
-def _gemm_bound(av, wv, ref, dtype):
+def _gemm_bound(k, mag, ref, dtype):
     """Half a step of the output type, plus fp32 accumulation: each of the K/32
     block sums is exact (64 products of 4-bit numbers), and each addition of
     one to the running sum may lose one fp32 step (2^-23, truncation allowed
-    for) of the sum of magnitudes."""
-    k = av.shape[1]
-    return torch.finfo(dtype).eps / 2 * ref.abs() + (k // 32 + 2) * 2.0 ** -23 * (av.abs() @ wv.abs().T) + 1e-30
+    for) of the sum of magnitudes `mag`."""
+    return torch.finfo(dtype).eps / 2 * ref.abs() + (k // 32 + 2) * 2.0 ** -23 * mag + 1e-30
 
 
 # ------------------------------------------------------------------ quantisers
@@ -180,23 +179,27 @@ def test_rmsnorm_quant_extremes(pkg, cuda_dev):
 # --------------------------------------------------------------------- product
 @pytest.mark.parametrize("m,n,k", [(1, 128, 64), (1, 16, 32), (16, 128, 256), (1, 1, 32), (5, 130, 96), (16, 384, 1056), (17, 200, 512),
                                    (32, 256, 2080), (33, 512, 768), (64, 1000, 4096), (65, 384, 320), (128, 256, 1024),
-                                   (129, 257, 288), (300, 1024, 512), (1, 2048, 8192), (513, 640, 1280)])
+                                   (129, 257, 288), (300, 1024, 512), (1, 2048, 8192), (513, 640, 1280),
+                                   # 256 x 256 blocks: whole, ragged in M, N and K, several per SM pair
+                                   (4096, 1024, 256), (2000, 2040, 544), (129, 9600, 96), (1025, 4099, 320),
+                                   (3000, 8192, 1056)])
 @pytest.mark.parametrize("dtype", TYPES)
 def test_gemm(pkg, cuda_dev, m, n, k, dtype):
     a, av = _operand(pkg, m, k, 1.0, m + k, cuda_dev)
     w, wv = _operand(pkg, n, k, 0.05, n + k, cuda_dev, spread=2)
     bias = (0.1 * torch.randn(n, generator=_gen(n))).to(dtype).to(cuda_dev)
-    ref = av @ wv.T
+    ref = (av.to(cuda_dev) @ wv.to(cuda_dev).T).cpu()
+    mag = (av.abs().to(cuda_dev) @ wv.abs().to(cuda_dev).T).cpu()
     for b in (None, bias):
         want = ref if b is None else ref + b.cpu().double()
         out = pkg.ops.mxfp4_gemm(a, w, b, out_dtype=dtype)
         assert out.dtype == dtype and tuple(out.shape) == (m, n)
         err = (out.cpu().double() - want).abs()
-        bound = _gemm_bound(av, wv, want, dtype)
+        bound = _gemm_bound(k, mag, want, dtype)
         assert (err <= bound).all(), (err / bound).max()
 
 
-@pytest.mark.parametrize("m,n,k", [(1, 256, 512), (40, 128, 1024), (200, 384, 256), (512, 512, 2048)])
+@pytest.mark.parametrize("m,n,k", [(1, 256, 512), (40, 128, 1024), (200, 384, 256), (512, 512, 2048), (1024, 2560, 256)])
 def test_gemm_nan_scales_and_wide_scales(pkg, cuda_dev, m, n, k):
     """A NaN-scaled block makes its output row (or column) NaN and no other;
     scales at both ends of E8M0 multiply as numbers."""
@@ -217,7 +220,7 @@ def test_gemm_nan_scales_and_wide_scales(pkg, cuda_dev, m, n, k):
     nan[:, n - 1] = True
     assert torch.equal(out.isnan(), nan)
     err = (out.double() - want).abs()
-    bound = _gemm_bound(av.nan_to_num(0), wv.nan_to_num(0), want, torch.bfloat16)
+    bound = _gemm_bound(k, av.nan_to_num(0).abs() @ wv.nan_to_num(0).abs().T, want, torch.bfloat16)
     assert (err[~nan] <= bound[~nan]).all()
 
 
@@ -237,10 +240,13 @@ def _silu_gemm_check(y, gv, uv, slack):
     assert ((got >= lo) & (got <= hi)).all()
     sign = O.values(O.unpack(y.data), byte) * want
     assert (sign >= 0).all()
+    cols = 4 * y.scales.shape[1]
+    assert (O.untile(y.scales, r, cols)[:, k // 32:] == 0).all()
 
 
 @pytest.mark.parametrize("m,i,k", [(1, 128, 64), (16, 256, 512), (9, 384, 1056), (32, 128, 288), (50, 512, 256), (64, 128, 2048),
-                                   (100, 256, 96), (128, 384, 1024), (130, 128, 512), (333, 768, 640)])
+                                   (100, 256, 96), (128, 384, 1024), (130, 128, 512), (333, 768, 640),
+                                   (2000, 640, 544), (129, 4992, 96), (3000, 2048, 256)])
 @pytest.mark.parametrize("dtype", TYPES)
 def test_gate_up_silu_quant(pkg, cuda_dev, m, i, k, dtype):
     """The fused epilogue on operands whose sums are exact in fp32 (block
@@ -251,7 +257,7 @@ def test_gate_up_silu_quant(pkg, cuda_dev, m, i, k, dtype):
     a, av = _operand(pkg, m, k, 1.0, m + k, cuda_dev)
     w, wv = _operand(pkg, 2 * i, k, 0.05, i + k, cuda_dev)
     bias = torch.randint(-8, 9, (2 * i,), generator=_gen(i)).to(dtype) / 16
-    full = av @ wv.T
+    full = (av.to(cuda_dev) @ wv.to(cuda_dev).T).cpu()
     assert torch.equal(full.float().double(), full)
     for b in (None, bias):
         gu = full if b is None else full + b.double()
