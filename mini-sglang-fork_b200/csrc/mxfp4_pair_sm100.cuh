@@ -9,10 +9,11 @@
 // bound by that.
 //
 // Two 256-column accumulators and the scales do not fit TMEM's 512 columns, so
-// the accumulators overlap by 64: accumulator 0 is columns [0, 256),
-// accumulator 1 [192, 448), the scales of two k blocks [448, 512).  The
-// epilogue reads the 64 shared columns first and releases them; the next
-// block's MMAs wait for those only, while the rest is still being read.
+// the accumulators overlap by 128: accumulator 0 is columns [0, 256),
+// accumulator 1 [128, 384), and every stage of the ring has its own 24 scale
+// columns from 384 on.  The epilogue reads the 128 shared columns into
+// registers first and releases them; the next block's MMAs wait for those
+// only, while the rest is still being read.
 #pragma once
 
 #include "mxfp4_sm100.cuh"
@@ -27,8 +28,10 @@ struct PairTraits {
   static constexpr int kStageBytes = 2 * kTile + 3 * kSf;
   static constexpr int kEpiWarps = 8;
   static constexpr int kThreads = 32 * (2 + kEpiWarps);
-  static constexpr int kAccStep = 192;  // columns from accumulator 0 to accumulator 1
-  static constexpr int kSfCol = 448;    // two buffers of 32 columns (A 8, B 16)
+  static constexpr int kAccStep = 128;  // columns from accumulator 0 to accumulator 1
+  static constexpr int kSfCol = 384;    // a stage's scales: A 8 columns, B 16
+  static constexpr int kSfCols = 24;
+  static_assert(kSfCol + kStages * kSfCols <= 512, "TMEM");
   static constexpr int kBarrierBytes = 256;
   static constexpr int kStagingBytes = kEpiWarps * 2048;
   static constexpr int kSmemBytes = 1024 + kStages * kStageBytes + kBarrierBytes + kStagingBytes;
@@ -52,6 +55,15 @@ __device__ __forceinline__ void mma_mxf4_pair(uint32_t d_tmem, uint64_t adesc, u
       : "memory");
 }
 
+// Arrive on an mbarrier of either CTA without releasing this thread's memory
+// operations.  It announces only that tcgen05.ld has delivered its registers
+// (tcgen05.wait::ld and fence::before_thread_sync come first); a releasing
+// arrive waits for the warp's output stores of the block before, 1500 clocks
+// during which the next block's MMAs stand still.
+__device__ __forceinline__ void mbar_arrive_relaxed(uint32_t cluster_bar) {
+  asm volatile("mbarrier.arrive.relaxed.cluster.shared::cluster.b64 _, [%0];" ::"r"(cluster_bar) : "memory");
+}
+
 struct PairArgs {
   MxGemmArgs g;
   int pairs_m;  // 256-row blocks of the output
@@ -69,6 +81,85 @@ __device__ __forceinline__ void pair_block(const PairArgs& a, int p, int& pm, in
   const int r = p - group * kGroup * a.tiles_n;
   pm = first + r % rows;
   tn = r / rows;
+}
+
+// SiLU epilogue of 32 features of one output row per lane: one MXFP4 block.
+template <typename O>
+__device__ __forceinline__ void silu_chunk(const PairArgs& args, const uint32_t (&gate)[32], const uint32_t (&up)[32],
+                                           int64_t row, int tn, int j) {
+  const MxGemmArgs& g = args.g;
+  const int f0 = tn * 128 + 32 * j;
+  float y[32];
+  if (g.bias) {
+    const O* b = static_cast<const O*>(g.bias) + f0;
+#pragma unroll
+    for (int e = 0; e < 32; ++e)
+      y[e] = silu_mul_fast(__uint_as_float(gate[e]) + to_float(b[e]), __uint_as_float(up[e]) + to_float(b[g.N + e]));
+  } else {
+#pragma unroll
+    for (int e = 0; e < 32; ++e) y[e] = silu_mul_fast(__uint_as_float(gate[e]), __uint_as_float(up[e]));
+  }
+  uint32_t m = 0;
+#pragma unroll
+  for (int e = 0; e < 32; ++e) m = max(m, abs_bits(y[e]));
+  const int byte = scale_byte(m);
+  const float f = inv_scale(byte);
+  uint32_t w[4];
+#pragma unroll
+  for (int e = 0; e < 4; ++e) {
+    const float v[8] = {y[8 * e],     y[8 * e + 1], y[8 * e + 2], y[8 * e + 3],
+                        y[8 * e + 4], y[8 * e + 5], y[8 * e + 6], y[8 * e + 7]};
+    w[e] = byte == kNanScale ? 0u : pack8_scaled(v, f);
+  }
+  if (row < g.M) {
+    const int64_t kt = k_tiles(g.N);
+    *reinterpret_cast<uint4*>(g.q + row * (g.N >> 1) + (f0 >> 1)) = make_uint4(w[0], w[1], w[2], w[3]);
+    uint8_t* s = g.qs + scale_offset(row, tn, kt) + j;
+    *s = static_cast<uint8_t>(byte);
+    if (tn + 1 == args.tiles_n && tn + 1 < kt) s[kTileBytes] = 0;  // the padding tile
+  }
+}
+
+// Plain epilogue of 32 columns (from `col0`) of a warp's 32 rows: through the
+// warp's 2 KB of shared memory (16-byte pieces, the piece index XORed with the
+// row pair: no bank conflict either way) to rows of 64 contiguous bytes.
+template <typename O>
+__device__ __forceinline__ void plain_chunk(const MxGemmArgs& g, uint32_t (&v)[32], uint4* stg, int lane, int64_t row0,
+                                            int col0) {
+  if (g.bias) {
+    const O* b = static_cast<const O*>(g.bias) + col0;
+#pragma unroll
+    for (int e = 0; e < 32; ++e)
+      if (col0 + e < g.N) v[e] = __float_as_uint(__uint_as_float(v[e]) + to_float(b[e]));
+  }
+#pragma unroll
+  for (int e = 0; e < 4; ++e) {
+    uint32_t w[4];
+#pragma unroll
+    for (int k = 0; k < 4; ++k)
+      w[k] = pack2<O>(__uint_as_float(v[8 * e + 2 * k]), __uint_as_float(v[8 * e + 2 * k + 1]));
+    stg[lane * 4 + (e ^ ((lane >> 1) & 3))] = make_uint4(w[0], w[1], w[2], w[3]);
+  }
+  __syncwarp();
+  O* out = static_cast<O*>(g.out);
+#pragma unroll
+  for (int e = 0; e < 4; ++e) {
+    const int r = e * 8 + (lane >> 2), piece = lane & 3;
+    const uint4 w = stg[r * 4 + (piece ^ ((r >> 1) & 3))];
+    const int64_t row = row0 + r;
+    const int col = col0 + piece * 8;
+    if (row >= g.M || col >= g.N) continue;
+    O* dst = out + row * g.N + col;
+    if ((g.N & 7) == 0) {
+      *reinterpret_cast<uint4*>(dst) = w;
+    } else {  // rows that are not 16-byte aligned
+      const uint32_t x[4] = {w.x, w.y, w.z, w.w};
+#pragma unroll
+      for (int k = 0; k < 8; ++k)
+        if (col + k < g.N) reinterpret_cast<uint16_t*>(dst)[k] = static_cast<uint16_t>(x[k >> 1] >> (16 * (k & 1)));
+    }
+  }
+  __syncwarp();
 }
 
 template <typename O, bool SILU>
@@ -174,30 +265,28 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(PairTraits::kThreads
   } else if (warp == 1) {
     if (half == 0) {
       // --------------------------------------------- MMA issuer (leader only)
-      int stage = 0, stage2 = 0;  // this k block's stage, the one two k blocks back
-      uint32_t phase = 0, phase2 = 0;
-      uint32_t it = 0, blk = 0;
-      bool ok = true;
+      int stage = 0;
+      uint32_t phase = 0, blk = 0;
+      bool ok = true, ready = false;  // ready: the next stage has been seen full
       for (int p = first; ok && p < blocks; p += step, ++blk) {
         if (blk > 0 && !__all_sync(0xffffffffu, dev::mbar_wait_cluster(dev::smem_u32(acc_free), (blk - 1) & 1u,
                                                                        abort_flag, g.err, kErrGemmWait, tmo)))
           break;
         dev::tc_fence_after();
         const uint32_t d = tmem + (blk & 1u) * P::kAccStep;
-        for (int kb = 0; kb < g.kblocks; ++kb, ++it) {
-          if (it >= 2) {  // the scale buffer's last readers are done
-            ok = warp_wait(dev::smem_u32(empty + stage2), phase2, abort_flag, g.err, tmo);
+        for (int kb = 0; kb < g.kblocks; ++kb) {
+          if (!ready) {
+            ok = warp_wait(dev::smem_u32(full + stage), phase, abort_flag, g.err, tmo);
             if (!ok) break;
-            if (++stage2 == P::kStages) {
-              stage2 = 0;
-              phase2 ^= 1u;
-            }
           }
-          ok = warp_wait(dev::smem_u32(full + stage), phase, abort_flag, g.err, tmo);
-          if (!ok) break;
           dev::tc_fence_after();
+          const int next = stage + 1 == P::kStages ? 0 : stage + 1;
+          const uint32_t next_phase = next == 0 ? phase ^ 1u : phase;
+          // looked at before this block's MMAs are issued: the issue blocks
+          // while earlier MMAs run, and hides the look's latency
+          ready = __all_sync(0xffffffffu, dev::mbar_peek(dev::smem_u32(full + next), next_phase));
           if (elect_one()) {
-            const uint32_t sfa = tmem + P::kSfCol + (it & 1u) * 32;
+            const uint32_t sfa = tmem + P::kSfCol + stage * P::kSfCols;
             const uint32_t sfb = sfa + 8;
 #pragma unroll
             for (int c = 0; c < 2; ++c) {
@@ -220,10 +309,8 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(PairTraits::kThreads
             dev::tc_commit_pair(dev::mapa(dev::smem_u32(empty + stage), 1));
           }
           __syncwarp();
-          if (++stage == P::kStages) {
-            stage = 0;
-            phase ^= 1u;
-          }
+          stage = next;
+          phase = next_phase;
         }
         if (!ok) break;
         if (elect_one()) {
@@ -254,107 +341,37 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(PairTraits::kThreads
       if (!__all_sync(0xffffffffu, ok)) break;
       dev::tc_fence_after();
       const uint32_t t = tmem + lanes + acc * P::kAccStep;
-      auto release = [&]() {  // after the loads of the shared columns
-        dev::tc_fence_before();
-        __syncwarp();
-        if (lane == 0) dev::mbar_arrive_cluster(free_bar);
-      };
+      // the shared columns: chunks of 32, 4.. 7 of accumulator 0, 0..3 of
+      // accumulator 1; this warp's are hh and hh + 2 of the four
+      const uint32_t shared_t = t + (acc ? 0 : 128), own_t = t + (acc ? 128 : 0);
+      uint32_t s0[32], s1[32], v[32];
+      dev::tmem_ld32(shared_t + 32 * hh, s0);
+      dev::tmem_ld32(shared_t + 32 * hh + 64, s1);
+      dev::tmem_wait_ld(s0);
+      dev::tmem_wait_ld(s1);
+      dev::tc_fence_before();
+      __syncwarp();
+      if (lane == 0) mbar_arrive_relaxed(free_bar);
       if constexpr (SILU) {
-        // columns [0, 128): gate features, [128, 256): their up features.
-        // Chunks of 32 features, first one with a shared column: 2 + hh (its
-        // up columns) of accumulator 0, hh (its gate columns) of accumulator 1.
-        const int64_t row = row0 + lane;
-        const int64_t kt = k_tiles(g.N);
-#pragma unroll 1
-        for (int i = 0; i < 2; ++i) {
-          const int j = 2 * (acc ^ 1u ^ static_cast<uint32_t>(i)) + hh;
-          uint32_t vg[32], vu[32];
-          dev::tmem_ld32(t + 32 * j, vg);
-          dev::tmem_ld32(t + 128 + 32 * j, vu);
-          dev::tmem_wait_ld(vg);
-          dev::tmem_wait_ld(vu);
-          if (i == 0) release();
-          const int f0 = tn * 128 + 32 * j;
-          float y[32];
-          if (g.bias) {
-            const O* b = static_cast<const O*>(g.bias) + f0;
-#pragma unroll
-            for (int e = 0; e < 32; ++e)
-              y[e] = silu_mul_fast(__uint_as_float(vg[e]) + to_float(b[e]),
-                                   __uint_as_float(vu[e]) + to_float(b[g.N + e]));
-          } else {
-#pragma unroll
-            for (int e = 0; e < 32; ++e) y[e] = silu_mul_fast(__uint_as_float(vg[e]), __uint_as_float(vu[e]));
-          }
-          uint32_t m = 0;
-#pragma unroll
-          for (int e = 0; e < 32; ++e) m = max(m, abs_bits(y[e]));
-          const int byte = scale_byte(m);
-          const float f = inv_scale(byte);
-          uint32_t w[4];
-#pragma unroll
-          for (int e = 0; e < 4; ++e) {
-            const float v[8] = {y[8 * e],     y[8 * e + 1], y[8 * e + 2], y[8 * e + 3],
-                                y[8 * e + 4], y[8 * e + 5], y[8 * e + 6], y[8 * e + 7]};
-            w[e] = byte == kNanScale ? 0u : pack8_scaled(v, f);
-          }
-          if (row < g.M) {
-            *reinterpret_cast<uint4*>(g.q + row * (g.N >> 1) + (f0 >> 1)) = make_uint4(w[0], w[1], w[2], w[3]);
-            uint8_t* s = g.qs + scale_offset(row, tn, kt);
-            s[j] = static_cast<uint8_t>(byte);
-            if (tn + 1 == args.tiles_n && tn + 1 < kt) s[kTileBytes + j] = 0;  // the padding tile
-          }
-        }
+        // columns [0, 128): gate features, [128, 256): their up features
+        dev::tmem_ld32(own_t + 32 * hh, v);
+        dev::tmem_wait_ld(v);
+        if (acc) silu_chunk<O>(args, s0, v, row0 + lane, tn, hh);
+        else silu_chunk<O>(args, v, s0, row0 + lane, tn, hh);
+        dev::tmem_ld32(own_t + 32 * hh + 64, v);
+        dev::tmem_wait_ld(v);
+        if (acc) silu_chunk<O>(args, s1, v, row0 + lane, tn, hh + 2);
+        else silu_chunk<O>(args, v, s1, row0 + lane, tn, hh + 2);
       } else {
-        // chunks of 32 columns: the shared one first (6 + hh of accumulator
-        // 0, hh of accumulator 1), then three of the other six
-#pragma unroll 1
-        for (int i = 0; i < 4; ++i) {
-          const int c = i == 0 ? (acc ? hh : 6 + hh) : (acc ? 2 : 0) + 2 * (i - 1) + hh;
-          uint32_t v[32];
-          dev::tmem_ld32(t + 32 * c, v);
-          dev::tmem_wait_ld(v);
-          if (i == 0) release();
-          const int col0 = tn * 256 + 32 * c;
-          if (g.bias) {
-            const O* b = static_cast<const O*>(g.bias) + col0;
-#pragma unroll
-            for (int e = 0; e < 32; ++e)
-              if (col0 + e < g.N) v[e] = __float_as_uint(__uint_as_float(v[e]) + to_float(b[e]));
-          }
-          // through the warp's 2 KB of shared memory (16-byte pieces, the
-          // piece index XORed with the row pair: no bank conflict either way)
-          // to rows of 64 contiguous bytes
-#pragma unroll
-          for (int e = 0; e < 4; ++e) {
-            uint32_t w[4];
-#pragma unroll
-            for (int k = 0; k < 4; ++k)
-              w[k] = pack2<O>(__uint_as_float(v[8 * e + 2 * k]), __uint_as_float(v[8 * e + 2 * k + 1]));
-            stg[lane * 4 + (e ^ ((lane >> 1) & 3))] = make_uint4(w[0], w[1], w[2], w[3]);
-          }
-          __syncwarp();
-          O* out = static_cast<O*>(g.out);
-#pragma unroll
-          for (int e = 0; e < 4; ++e) {
-            const int r = e * 8 + (lane >> 2), piece = lane & 3;
-            const uint4 w = stg[r * 4 + (piece ^ ((r >> 1) & 3))];
-            const int64_t row = row0 + r;
-            const int col = col0 + piece * 8;
-            if (row >= g.M || col >= g.N) continue;
-            O* dst = out + row * g.N + col;
-            if ((g.N & 7) == 0) {
-              *reinterpret_cast<uint4*>(dst) = w;
-            } else {  // rows that are not 16-byte aligned
-              const uint32_t x[4] = {w.x, w.y, w.z, w.w};
-#pragma unroll
-              for (int k = 0; k < 8; ++k)
-                if (col + k < g.N)
-                  reinterpret_cast<uint16_t*>(dst)[k] = static_cast<uint16_t>(x[k >> 1] >> (16 * (k & 1)));
-            }
-          }
-          __syncwarp();
-        }
+        const int cs = tn * 256 + (acc ? 0 : 128) + 32 * hh, co = tn * 256 + (acc ? 128 : 0) + 32 * hh;
+        dev::tmem_ld32(own_t + 32 * hh, v);  // lands while the first chunk is written
+        plain_chunk<O>(g, s0, stg, lane, row0, cs);
+        plain_chunk<O>(g, s1, stg, lane, row0, cs + 64);
+        dev::tmem_wait_ld(v);
+        dev::tmem_ld32(own_t + 32 * hh + 64, s0);
+        plain_chunk<O>(g, v, stg, lane, row0, co);
+        dev::tmem_wait_ld(s0);
+        plain_chunk<O>(g, s0, stg, lane, row0, co + 64);
       }
     }
     dev::tc_fence_before();
