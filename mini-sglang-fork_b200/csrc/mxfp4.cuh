@@ -48,9 +48,36 @@ __device__ __forceinline__ float inv_scale(int byte) {
 
 __device__ __forceinline__ uint32_t abs_bits(float x) { return __float_as_uint(x) & 0x7fffffffu; }
 
-// Eight values to eight E2M1 codes (nearest, ties to even, saturating), value
-// j in bits [4j, 4j + 4).
-__device__ __forceinline__ uint32_t pack8(const float (&v)[8]) {
+// max(|a|, |b|, |c|) and max(|a|, |b|), NaN if one is.
+__device__ __forceinline__ float max3_abs(float a, float b, float c) {
+  float m;
+  asm("max.NaN.abs.f32 %0, %1, %2, %3;" : "=f"(m) : "f"(a), "f"(b), "f"(c));
+  return m;
+}
+__device__ __forceinline__ float max2_nan(float a, float b) {
+  float m;
+  asm("max.NaN.f32 %0, %1, %2;" : "=f"(m) : "f"(a), "f"(b));
+  return m;
+}
+
+// Eight values as four pairs, the operands of the packed fp32 instructions.
+struct Vec8 {
+  float2 p[4];
+};
+
+__device__ __forceinline__ float amax8(const Vec8& v) {
+  const float a = max3_abs(v.p[0].x, v.p[0].y, v.p[1].x);
+  const float b = max3_abs(v.p[1].y, v.p[2].x, v.p[2].y);
+  return max3_abs(max3_abs(v.p[3].x, v.p[3].y, a), b, b);
+}
+
+// v * f to eight E2M1 codes (nearest, ties to even, saturating), value j in
+// bits [4j, 4j + 4).
+__device__ __forceinline__ uint32_t pack8_scaled(const Vec8& v, float f) {
+  const float2 ff = make_float2(f, f);
+  float2 t[4];
+#pragma unroll
+  for (int j = 0; j < 4; ++j) t[j] = __fmul2_rn(v.p[j], ff);
   uint32_t w;
   asm("{\n\t.reg .b8 b0, b1, b2, b3;\n\t"
       "cvt.rn.satfinite.e2m1x2.f32 b0, %2, %1;\n\t"
@@ -59,15 +86,19 @@ __device__ __forceinline__ uint32_t pack8(const float (&v)[8]) {
       "cvt.rn.satfinite.e2m1x2.f32 b3, %8, %7;\n\t"
       "mov.b32 %0, {b0, b1, b2, b3};\n\t}"
       : "=r"(w)
-      : "f"(v[0]), "f"(v[1]), "f"(v[2]), "f"(v[3]), "f"(v[4]), "f"(v[5]), "f"(v[6]), "f"(v[7]));
+      : "f"(t[0].x), "f"(t[0].y), "f"(t[1].x), "f"(t[1].y), "f"(t[2].x), "f"(t[2].y), "f"(t[3].x), "f"(t[3].y));
   return w;
 }
 
-__device__ __forceinline__ uint32_t pack8_scaled(const float (&v)[8], float f) {
-  float t[8];
-#pragma unroll
-  for (int j = 0; j < 8; ++j) t[j] = v[j] * f;
-  return pack8(t);
+// The E2M1 code of one value (already scaled).
+__device__ __forceinline__ uint32_t code_of(float t) {
+  uint32_t w;
+  asm("{\n\t.reg .b8 b0;\n\t"
+      "cvt.rn.satfinite.e2m1x2.f32 b0, %2, %1;\n\t"
+      "cvt.u32.u8 %0, b0;\n\t}"
+      : "=r"(w)
+      : "f"(t), "f"(0.0f));
+  return w;
 }
 
 // ---- 64-bit forms, for the values next to a border
@@ -95,27 +126,63 @@ __device__ inline int scale_byte(double amax) {
 
 // ---- 16-bit activations
 template <typename T>
-__device__ __forceinline__ void unpack8(const uint4& raw, float (&f)[8]);
+__device__ __forceinline__ Vec8 unpack8(const uint4& raw);
 
 template <>
-__device__ __forceinline__ void unpack8<__nv_bfloat16>(const uint4& raw, float (&f)[8]) {
+__device__ __forceinline__ Vec8 unpack8<__nv_bfloat16>(const uint4& raw) {
   const uint32_t w[4] = {raw.x, raw.y, raw.z, raw.w};
+  Vec8 v;
 #pragma unroll
-  for (int j = 0; j < 4; ++j) {
-    f[2 * j] = __uint_as_float(w[j] << 16);
-    f[2 * j + 1] = __uint_as_float(w[j] & 0xffff0000u);
-  }
+  for (int j = 0; j < 4; ++j) v.p[j] = make_float2(__uint_as_float(w[j] << 16), __uint_as_float(w[j] & 0xffff0000u));
+  return v;
 }
 
 template <>
-__device__ __forceinline__ void unpack8<__half>(const uint4& raw, float (&f)[8]) {
+__device__ __forceinline__ Vec8 unpack8<__half>(const uint4& raw) {
   const __half2* h = reinterpret_cast<const __half2*>(&raw);
+  Vec8 v;
 #pragma unroll
-  for (int j = 0; j < 4; ++j) {
-    const float2 v = __half22float2(h[j]);
-    f[2 * j] = v.x;
-    f[2 * j + 1] = v.y;
-  }
+  for (int j = 0; j < 4; ++j) v.p[j] = __half22float2(h[j]);
+  return v;
+}
+
+// Largest magnitude of eight 16-bit values, as a pair still to be joined (NaN
+// if one is): four-lane reductions work on the pair.
+template <typename T>
+struct Pair16;
+template <>
+struct Pair16<__nv_bfloat16> {
+  using V = __nv_bfloat162;
+};
+template <>
+struct Pair16<__half> {
+  using V = __half2;
+};
+
+template <typename T>
+__device__ __forceinline__ uint32_t max_pair(uint32_t a, uint32_t b) {
+  using V = typename Pair16<T>::V;
+  const V m = __hmax2_nan(reinterpret_cast<const V&>(a), reinterpret_cast<const V&>(b));
+  return reinterpret_cast<const uint32_t&>(m);
+}
+
+template <typename T>
+__device__ __forceinline__ uint32_t amax8_pair(const uint4& raw) {
+  constexpr uint32_t k = 0x7fff7fffu;
+  return max_pair<T>(max_pair<T>(raw.x & k, raw.y & k), max_pair<T>(raw.z & k, raw.w & k));
+}
+
+// fp32 bits of the larger of a pair of magnitudes.
+template <typename T>
+__device__ __forceinline__ uint32_t pair_bits(uint32_t m);
+template <>
+__device__ __forceinline__ uint32_t pair_bits<__nv_bfloat16>(uint32_t m) {
+  return max(m << 16, m & 0xffff0000u);
+}
+template <>
+__device__ __forceinline__ uint32_t pair_bits<__half>(uint32_t m) {
+  const float2 f = __half22float2(reinterpret_cast<const __half2&>(m));
+  return max(__float_as_uint(f.x), __float_as_uint(f.y)) & 0x7fffffffu;
 }
 
 template <typename T>
@@ -144,11 +211,26 @@ __device__ __forceinline__ float to_float<__half>(__half x) { return __half2floa
 // relative error is below 2^-18: the argument -g log2(e) carries at most
 // 58 (2^-24 + 2^-25.9) absolute error, i.e. 3e-6 relative in exp, ex2 and rcp
 // about 2^-22 each, and three roundings.  Below that see the callers.
+__device__ __forceinline__ float ex2_approx(float x) {
+  float y;
+  asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(y) : "f"(x));
+  return y;
+}
+__device__ __forceinline__ float rcp_approx(float x) {
+  float y;
+  asm("rcp.approx.ftz.f32 %0, %1;" : "=f"(y) : "f"(x));
+  return y;
+}
+
+__device__ __forceinline__ float2 silu_mul_fast(float2 g, float2 u) {
+  constexpr float c = -1.4426950408889634f;
+  const float2 t = __fmul2_rn(g, make_float2(c, c));
+  const float2 d = __fadd2_rn(make_float2(ex2_approx(t.x), ex2_approx(t.y)), make_float2(1.0f, 1.0f));
+  return __fmul2_rn(__fmul2_rn(g, make_float2(rcp_approx(d.x), rcp_approx(d.y))), u);
+}
+
 __device__ __forceinline__ float silu_mul_fast(float g, float u) {
-  float e, s;
-  asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(e) : "f"(g * -1.4426950408889634f));
-  asm("rcp.approx.ftz.f32 %0, %1;" : "=f"(s) : "f"(1.0f + e));
-  return g * s * u;
+  return silu_mul_fast(make_float2(g, 0.0f), make_float2(u, 0.0f)).x;
 }
 
 }  // namespace mx

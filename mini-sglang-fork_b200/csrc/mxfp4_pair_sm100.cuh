@@ -89,28 +89,24 @@ __device__ __forceinline__ void silu_chunk(const PairArgs& args, const uint32_t 
                                            int64_t row, int tn, int j) {
   const MxGemmArgs& g = args.g;
   const int f0 = tn * 128 + 32 * j;
-  float y[32];
-  if (g.bias) {
-    const O* b = static_cast<const O*>(g.bias) + f0;
+  Vec8 y[4];
 #pragma unroll
-    for (int e = 0; e < 32; ++e)
-      y[e] = silu_mul_fast(__uint_as_float(gate[e]) + to_float(b[e]), __uint_as_float(up[e]) + to_float(b[g.N + e]));
-  } else {
-#pragma unroll
-    for (int e = 0; e < 32; ++e) y[e] = silu_mul_fast(__uint_as_float(gate[e]), __uint_as_float(up[e]));
+  for (int e = 0; e < 16; ++e) {
+    float2 gv = make_float2(__uint_as_float(gate[2 * e]), __uint_as_float(gate[2 * e + 1]));
+    float2 uv = make_float2(__uint_as_float(up[2 * e]), __uint_as_float(up[2 * e + 1]));
+    if (g.bias) {
+      const O* b = static_cast<const O*>(g.bias) + f0 + 2 * e;
+      gv = __fadd2_rn(gv, make_float2(to_float(b[0]), to_float(b[1])));
+      uv = __fadd2_rn(uv, make_float2(to_float(b[g.N]), to_float(b[g.N + 1])));
+    }
+    y[e >> 2].p[e & 3] = silu_mul_fast(gv, uv);
   }
-  uint32_t m = 0;
-#pragma unroll
-  for (int e = 0; e < 32; ++e) m = max(m, abs_bits(y[e]));
-  const int byte = scale_byte(m);
+  const float m = max3_abs(max3_abs(amax8(y[0]), amax8(y[1]), amax8(y[2])), amax8(y[3]), 0.0f);
+  const int byte = scale_byte(abs_bits(m));
   const float f = inv_scale(byte);
   uint32_t w[4];
 #pragma unroll
-  for (int e = 0; e < 4; ++e) {
-    const float v[8] = {y[8 * e],     y[8 * e + 1], y[8 * e + 2], y[8 * e + 3],
-                        y[8 * e + 4], y[8 * e + 5], y[8 * e + 6], y[8 * e + 7]};
-    w[e] = byte == kNanScale ? 0u : pack8_scaled(v, f);
-  }
+  for (int e = 0; e < 4; ++e) w[e] = byte == kNanScale ? 0u : pack8_scaled(y[e], f);
   if (row < g.M) {
     const int64_t kt = k_tiles(g.N);
     *reinterpret_cast<uint4*>(g.q + row * (g.N >> 1) + (f0 >> 1)) = make_uint4(w[0], w[1], w[2], w[3]);

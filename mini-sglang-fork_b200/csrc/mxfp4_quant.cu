@@ -29,11 +29,33 @@ namespace {
 
 constexpr int kThreads = 256;
 
-// max over the four lanes of a block
-__device__ __forceinline__ uint32_t quad_max(uint32_t v) {
-  v = max(v, __shfl_xor_sync(0xffffffffu, v, 1));
-  return max(v, __shfl_xor_sync(0xffffffffu, v, 2));
-}
+// n / d for n < 2^31 by a multiplication (Granlund and Montgomery): the row of
+// a warp's task; a 64-bit division would be a quarter of the instructions that
+// a warp spends on its values.
+struct Divisor {
+  uint32_t d, mul, shift;
+  explicit Divisor(uint32_t d_) : d(d_) {
+    uint32_t l = 0;
+    while ((1ull << l) < d) ++l;
+    shift = l;
+    mul = static_cast<uint32_t>((((1ull << l) - d) << 32) / d + 1);
+  }
+  __device__ __forceinline__ uint32_t quotient(uint32_t n) const {
+    return (__umulhi(n, mul) + n) >> shift;  // n < 2^31: the sum does not wrap
+  }
+};
+
+// A warp's share: VPT groups of 256 values from group g0 of a row.
+struct Task {
+  int64_t row;
+  int g0;
+  __device__ __forceinline__ Task(const Divisor& segs, int vpt) {
+    const uint32_t t = blockIdx.x * (kThreads / 32) + (threadIdx.x >> 5);
+    const uint32_t r = segs.quotient(t);
+    row = r;
+    g0 = static_cast<int>(t - r * segs.d) * vpt;
+  }
+};
 
 // Stores a warp's scale bytes (one per block, in every lane of the block):
 // the words of k tiles kt and kt + 1, from lanes 0 and 16.
@@ -46,45 +68,43 @@ __device__ __forceinline__ void store_scales(uint8_t* scales, int64_t row, int64
     *reinterpret_cast<uint32_t*>(scales + scale_offset(row, kt + (lane >> 4), ktiles)) = w;
 }
 
-__device__ __forceinline__ uint32_t amax8(const float (&v)[8]) {
-  uint32_t m = abs_bits(v[0]);
-#pragma unroll
-  for (int j = 1; j < 8; ++j) m = max(m, abs_bits(v[j]));
-  return m;
+// Largest magnitude over the four lanes of a block, NaN if one is.
+__device__ __forceinline__ float quad_max(float v) {
+  v = max2_nan(v, __shfl_xor_sync(0xffffffffu, v, 1));
+  return max2_nan(v, __shfl_xor_sync(0xffffffffu, v, 2));
 }
 
 // ------------------------------------------------------------------- plain
 // A warp takes VPT consecutive groups of 256 values of one row.
 template <typename T, int VPT>
 __global__ void __launch_bounds__(kThreads) quant_kernel(const T* __restrict__ x, int64_t ldx, uint8_t* __restrict__ data,
-                                                         uint8_t* __restrict__ scales, int64_t M, int K, int segs) {
+                                                         uint8_t* __restrict__ scales, int64_t M, int K, Divisor segs) {
   const int lane = threadIdx.x & 31;
-  const int64_t task = static_cast<int64_t>(blockIdx.x) * (kThreads / 32) + (threadIdx.x >> 5);
-  const int64_t row = task / segs;
-  const int g0 = static_cast<int>(task - row * segs) * VPT;  // first 256-value group
+  const Task t(segs, VPT);
   const int nvec = K >> 3;
   const int64_t kt = k_tiles(K);
   dev::griddep_launch();
   dev::griddep_wait();
-  if (row >= M) return;
-  const uint4* xr = reinterpret_cast<const uint4*>(x + row * ldx);
-  uint32_t* qr = reinterpret_cast<uint32_t*>(data + row * (K >> 1));
+  if (t.row >= M) return;
+  const uint4* xr = reinterpret_cast<const uint4*>(x + t.row * ldx);
+  uint32_t* qr = reinterpret_cast<uint32_t*>(data + t.row * (K >> 1));
   uint4 raw[VPT];
 #pragma unroll
   for (int j = 0; j < VPT; ++j) {
-    const int vi = (g0 + j) * 32 + lane;
+    const int vi = (t.g0 + j) * 32 + lane;
     raw[j] = vi < nvec ? __ldcs(xr + vi) : make_uint4(0, 0, 0, 0);
   }
 #pragma unroll
   for (int j = 0; j < VPT; ++j) {
-    const int vi = (g0 + j) * 32 + lane;
-    if ((g0 + j) * 32 >= nvec) break;  // the whole warp is beyond the row
-    float v[8];
-    unpack8<T>(raw[j], v);
-    const int byte = scale_byte(quad_max(amax8(v)));
-    const uint32_t w = byte == kNanScale ? 0u : pack8_scaled(v, inv_scale(byte));
+    const int vi = (t.g0 + j) * 32 + lane;
+    if ((t.g0 + j) * 32 >= nvec) break;  // the whole warp is beyond the row
+    uint32_t m = amax8_pair<T>(raw[j]);
+    m = max_pair<T>(m, __shfl_xor_sync(0xffffffffu, m, 1));
+    m = max_pair<T>(m, __shfl_xor_sync(0xffffffffu, m, 2));
+    const int byte = scale_byte(pair_bits<T>(m));
+    const uint32_t w = byte == kNanScale ? 0u : pack8_scaled(unpack8<T>(raw[j]), inv_scale(byte));
     if (vi < nvec) qr[vi] = w;
-    store_scales(scales, row, 2 * (g0 + j), kt, lane, byte);
+    store_scales(scales, t.row, 2 * (t.g0 + j), kt, lane, byte);
   }
 }
 
@@ -97,10 +117,16 @@ __device__ inline double silu_mul_exact(float g, float u) {
 }
 
 template <typename T>
+__device__ inline void spread(const uint4& raw, float (&f)[8]) {
+  const Vec8 v = unpack8<T>(raw);
+  for (int j = 0; j < 8; ++j) f[j] = j & 1 ? v.p[j >> 1].y : v.p[j >> 1].x;
+}
+
+template <typename T>
 __device__ __noinline__ double silu_amax_exact(uint4 graw, uint4 uraw) {
   float g[8], u[8];
-  unpack8<T>(graw, g);
-  unpack8<T>(uraw, u);
+  spread<T>(graw, g);
+  spread<T>(uraw, u);
   double m = 0.0;
   for (int j = 0; j < 8; ++j) {
     const double a = fabs(silu_mul_exact(g[j], u[j]));
@@ -112,8 +138,8 @@ __device__ __noinline__ double silu_amax_exact(uint4 graw, uint4 uraw) {
 template <typename T>
 __device__ __noinline__ uint32_t silu_codes_exact(uint4 graw, uint4 uraw, int byte, uint32_t lo, uint32_t hi) {
   float g[8], u[8];
-  unpack8<T>(graw, g);
-  unpack8<T>(uraw, u);
+  spread<T>(graw, g);
+  spread<T>(uraw, u);
   const double f = ldexp(1.0, 127 - byte);
   for (int j = 0; j < 8; ++j) {
     if (((lo ^ hi) >> (4 * j)) & 15u)
@@ -149,55 +175,52 @@ __device__ __forceinline__ bool far_gate<__half>(const uint4& raw) {
 // The exact product, rounded once to fp32, of those gates.  Below -200 it is a
 // zero of the product's sign next to any scale, which the fast form gives.
 template <typename T>
-__device__ __noinline__ void silu_far(uint4 graw, uint4 uraw, float (&y)[8]) {
+__device__ __noinline__ Vec8 silu_far(uint4 graw, uint4 uraw, Vec8 y) {
   float g[8], u[8];
-  unpack8<T>(graw, g);
-  unpack8<T>(uraw, u);
+  spread<T>(graw, g);
+  spread<T>(uraw, u);
+  float* f = reinterpret_cast<float*>(&y);
   for (int j = 0; j < 8; ++j) {
     const bool low = g[j] < -40.0f && g[j] > -200.0f;
     const bool tiny = g[j] != 0.0f && fabsf(g[j]) < 7.888609052210118e-31f;
-    if (low || tiny) y[j] = static_cast<float>(silu_mul_exact(g[j], u[j]));
+    if (low || tiny) f[j] = static_cast<float>(silu_mul_exact(g[j], u[j]));
   }
+  return y;
 }
 
 template <typename T, int VPT>
 __global__ void __launch_bounds__(kThreads) silu_kernel(const T* __restrict__ gate_up, int64_t ld,
                                                         uint8_t* __restrict__ data, uint8_t* __restrict__ scales,
-                                                        int64_t M, int I, int segs) {
+                                                        int64_t M, int I, Divisor segs) {
   const int lane = threadIdx.x & 31;
-  const int64_t task = static_cast<int64_t>(blockIdx.x) * (kThreads / 32) + (threadIdx.x >> 5);
-  const int64_t row = task / segs;
-  const int g0 = static_cast<int>(task - row * segs) * VPT;
+  const Task t(segs, VPT);
   const int nvec = I >> 3;
   const int64_t kt = k_tiles(I);
   dev::griddep_launch();
   dev::griddep_wait();
-  if (row >= M) return;
-  const uint4* gr = reinterpret_cast<const uint4*>(gate_up + row * ld);
+  if (t.row >= M) return;
+  const uint4* gr = reinterpret_cast<const uint4*>(gate_up + t.row * ld);
   const uint4* ur = gr + nvec;
-  uint32_t* qr = reinterpret_cast<uint32_t*>(data + row * (I >> 1));
+  uint32_t* qr = reinterpret_cast<uint32_t*>(data + t.row * (I >> 1));
   uint4 graw[VPT], uraw[VPT];
 #pragma unroll
   for (int j = 0; j < VPT; ++j) {
-    const int vi = (g0 + j) * 32 + lane;
+    const int vi = (t.g0 + j) * 32 + lane;
     graw[j] = vi < nvec ? __ldcs(gr + vi) : make_uint4(0, 0, 0, 0);
     uraw[j] = vi < nvec ? __ldcs(ur + vi) : make_uint4(0, 0, 0, 0);
   }
 #pragma unroll
   for (int j = 0; j < VPT; ++j) {
-    const int vi = (g0 + j) * 32 + lane;
-    if ((g0 + j) * 32 >= nvec) break;
-    float y[8];
+    const int vi = (t.g0 + j) * 32 + lane;
+    if ((t.g0 + j) * 32 >= nvec) break;
+    Vec8 y;
     {
-      float g[8], u[8];
-      unpack8<T>(graw[j], g);
-      unpack8<T>(uraw[j], u);
+      const Vec8 g = unpack8<T>(graw[j]), u = unpack8<T>(uraw[j]);
 #pragma unroll
-      for (int e = 0; e < 8; ++e) y[e] = silu_mul_fast(g[e], u[e]);
-      if (far_gate<T>(graw[j])) silu_far<T>(graw[j], uraw[j], y);
+      for (int e = 0; e < 4; ++e) y.p[e] = silu_mul_fast(g.p[e], u.p[e]);
+      if (far_gate<T>(graw[j])) y = silu_far<T>(graw[j], uraw[j], y);
     }
-    const uint32_t m = quad_max(amax8(y));
-    const float amax = __uint_as_float(m);
+    const float amax = quad_max(amax8(y));
     int byte = scale_byte(abs_bits(amax * (1.0f - kSiluDelta)));
     if (byte != scale_byte(abs_bits(amax * (1.0f + kSiluDelta)))) {
       // next to a power of two: all four lanes of the block come here
@@ -218,16 +241,18 @@ __global__ void __launch_bounds__(kThreads) silu_kernel(const T* __restrict__ ga
       if (w != hi) w = silu_codes_exact<T>(graw[j], uraw[j], byte, w, hi);
     }
     if (vi < nvec) qr[vi] = w;
-    store_scales(scales, row, 2 * (g0 + j), kt, lane, byte);
+    store_scales(scales, t.row, 2 * (t.g0 + j), kt, lane, byte);
   }
 }
 
 // ----------------------------------------------------------------- RMSNorm
-// One CTA per row, lane t of the CTA holding vectors t + blockDim * j.  The
-// sum of squares is taken in fp32 over four values and in 64 bits from there
-// (one conversion and one add per four values), so r is good to fp32 and the
-// exact path can use the same sum.  y = (v r) w in fp32: errors of r (2.5e-7)
-// and of the two products stay below 2^-20.
+// One CTA per row, thread t holding vectors t + blockDim * j.  The sum of
+// squares is taken in fp32 over four values and in 64 bits from there (one
+// conversion and one add per four values), so r is good to fp32 and the exact
+// path can use the same sum.  y = (v r) w in fp32: errors of r (2.5e-7) and of
+// the two products stay below 2^-20.  x and the residual stay in registers as
+// they were loaded and v is formed again in the second pass, which halves the
+// registers of a row.
 constexpr float kNormDelta = 9.5367431640625e-7f;  // 2^-20
 constexpr int kNormMaxThreads = 1024;
 
@@ -246,9 +271,9 @@ __device__ inline double norm_exact(float x, float res, float w, const NormRow& 
 template <typename T>
 __device__ __noinline__ double norm_amax_exact(uint4 xr, uint4 rr, uint4 wr, NormRow n) {
   float x[8], r[8], w[8];
-  unpack8<T>(xr, x);
-  unpack8<T>(rr, r);
-  unpack8<T>(wr, w);
+  spread<T>(xr, x);
+  spread<T>(rr, r);
+  spread<T>(wr, w);
   double m = 0.0;
   for (int j = 0; j < 8; ++j) {
     const double a = fabs(norm_exact<T>(x[j], r[j], w[j], n));
@@ -261,9 +286,9 @@ template <typename T>
 __device__ __noinline__ uint32_t norm_codes_exact(uint4 xr, uint4 rr, uint4 wr, NormRow n, int byte, uint32_t lo,
                                                   uint32_t hi) {
   float x[8], r[8], w[8];
-  unpack8<T>(xr, x);
-  unpack8<T>(rr, r);
-  unpack8<T>(wr, w);
+  spread<T>(xr, x);
+  spread<T>(rr, r);
+  spread<T>(wr, w);
   const double f = ldexp(1.0, 127 - byte);
   for (int j = 0; j < 8; ++j) {
     if (((lo ^ hi) >> (4 * j)) & 15u)
@@ -273,19 +298,34 @@ __device__ __noinline__ uint32_t norm_codes_exact(uint4 xr, uint4 rr, uint4 wr, 
 }
 
 template <typename T>
-__device__ __noinline__ void norm_far(uint4 xr, uint4 rr, uint4 wr, NormRow n, float (&y)[8]) {
+__device__ __noinline__ Vec8 norm_far(uint4 xr, uint4 rr, uint4 wr, NormRow n) {
   float x[8], r[8], w[8];
-  unpack8<T>(xr, x);
-  unpack8<T>(rr, r);
-  unpack8<T>(wr, w);
-  for (int j = 0; j < 8; ++j) y[j] = static_cast<float>(norm_exact<T>(x[j], r[j], w[j], n));
+  spread<T>(xr, x);
+  spread<T>(rr, r);
+  spread<T>(wr, w);
+  Vec8 y;
+  float* f = reinterpret_cast<float*>(&y);
+  for (int j = 0; j < 8; ++j) f[j] = static_cast<float>(norm_exact<T>(x[j], r[j], w[j], n));
+  return y;
 }
 
-template <typename T, int VPT, bool ADD>
-__global__ void __launch_bounds__(kNormMaxThreads)
+// v = x (+ residual) of a vector
+template <typename T, bool ADD>
+__device__ __forceinline__ Vec8 norm_input(const uint4& xr, const uint4& rr) {
+  Vec8 v = unpack8<T>(xr);
+  if constexpr (ADD) {
+    const Vec8 r = unpack8<T>(rr);
+#pragma unroll
+    for (int e = 0; e < 4; ++e) v.p[e] = __fadd2_rn(v.p[e], r.p[e]);
+  }
+  return v;
+}
+
+template <typename T, int VPT, int MAX_THREADS, bool ADD>
+__global__ void __launch_bounds__(MAX_THREADS)
     rmsnorm_kernel(const T* __restrict__ x, int64_t ldx, T* residual, int64_t ldr, const T* __restrict__ weight,
-                   float eps, uint8_t* __restrict__ data, uint8_t* __restrict__ scales, int64_t M, int K) {
-  __shared__ double part[32];
+                   float eps, uint8_t* __restrict__ data, uint8_t* __restrict__ scales, int K) {
+  __shared__ double part[MAX_THREADS / 32];
   const int lane = threadIdx.x & 31;
   const int warps = blockDim.x >> 5;
   const int nvec = K >> 3;
@@ -302,31 +342,23 @@ __global__ void __launch_bounds__(kNormMaxThreads)
   for (int j = 0; j < VPT; ++j) {
     const int vi = threadIdx.x + j * blockDim.x;
     xa[j] = vi < nvec ? __ldcs(xr + vi) : zero;
-    ra[j] = ADD && vi < nvec ? rr[vi] : zero;
+    ra[j] = ADD && vi < nvec ? __ldcs(rr + vi) : zero;
   }
-  float v[VPT][8];
   double ss = 0.0;
 #pragma unroll
   for (int j = 0; j < VPT; ++j) {
     const int vi = threadIdx.x + j * blockDim.x;
-    unpack8<T>(xa[j], v[j]);
-    if constexpr (ADD) {
-      float r[8];
-      unpack8<T>(ra[j], r);
+    const Vec8 v = norm_input<T, ADD>(xa[j], ra[j]);
+    if (ADD && vi < nvec)
+      rr[vi] = make_uint4(pack2<T>(v.p[0].x, v.p[0].y), pack2<T>(v.p[1].x, v.p[1].y), pack2<T>(v.p[2].x, v.p[2].y),
+                          pack2<T>(v.p[3].x, v.p[3].y));
 #pragma unroll
-      for (int e = 0; e < 8; ++e) v[j][e] += r[e];
-      if (vi < nvec)
-        rr[vi] = make_uint4(pack2<T>(v[j][0], v[j][1]), pack2<T>(v[j][2], v[j][3]), pack2<T>(v[j][4], v[j][5]),
-                            pack2<T>(v[j][6], v[j][7]));
-    }
-#pragma unroll
-    for (int e = 0; e < 8; e += 4) {
-      // a sum that leaves fp32 (|v| above 1e19) is taken in 64 bits
-      const float s = v[j][e] * v[j][e] + v[j][e + 1] * v[j][e + 1] + v[j][e + 2] * v[j][e + 2] +
-                      v[j][e + 3] * v[j][e + 3];
-      if (s > 1e30f || s < 1e-30f) {
-#pragma unroll
-        for (int i = 0; i < 4; ++i) ss += static_cast<double>(v[j][e + i]) * v[j][e + i];
+    for (int e = 0; e < 4; e += 2) {
+      const float2 q = __ffma2_rn(v.p[e + 1], v.p[e + 1], __fmul2_rn(v.p[e], v.p[e]));
+      const float s = q.x + q.y;
+      if (s > 1e30f || s < 1e-30f) {  // squares near the ends of fp32's range
+        for (int i = 0; i < 2; ++i)
+          ss += static_cast<double>(v.p[e + i].x) * v.p[e + i].x + static_cast<double>(v.p[e + i].y) * v.p[e + i].y;
       } else {
         ss += s;
       }
@@ -334,11 +366,12 @@ __global__ void __launch_bounds__(kNormMaxThreads)
   }
 #pragma unroll
   for (int o = 16; o > 0; o >>= 1) ss += __shfl_xor_sync(0xffffffffu, ss, o);
-  if (lane == 0) part[threadIdx.x >> 5] = ss;
-  __syncthreads();
-  ss = lane < warps ? part[lane] : 0.0;
-#pragma unroll
-  for (int o = 16; o > 0; o >>= 1) ss += __shfl_xor_sync(0xffffffffu, ss, o);
+  if (warps > 1) {
+    if (lane == 0) part[threadIdx.x >> 5] = ss;
+    __syncthreads();
+    ss = 0.0;
+    for (int i = 0; i < warps; ++i) ss += part[i];
+  }
   const NormRow n = {ss, K, eps};
   const double mean = ss * (1.0 / K) + static_cast<double>(eps);
   // a row whose mean square nears the ends of fp32's range is taken in 64 bits
@@ -350,17 +383,15 @@ __global__ void __launch_bounds__(kNormMaxThreads)
     if (base >= nvec) break;
     const int vi = base + lane;
     const uint4 wraw = vi < nvec ? __ldg(wr + vi) : zero;
-    float w[8], y[8];
-    unpack8<T>(wraw, w);
+    Vec8 y = norm_input<T, ADD>(xa[j], ra[j]);
+    const Vec8 w = unpack8<T>(wraw);
+    const float2 r2 = make_float2(r, r);
 #pragma unroll
-    for (int e = 0; e < 8; ++e) y[e] = v[j][e] * r * w[e];
-    if (far) norm_far<T>(xa[j], ra[j], wraw, n, y);
-    // a lane beyond the row holds zeros whatever r is (0 * inf would be NaN)
-    if (vi >= nvec) {
-#pragma unroll
-      for (int e = 0; e < 8; ++e) y[e] = 0.0f;
-    }
-    const float amax = __uint_as_float(quad_max(amax8(y)));
+    for (int e = 0; e < 4; ++e) y.p[e] = __fmul2_rn(__fmul2_rn(y.p[e], r2), w.p[e]);
+    if (far) y = norm_far<T>(xa[j], ra[j], wraw, n);
+    float am = amax8(y);
+    if (vi >= nvec) am = 0.0f;  // a lane beyond the row: 0 times an infinite r is no value of the block
+    const float amax = quad_max(am);
     int byte = scale_byte(abs_bits(amax * (1.0f - kNormDelta)));
     if (byte != scale_byte(abs_bits(amax * (1.0f + kNormDelta)))) {
       double d = norm_amax_exact<T>(xa[j], ra[j], wraw, n);
@@ -386,57 +417,53 @@ __global__ void __launch_bounds__(kNormMaxThreads)
 
 // ----------------------------------------------------------------- inverse
 template <typename O>
-__device__ __forceinline__ void store8(O* out, const float (&v)[8]) {
+__device__ __forceinline__ void store8(O* out, const Vec8& v) {
   if constexpr (sizeof(O) == 4) {
-    reinterpret_cast<float4*>(out)[0] = make_float4(v[0], v[1], v[2], v[3]);
-    reinterpret_cast<float4*>(out)[1] = make_float4(v[4], v[5], v[6], v[7]);
+    reinterpret_cast<float4*>(out)[0] = make_float4(v.p[0].x, v.p[0].y, v.p[1].x, v.p[1].y);
+    reinterpret_cast<float4*>(out)[1] = make_float4(v.p[2].x, v.p[2].y, v.p[3].x, v.p[3].y);
   } else {
-    *reinterpret_cast<uint4*>(out) = make_uint4(pack2<O>(v[0], v[1]), pack2<O>(v[2], v[3]), pack2<O>(v[4], v[5]),
-                                                pack2<O>(v[6], v[7]));
+    *reinterpret_cast<uint4*>(out) = make_uint4(pack2<O>(v.p[0].x, v.p[0].y), pack2<O>(v.p[1].x, v.p[1].y),
+                                                pack2<O>(v.p[2].x, v.p[2].y), pack2<O>(v.p[3].x, v.p[3].y));
   }
 }
 
 template <typename O, int VPT>
 __global__ void __launch_bounds__(kThreads) dequant_kernel(const uint8_t* __restrict__ data,
                                                            const uint8_t* __restrict__ scales, O* __restrict__ out,
-                                                           int64_t M, int K, int segs) {
+                                                           int64_t M, int K, Divisor segs) {
   const int lane = threadIdx.x & 31;
-  const int64_t task = static_cast<int64_t>(blockIdx.x) * (kThreads / 32) + (threadIdx.x >> 5);
-  const int64_t row = task / segs;
-  const int g0 = static_cast<int>(task - row * segs) * VPT;
+  const Task t(segs, VPT);
   const int nvec = K >> 3;
   const int64_t kt = k_tiles(K);
   dev::griddep_launch();
   dev::griddep_wait();
-  if (row >= M) return;
-  const uint32_t* qr = reinterpret_cast<const uint32_t*>(data + row * (K >> 1));
+  if (t.row >= M) return;
+  const uint32_t* qr = reinterpret_cast<const uint32_t*>(data + t.row * (K >> 1));
   uint32_t w[VPT], s[VPT];
 #pragma unroll
   for (int j = 0; j < VPT; ++j) {
-    const int vi = (g0 + j) * 32 + lane;
+    const int vi = (t.g0 + j) * 32 + lane;
     w[j] = vi < nvec ? qr[vi] : 0u;
-    s[j] = vi < nvec ? scales[scale_offset(row, vi >> 4, kt) + ((vi >> 2) & 3)] : 0u;
+    s[j] = vi < nvec ? scales[scale_offset(t.row, vi >> 4, kt) + ((vi >> 2) & 3)] : 0u;
   }
 #pragma unroll
   for (int j = 0; j < VPT; ++j) {
-    const int vi = (g0 + j) * 32 + lane;
+    const int vi = (t.g0 + j) * 32 + lane;
     if (vi >= nvec) break;
     // 2^(s - 127): a subnormal for s = 0, NaN for s = 255
     const float f = s[j] == kNanScale ? __uint_as_float(0x7fffffffu)
                     : s[j] == 0       ? __uint_as_float(0x00400000u)
                                       : __uint_as_float(s[j] << 23);
-    float v[8];
+    Vec8 v;
 #pragma unroll
     for (int b = 0; b < 4; ++b) {
       uint32_t h;
       asm("{\n\t.reg .b8 t;\n\tcvt.u8.u32 t, %1;\n\tcvt.rn.f16x2.e2m1x2 %0, t;\n\t}"
           : "=r"(h)
           : "r"((w[j] >> (8 * b)) & 255u));
-      const float2 p = __half22float2(reinterpret_cast<const __half2&>(h));
-      v[2 * b] = p.x * f;
-      v[2 * b + 1] = p.y * f;
+      v.p[b] = __fmul2_rn(__half22float2(reinterpret_cast<const __half2&>(h)), make_float2(f, f));
     }
-    store8(out + row * K + static_cast<int64_t>(vi) * 8, v);
+    store8(out + t.row * K + static_cast<int64_t>(vi) * 8, v);
   }
 }
 
@@ -462,12 +489,13 @@ int pick_vpt(int64_t M, int64_t K) {
   return groups >= 4 * 16 * static_cast<int64_t>(sm_count()) ? 4 : 1;
 }
 
-int grid_of(const char* what, int64_t M, int64_t K, int vpt, int* segs, unsigned* grid) {
+int grid_of(const char* what, int64_t M, int64_t K, int vpt, uint32_t* segs, unsigned* grid) {
   const int64_t groups = (K + 255) / 256;
-  *segs = static_cast<int>((groups + vpt - 1) / vpt);
+  *segs = static_cast<uint32_t>((groups + vpt - 1) / vpt);
   const int64_t ctas = (M * *segs + kThreads / 32 - 1) / (kThreads / 32);
-  W8A8_REQUIRE(ctas <= 0x7fffffffLL, W8A8_ERR_UNSUPPORTED, "%s: %lld x %lld is too large for one launch", what,
-               (long long)M, (long long)K);
+  // (Divisor and Task count a launch's warps in 31 bits)
+  W8A8_REQUIRE(ctas < (1LL << 31) / (kThreads / 32), W8A8_ERR_UNSUPPORTED, "%s: %lld x %lld is too large for one launch",
+               what, (long long)M, (long long)K);
   *grid = static_cast<unsigned>(ctas);
   return W8A8_OK;
 }
@@ -475,49 +503,68 @@ int grid_of(const char* what, int64_t M, int64_t K, int vpt, int* segs, unsigned
 template <typename T>
 int run_quant(const void* x, int64_t ldx, uint8_t* data, uint8_t* scales, int64_t M, int64_t K, cudaStream_t s) {
   const int vpt = pick_vpt(M, K);
-  int segs;
+  uint32_t segs;
   unsigned grid;
   if (int rc = grid_of("mxfp4_quant", M, K, vpt, &segs, &grid)) return rc;
   auto kern = vpt == 4 ? quant_kernel<T, 4> : quant_kernel<T, 1>;
   W8A8_CUDA_TRY(launch_pdl(kern, dim3(grid), dim3(kThreads), 0, s, static_cast<const T*>(x), ldx, data, scales, M,
-                           static_cast<int>(K), segs));
+                           static_cast<int>(K), Divisor(segs)));
   return W8A8_OK;
 }
 
 template <typename T>
 int run_silu(const void* gu, int64_t ld, uint8_t* data, uint8_t* scales, int64_t M, int64_t I, cudaStream_t s) {
   const int vpt = pick_vpt(M, I) == 4 ? 2 : 1;
-  int segs;
+  uint32_t segs;
   unsigned grid;
   if (int rc = grid_of("mxfp4_silu_mul_quant", M, I, vpt, &segs, &grid)) return rc;
   auto kern = vpt == 2 ? silu_kernel<T, 2> : silu_kernel<T, 1>;
   W8A8_CUDA_TRY(launch_pdl(kern, dim3(grid), dim3(kThreads), 0, s, static_cast<const T*>(gu), ld, data, scales, M,
-                           static_cast<int>(I), segs));
+                           static_cast<int>(I), Divisor(segs)));
   return W8A8_OK;
 }
 
+// Threads and vectors per thread of a row: with few rows one vector per thread
+// (the shortest chain), with many up to six, so that a CTA is small and an SM
+// holds many rows at different stages.
 template <typename T, bool ADD>
 int run_norm(const void* x, int64_t ldx, void* residual, int64_t ldr, const void* weight, float eps, uint8_t* data,
              uint8_t* scales, int64_t M, int64_t K, cudaStream_t s) {
   const int nvec = static_cast<int>(K / 8);
-  const int vpt = nvec <= kNormMaxThreads ? 1 : nvec <= 2 * kNormMaxThreads ? 2 : 4;
+  const bool many = M >= 2 * sm_count();
+  int vpt = (nvec + 1023) / 1024;
+  if (many) vpt = nvec <= 32 ? 1 : nvec <= 6 * 256 ? 6 : vpt;
+  if (many && nvec > 32 && nvec <= 6 * 256) {  // the fewest warps that hold the row, their vectors evened out
+    const int warps = (nvec + 6 * 32 - 1) / (6 * 32);
+    vpt = (nvec + warps * 32 - 1) / (warps * 32);
+  }
   const int threads = ((nvec + vpt - 1) / vpt + 31) / 32 * 32;
-  auto kern = vpt == 1 ? rmsnorm_kernel<T, 1, ADD> : vpt == 2 ? rmsnorm_kernel<T, 2, ADD> : rmsnorm_kernel<T, 4, ADD>;
-  W8A8_CUDA_TRY(launch_pdl(kern, dim3(static_cast<unsigned>(M)), dim3(threads), 0, s, static_cast<const T*>(x), ldx,
-                           static_cast<T*>(residual), ldr, static_cast<const T*>(weight), eps, data, scales, M,
-                           static_cast<int>(K)));
+#define MXFP4_NORM(V, THREADS)                                                                                      \
+  W8A8_CUDA_TRY(launch_pdl(rmsnorm_kernel<T, V, THREADS, ADD>, dim3(static_cast<unsigned>(M)), dim3(threads), 0, s, \
+                           static_cast<const T*>(x), ldx, static_cast<T*>(residual), ldr,                           \
+                           static_cast<const T*>(weight), eps, data, scales, static_cast<int>(K)))
+  if (threads > 256) {
+    if (vpt <= 1) MXFP4_NORM(1, 1024); else if (vpt <= 2) MXFP4_NORM(2, 1024); else MXFP4_NORM(4, 1024);
+  } else if (vpt <= 1) {
+    MXFP4_NORM(1, 256);
+  } else if (vpt <= 4) {
+    MXFP4_NORM(4, 256);
+  } else {
+    MXFP4_NORM(6, 256);
+  }
+#undef MXFP4_NORM
   return W8A8_OK;
 }
 
 template <typename O>
 int run_dequant(const uint8_t* data, const uint8_t* scales, void* out, int64_t M, int64_t K, cudaStream_t s) {
   const int vpt = pick_vpt(M, K);
-  int segs;
+  uint32_t segs;
   unsigned grid;
   if (int rc = grid_of("mxfp4_dequant", M, K, vpt, &segs, &grid)) return rc;
   auto kern = vpt == 4 ? dequant_kernel<O, 4> : dequant_kernel<O, 1>;
   W8A8_CUDA_TRY(launch_pdl(kern, dim3(grid), dim3(kThreads), 0, s, data, scales, static_cast<O*>(out), M,
-                           static_cast<int>(K), segs));
+                           static_cast<int>(K), Divisor(segs)));
   return W8A8_OK;
 }
 

@@ -172,8 +172,7 @@ __device__ __forceinline__ void emit(const MxGemmArgs& a, int t, int col, int la
     const float y = silu_mul_fast(g + bg, u + bu);
     const uint32_t m = __reduce_max_sync(0xffffffffu, abs_bits(y));
     const int byte = scale_byte(m);
-    const float v[8] = {y * inv_scale(byte), 0, 0, 0, 0, 0, 0, 0};
-    uint32_t w = byte == kNanScale ? 0u : (pack8(v) & 15u) << (4 * (lane & 7));
+    uint32_t w = byte == kNanScale ? 0u : code_of(y * inv_scale(byte)) << (4 * (lane & 7));
     w |= __shfl_xor_sync(0xffffffffu, w, 1);
     w |= __shfl_xor_sync(0xffffffffu, w, 2);
     w |= __shfl_xor_sync(0xffffffffu, w, 4);

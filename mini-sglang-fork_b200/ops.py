@@ -77,7 +77,8 @@ class QuantizedActivation:
 
 
 def _stream(t: torch.Tensor) -> int:
-    return torch.cuda.current_stream(t.device).cuda_stream
+    # the raw handle: torch.cuda.current_stream builds a Stream object first (2 us)
+    return torch._C._cuda_getCurrentRawStream(t.get_device())
 
 
 def _require_cuda(name: str, *ts: Optional[torch.Tensor]) -> None:
@@ -504,25 +505,64 @@ class MXFP4Tensor:
     :func:`mxfp4_quant` and its fused forms, an operand of :func:`mxfp4_gemm`,
     and accepted by the MXFP4 layers in place of a 16-bit activation."""
 
-    __slots__ = ("data", "scales", "shape")
+    # The operators' results keep codes and scales in one buffer (one
+    # allocation per call) and make the two views when asked for them.
+    __slots__ = ("_buf", "_data", "_scales", "_ptrs", "shape")
 
     def __init__(self, data: torch.Tensor, scales: torch.Tensor):
         if data.dtype != torch.uint8 or data.dim() != 2 or not data.is_contiguous() or data.shape[1] % 16:
             raise _lib.W8A8Error(_lib.ERR_INVALID_ARG, "MXFP4Tensor: data must be contiguous uint8 [R, K/2], K % 32 == 0")
         r, half = data.shape
         if (scales.dtype != torch.uint8 or not scales.is_contiguous()
-                or tuple(scales.shape) != mxfp4_scale_shape(r, 2 * half)):
+                or scales.shape != mxfp4_scale_shape(r, 2 * half)):
             raise _lib.W8A8Error(_lib.ERR_INVALID_ARG, f"MXFP4Tensor: scales must be contiguous uint8 tiles "
                                  f"{mxfp4_scale_shape(r, 2 * half)}, got {scales.dtype} {tuple(scales.shape)}")
         if scales.device != data.device:
             raise _lib.W8A8Error(_lib.ERR_INVALID_ARG, f"MXFP4Tensor: data on {data.device}, scales on {scales.device}")
-        self.data = data
-        self.scales = scales
-        self.shape = torch.Size((r, 2 * half))
+        self._buf = self._data = data
+        self._scales = scales
+        self._ptrs = (data.data_ptr(), scales.data_ptr())
+        self.shape = (r, 2 * half)
+
+    @classmethod
+    def _empty(cls, rows: int, k: int, like: torch.Tensor) -> "MXFP4Tensor":
+        if k <= 0 or k % 32:
+            raise _lib.W8A8Error(_lib.ERR_INVALID_ARG,
+                                 f"MXFP4: the last dimension ({k}) must be a positive multiple of 32")
+        t = cls.__new__(cls)
+        codes = rows * (k // 2)
+        t._buf = torch.empty(codes + (rows + 127) // 128 * ((k + 255) // 256) * 1024, dtype=torch.uint8,
+                             device=like.device)
+        p = t._buf.data_ptr()
+        t._data = t._scales = None
+        t._ptrs = (p, p + codes)
+        t.shape = (rows, k)
+        return t
 
     @property
-    def device(self):
-        return self.data.device
+    def data(self) -> torch.Tensor:
+        if self._data is None:
+            r, k = self.shape
+            self._data = self._buf[:r * (k // 2)].view(r, k // 2)
+        return self._data
+
+    @property
+    def scales(self) -> torch.Tensor:
+        if self._scales is None:
+            r, k = self.shape
+            self._scales = self._buf[r * (k // 2):].view(mxfp4_scale_shape(r, k))
+        return self._scales
+
+    @property
+    def device(self) -> torch.device:
+        return self._buf.device
+
+    def record_stream(self, stream) -> None:
+        """Marks the memory as in use on another stream (as
+        ``torch.Tensor.record_stream``)."""
+        self._buf.record_stream(stream)
+        if self._scales is not None and self._buf is self._data:
+            self._scales.record_stream(stream)
 
 
 def mxfp4_tile_scales(scales: torch.Tensor) -> torch.Tensor:
@@ -544,22 +584,17 @@ def mxfp4_plain_scales(t: MXFP4Tensor) -> torch.Tensor:
     return plain[:r, :k // 32].contiguous()
 
 
-class _OnDevice:
-    """Makes a tensor's device current around a launch when it is not."""
-
-    __slots__ = ("idx", "prev")
-
-    def __init__(self, t: torch.Tensor):
-        self.idx = t.device.index
-
-    def __enter__(self):
-        self.prev = torch.cuda.current_device()
-        if self.prev != self.idx:
-            torch.cuda.set_device(self.idx)
-
-    def __exit__(self, *exc):
-        if self.prev != self.idx:
-            torch.cuda.set_device(self.prev)
+def _mx_call(what: str, fn, t: torch.Tensor, *args) -> None:
+    """Launches ``fn(*args, stream)`` on ``t``'s device and that device's
+    current stream, whichever device is current."""
+    idx = t.get_device()
+    if idx == torch.cuda.current_device():
+        status = fn(*args, torch._C._cuda_getCurrentRawStream(idx))
+    else:
+        with torch.cuda.device(idx):
+            status = fn(*args, torch._C._cuda_getCurrentRawStream(idx))
+    if status != _lib.OK:
+        _lib.check(status, what)
 
 
 def _check_mx_input(name: str, what: str, x: torch.Tensor) -> int:
@@ -579,16 +614,6 @@ def _row_stride(x: torch.Tensor) -> int:
     return x.stride(0) if x.shape[0] > 1 else (x.shape[1] + 7) // 8 * 8
 
 
-def _mx_empty(rows: int, k: int, device: torch.device) -> MXFP4Tensor:
-    if k <= 0 or k % 32:
-        raise _lib.W8A8Error(_lib.ERR_INVALID_ARG, f"MXFP4: the last dimension ({k}) must be a positive multiple of 32")
-    t = MXFP4Tensor.__new__(MXFP4Tensor)
-    t.data = torch.empty(rows, k // 2, dtype=torch.uint8, device=device)
-    t.scales = torch.empty(mxfp4_scale_shape(rows, k), dtype=torch.uint8, device=device)
-    t.shape = torch.Size((rows, k))
-    return t
-
-
 def mxfp4_quant(x: torch.Tensor) -> MXFP4Tensor:
     """``x [M, K]`` bf16 or fp16 to MXFP4: per 32 values the scale
     ``2^(floor(log2 amax) - 2)``, values rounded to the nearest E2M1 number
@@ -596,10 +621,8 @@ def mxfp4_quant(x: torch.Tensor) -> MXFP4Tensor:
     the NaN scale.  Rows may be strided (multiples of 8); K % 32 == 0."""
     dt = _check_mx_input("mxfp4_quant", "x", x)
     m, k = x.shape
-    q = _mx_empty(m, k, x.device)
-    with _OnDevice(x):
-        _lib.check(_lib.load().mxfp4_quant(_ptr(x), _row_stride(x), dt, _ptr(q.data), _ptr(q.scales), m, k,
-                                           _stream(x)), "mxfp4_quant")
+    q = MXFP4Tensor._empty(m, k, x)
+    _mx_call("mxfp4_quant", _lib.load().mxfp4_quant, x, x.data_ptr(), _row_stride(x), dt, *q._ptrs, m, k)
     return q
 
 
@@ -608,12 +631,10 @@ def mxfp4_dequant(q: MXFP4Tensor, dtype: torch.dtype = torch.bfloat16) -> torch.
     tensor (exact in bf16 and fp32; a NaN-scaled block is NaN)."""
     if dtype not in _MX_DTYPE:
         raise _lib.W8A8Error(_lib.ERR_INVALID_ARG, f"mxfp4_dequant: bf16, fp16 or fp32, not {dtype}")
-    _require_cuda("mxfp4_dequant", q.data)
+    _require_cuda("mxfp4_dequant", q._buf)
     m, k = q.shape
     out = torch.empty(m, k, dtype=dtype, device=q.device)
-    with _OnDevice(q.data):
-        _lib.check(_lib.load().mxfp4_dequant(_ptr(q.data), _ptr(q.scales), _ptr(out), _MX_DTYPE[dtype], m, k,
-                                             _stream(out)), "mxfp4_dequant")
+    _mx_call("mxfp4_dequant", _lib.load().mxfp4_dequant, out, *q._ptrs, out.data_ptr(), _MX_DTYPE[dtype], m, k)
     return out
 
 
@@ -625,11 +646,10 @@ def mxfp4_silu_and_mul_quant(gate_up: torch.Tensor) -> MXFP4Tensor:
     m, two_i = gate_up.shape
     if two_i % 2:
         raise _lib.W8A8Error(_lib.ERR_INVALID_ARG, "mxfp4_silu_and_mul_quant: last dim must be even")
-    q = _mx_empty(m, two_i // 2, gate_up.device)
-    with _OnDevice(gate_up):
-        _lib.check(_lib.load().mxfp4_silu_mul_quant(_ptr(gate_up), _row_stride(gate_up), dt, _ptr(q.data),
-                                                    _ptr(q.scales), m, two_i // 2, _stream(gate_up)),
-                   "mxfp4_silu_and_mul_quant")
+    i = two_i // 2
+    q = MXFP4Tensor._empty(m, i, gate_up)
+    _mx_call("mxfp4_silu_and_mul_quant", _lib.load().mxfp4_silu_mul_quant, gate_up, gate_up.data_ptr(),
+             _row_stride(gate_up), dt, *q._ptrs, m, i)
     return q
 
 
@@ -650,11 +670,9 @@ def mxfp4_rmsnorm_quant(x: torch.Tensor, weight: torch.Tensor, eps: float,
                              "mxfp4_rmsnorm_quant: residual must match x (shape, type, unit column stride)")
     _require_cuda("mxfp4_rmsnorm_quant", weight, residual)
     _one_device("mxfp4_rmsnorm_quant", x, weight, residual)
-    q = _mx_empty(m, k, x.device)
-    with _OnDevice(x):
-        _lib.check(_lib.load().mxfp4_rmsnorm_quant(
-            _ptr(x), _row_stride(x), _ptr(residual), _row_stride(residual) if residual is not None else k,
-            _ptr(weight), float(eps), dt, _ptr(q.data), _ptr(q.scales), m, k, _stream(x)), "mxfp4_rmsnorm_quant")
+    q = MXFP4Tensor._empty(m, k, x)
+    _mx_call("mxfp4_rmsnorm_quant", _lib.load().mxfp4_rmsnorm_quant, x, x.data_ptr(), _row_stride(x), _ptr(residual),
+             _row_stride(residual) if residual is not None else k, weight.data_ptr(), float(eps), dt, *q._ptrs, m, k)
     return q, residual if residual is not None else x
 
 
@@ -666,8 +684,9 @@ def _check_mx_gemm(name: str, a: MXFP4Tensor, w: MXFP4Tensor, bias: Optional[tor
         raise _lib.W8A8Error(_lib.ERR_INVALID_ARG, f"{name}: shape mismatch A{tuple(a.shape)} B{tuple(w.shape)}")
     if bias is not None and (bias.dtype != dtype or bias.shape != (w.shape[0],) or not bias.is_contiguous()):
         raise _lib.W8A8Error(_lib.ERR_INVALID_ARG, f"{name}: bias must be contiguous {dtype} [{w.shape[0]}]")
-    _require_cuda(name, a.data, w.data, bias)
-    _one_device(name, a.data, w.data, bias)
+    _require_cuda(name, a._buf, w._buf, bias)
+    if a.device != w.device or (bias is not None and bias.device != a.device):
+        _one_device(name, a._buf, w._buf, bias)
 
 
 def mxfp4_gemm(a: MXFP4Tensor, w: MXFP4Tensor, bias: Optional[torch.Tensor] = None,
@@ -684,11 +703,10 @@ def mxfp4_gemm(a: MXFP4Tensor, w: MXFP4Tensor, bias: Optional[torch.Tensor] = No
         out = torch.empty(m, n, dtype=out_dtype, device=a.device)
     else:
         _require_cuda("mxfp4_gemm", out)
-        _one_device("mxfp4_gemm", a.data, out)
+        _one_device("mxfp4_gemm", a._buf, out)
         _check_2d("mxfp4_gemm out", out, out_dtype, (m, n))
-    with _OnDevice(out):
-        _lib.check(_lib.load().mxfp4_gemm(_ptr(a.data), _ptr(a.scales), _ptr(w.data), _ptr(w.scales), _ptr(bias),
-                                          _ptr(out), _MX_DTYPE[out_dtype], m, n, k, _stream(out)), "mxfp4_gemm")
+    _mx_call("mxfp4_gemm", _lib.load().mxfp4_gemm, out, *a._ptrs, *w._ptrs, _ptr(bias), out.data_ptr(),
+             _MX_DTYPE[out_dtype], m, n, k)
     return out
 
 
@@ -708,11 +726,9 @@ def mxfp4_gate_up_silu_quant(a: MXFP4Tensor, w: MXFP4Tensor, bias: Optional[torc
                              f"mxfp4_gate_up_silu_quant: {w.shape[0]} weight rows are not [gate; up] of a multiple of 32")
     if i % 128:
         return mxfp4_silu_and_mul_quant(mxfp4_gemm(a, w, bias, out_dtype=dtype))
-    y = _mx_empty(m, i, a.device)
-    with _OnDevice(a.data):
-        _lib.check(_lib.load().mxfp4_gemm_silu_quant(_ptr(a.data), _ptr(a.scales), _ptr(w.data), _ptr(w.scales),
-                                                     _ptr(bias), _MX_DTYPE[dtype], _ptr(y.data), _ptr(y.scales),
-                                                     m, i, k, _stream(a.data)), "mxfp4_gate_up_silu_quant")
+    y = MXFP4Tensor._empty(m, i, a._buf)
+    _mx_call("mxfp4_gate_up_silu_quant", _lib.load().mxfp4_gemm_silu_quant, a._buf, *a._ptrs, *w._ptrs, _ptr(bias),
+             _MX_DTYPE[dtype], *y._ptrs, m, i, k)
     return y
 
 
