@@ -31,12 +31,47 @@ struct Operands {
   int64_t b_rows;  // rows of B: N, or 2I
 };
 
-// Shares of K per output tile: enough CTAs to give every SM about two, at least
-// two k blocks each (one for the shortest K), at most a portable cluster's 8.
-int pick_split(int tiles, int kblocks, int nsm) {
-  int s = 1;
-  while (s < 8 && tiles * s * 2 <= 2 * nsm && kblocks >= 2 * (2 * s)) s *= 2;
-  return s;
+// Clusters of s CTAs of `Kern` (one CTA per SM) that the device holds at once:
+// fewer than SMs / s, since a cluster lives in one group of SMs.
+template <auto Kern>
+int active_clusters(int s, int threads, int smem, int* out) {
+  static std::mutex mu;
+  static int known[64][9] = {{0}};
+  const int dev = current_device();
+  W8A8_REQUIRE(dev >= 0 && dev < 64, W8A8_ERR_CUDA, "no current device");
+  std::lock_guard<std::mutex> lk(mu);
+  int& n = known[dev][s];
+  if (n == 0) {
+    cudaLaunchConfig_t cfg = {};
+    cfg.gridDim = dim3(static_cast<unsigned>(s));
+    cfg.blockDim = dim3(static_cast<unsigned>(threads));
+    cfg.dynamicSmemBytes = static_cast<size_t>(smem);
+    cudaLaunchAttribute attr[1];
+    attr[0].id = cudaLaunchAttributeClusterDimension;
+    attr[0].val.clusterDim.x = static_cast<unsigned>(s);
+    attr[0].val.clusterDim.y = 1;
+    attr[0].val.clusterDim.z = 1;
+    cfg.attrs = attr;
+    cfg.numAttrs = 1;
+    W8A8_CUDA_TRY(cudaOccupancyMaxActiveClusters(&n, Kern, &cfg));
+    if (n < 1) n = 1;
+  }
+  *out = n;
+  return W8A8_OK;
+}
+
+// CTAs that share an output tile's K: as many as leave every tile's cluster
+// resident at once (a second wave would cost as much as the first), with two k
+// blocks each at least, at most a portable cluster's 8.
+template <auto Kern>
+int pick_split(int64_t tiles, int kblocks, int threads, int smem, int* out) {
+  *out = 1;
+  for (int s = 2; s <= std::min(8, kblocks / 2) && tiles * s <= sm_count(); ++s) {
+    int n = 0;
+    if (int rc = active_clusters<Kern>(s, threads, smem, &n)) return rc;
+    if (tiles <= n) *out = s;
+  }
+  return W8A8_OK;
 }
 
 template <typename O, int T, bool SILU>
@@ -52,10 +87,13 @@ int launch_row(const Operands& o, MxGemmArgs args, cudaStream_t stream) {
   if (int rc = encode_operand(&tx, o.a, args.M, args.K / 2, T)) return rc;
   if (int rc = encode_words(&txs, o.as, row_tiles(args.M), k_tiles(args.K) * kTileBytes / 4, 256)) return rc;
   const int64_t tiles = wtiles * args.ttiles;
-  const int split = tiles > 4096 ? 1 : pick_split(static_cast<int>(tiles), args.kblocks, sm_count());
-  W8A8_REQUIRE(tiles * split <= 0x7fffffffLL, W8A8_ERR_UNSUPPORTED, "mxfp4_gemm: too many output tiles");
+  W8A8_REQUIRE(tiles <= 0x7fff0000LL, W8A8_ERR_UNSUPPORTED, "mxfp4_gemm: too many output tiles");
+  args.tiles = static_cast<int>(tiles);
+  int split = 1;
+  if (int rc = pick_split<kern>(tiles, args.kblocks, kRowThreads, P::kSmemBytes, &split)) return rc;
+  const int64_t grid = split > 1 ? tiles * split : std::min<int64_t>(tiles, std::max(1, sm_count()));
   cudaLaunchConfig_t cfg = {};
-  cfg.gridDim = dim3(static_cast<unsigned>(tiles * split));
+  cfg.gridDim = dim3(static_cast<unsigned>(grid));
   cfg.blockDim = dim3(kRowThreads);
   cfg.dynamicSmemBytes = P::kSmemBytes;
   cfg.stream = stream;

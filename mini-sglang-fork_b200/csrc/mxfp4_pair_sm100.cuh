@@ -36,8 +36,7 @@ struct PairTraits {
   static constexpr int kStagingBytes = kEpiWarps * 2048;
   static constexpr int kSmemBytes = 1024 + kStages * kStageBytes + kBarrierBytes + kStagingBytes;
   static_assert(kSmemBytes <= 227 * 1024, "shared memory");
-  // 512 TMEM columns: no other CTA with TMEM may share the SM (MxRowTraits)
-  static_assert(kSmemBytes >= 120 * 1024, "one CTA per SM");
+  static_assert(kSmemBytes > 114 * 1024, "one CTA per SM");  // as for MxRowTraits
 };
 
 __device__ __forceinline__ void cp_scales_pair(uint32_t taddr, uint64_t sdesc) {
@@ -81,39 +80,6 @@ __device__ __forceinline__ void pair_block(const PairArgs& a, int p, int& pm, in
   const int r = p - group * kGroup * a.tiles_n;
   pm = first + r % rows;
   tn = r / rows;
-}
-
-// SiLU epilogue of 32 features of one output row per lane: one MXFP4 block.
-template <typename O>
-__device__ __forceinline__ void silu_chunk(const PairArgs& args, const uint32_t (&gate)[32], const uint32_t (&up)[32],
-                                           int64_t row, int tn, int j) {
-  const MxGemmArgs& g = args.g;
-  const int f0 = tn * 128 + 32 * j;
-  Vec8 y[4];
-#pragma unroll
-  for (int e = 0; e < 16; ++e) {
-    float2 gv = make_float2(__uint_as_float(gate[2 * e]), __uint_as_float(gate[2 * e + 1]));
-    float2 uv = make_float2(__uint_as_float(up[2 * e]), __uint_as_float(up[2 * e + 1]));
-    if (g.bias) {
-      const O* b = static_cast<const O*>(g.bias) + f0 + 2 * e;
-      gv = __fadd2_rn(gv, make_float2(to_float(b[0]), to_float(b[1])));
-      uv = __fadd2_rn(uv, make_float2(to_float(b[g.N]), to_float(b[g.N + 1])));
-    }
-    y[e >> 2].p[e & 3] = silu_mul_fast(gv, uv);
-  }
-  const float m = max3_abs(max3_abs(amax8(y[0]), amax8(y[1]), amax8(y[2])), amax8(y[3]), 0.0f);
-  const int byte = scale_byte(abs_bits(m));
-  const float f = inv_scale(byte);
-  uint32_t w[4];
-#pragma unroll
-  for (int e = 0; e < 4; ++e) w[e] = byte == kNanScale ? 0u : pack8_scaled(y[e], f);
-  if (row < g.M) {
-    const int64_t kt = k_tiles(g.N);
-    *reinterpret_cast<uint4*>(g.q + row * (g.N >> 1) + (f0 >> 1)) = make_uint4(w[0], w[1], w[2], w[3]);
-    uint8_t* s = g.qs + scale_offset(row, tn, kt) + j;
-    *s = static_cast<uint8_t>(byte);
-    if (tn + 1 == args.tiles_n && tn + 1 < kt) s[kTileBytes] = 0;  // the padding tile
-  }
 }
 
 // Plain epilogue of 32 columns (from `col0`) of a warp's 32 rows: through the
@@ -350,14 +316,21 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(PairTraits::kThreads
       if (lane == 0) mbar_arrive_relaxed(free_bar);
       if constexpr (SILU) {
         // columns [0, 128): gate features, [128, 256): their up features
+        const auto block = [&](const uint32_t (&sh)[32], const uint32_t (&own)[32], int j) {
+          float gate[32], up[32];
+#pragma unroll
+          for (int e = 0; e < 32; ++e) {
+            gate[e] = __uint_as_float(acc ? sh[e] : own[e]);
+            up[e] = __uint_as_float(acc ? own[e] : sh[e]);
+          }
+          silu_block<O>(g, gate, up, row0 + lane, tn, j);
+        };
         dev::tmem_ld32(own_t + 32 * hh, v);
         dev::tmem_wait_ld(v);
-        if (acc) silu_chunk<O>(args, s0, v, row0 + lane, tn, hh);
-        else silu_chunk<O>(args, v, s0, row0 + lane, tn, hh);
+        block(s0, v, hh);
         dev::tmem_ld32(own_t + 32 * hh + 64, v);
         dev::tmem_wait_ld(v);
-        if (acc) silu_chunk<O>(args, s1, v, row0 + lane, tn, hh + 2);
-        else silu_chunk<O>(args, v, s1, row0 + lane, tn, hh + 2);
+        block(s1, v, hh + 2);
       } else {
         const int cs = tn * 256 + (acc ? 0 : 128) + 32 * hh, co = tn * 256 + (acc ? 128 : 0) + 32 * hh;
         dev::tmem_ld32(own_t + 32 * hh, v);  // lands while the first chunk is written

@@ -57,15 +57,28 @@ struct Task {
   }
 };
 
-// Stores a warp's scale bytes (one per block, in every lane of the block):
-// the words of k tiles kt and kt + 1, from lanes 0 and 16.
-__device__ __forceinline__ void store_scales(uint8_t* scales, int64_t row, int64_t kt, int64_t ktiles, int lane,
-                                             int byte) {
+// A lane's place in the scale tiles for 256-value group 0 of a row: the word of
+// its k tile (lanes 0-15 the even one, 16-31 the odd one).  Group g is 1024
+// bytes further on.
+__device__ __forceinline__ int64_t scale_word(int64_t row, int64_t ktiles, int lane) {
+  return scale_offset(row, lane >> 4, ktiles);
+}
+
+// Stores a warp's scale bytes (one per block, in every lane of the block) of a
+// group whose words start at `word`.
+__device__ __forceinline__ void store_scales(uint8_t* word, int lane, int byte) {
   uint32_t w = static_cast<uint32_t>(byte);
   w |= __shfl_down_sync(0xffffffffu, w, 4) << 8;
   w |= __shfl_down_sync(0xffffffffu, w, 8) << 16;
-  if ((lane & 15) == 0)
-    *reinterpret_cast<uint32_t*>(scales + scale_offset(row, kt + (lane >> 4), ktiles)) = w;
+  if ((lane & 15) == 0) *reinterpret_cast<uint32_t*>(word) = w;
+}
+
+// Whether a (1 - d) and a (1 + d) lie in different binades (or only one is
+// finite), for a magnitude `a`; `lo` receives the scale byte of the lower.
+__device__ __forceinline__ bool scale_open(float a, float d, int& lo) {
+  const uint32_t l = abs_bits(a * (1.0f - d)), h = abs_bits(a * (1.0f + d));
+  lo = scale_byte(l);
+  return (l ^ h) >> 23;
 }
 
 // Largest magnitude over the four lanes of a block, NaN if one is.
@@ -86,25 +99,23 @@ __global__ void __launch_bounds__(kThreads) quant_kernel(const T* __restrict__ x
   dev::griddep_launch();
   dev::griddep_wait();
   if (t.row >= M) return;
-  const uint4* xr = reinterpret_cast<const uint4*>(x + t.row * ldx);
-  uint32_t* qr = reinterpret_cast<uint32_t*>(data + t.row * (K >> 1));
+  const int v0 = t.g0 * 32 + lane;
+  const uint4* xr = reinterpret_cast<const uint4*>(x + t.row * ldx) + v0;
+  uint32_t* qr = reinterpret_cast<uint32_t*>(data + t.row * (K >> 1)) + v0;
+  uint8_t* sw = scales + scale_word(t.row, kt, lane) + static_cast<int64_t>(t.g0) * 1024;
   uint4 raw[VPT];
 #pragma unroll
-  for (int j = 0; j < VPT; ++j) {
-    const int vi = (t.g0 + j) * 32 + lane;
-    raw[j] = vi < nvec ? __ldcs(xr + vi) : make_uint4(0, 0, 0, 0);
-  }
+  for (int j = 0; j < VPT; ++j) raw[j] = v0 + 32 * j < nvec ? __ldcs(xr + 32 * j) : make_uint4(0, 0, 0, 0);
 #pragma unroll
   for (int j = 0; j < VPT; ++j) {
-    const int vi = (t.g0 + j) * 32 + lane;
     if ((t.g0 + j) * 32 >= nvec) break;  // the whole warp is beyond the row
     uint32_t m = amax8_pair<T>(raw[j]);
     m = max_pair<T>(m, __shfl_xor_sync(0xffffffffu, m, 1));
     m = max_pair<T>(m, __shfl_xor_sync(0xffffffffu, m, 2));
     const int byte = scale_byte(pair_bits<T>(m));
     const uint32_t w = byte == kNanScale ? 0u : pack8_scaled(unpack8<T>(raw[j]), inv_scale(byte));
-    if (vi < nvec) qr[vi] = w;
-    store_scales(scales, t.row, 2 * (t.g0 + j), kt, lane, byte);
+    if (v0 + 32 * j < nvec) qr[32 * j] = w;
+    store_scales(sw + 1024 * j, lane, byte);
   }
 }
 
@@ -189,7 +200,7 @@ __device__ __noinline__ Vec8 silu_far(uint4 graw, uint4 uraw, Vec8 y) {
 }
 
 template <typename T, int VPT>
-__global__ void __launch_bounds__(kThreads) silu_kernel(const T* __restrict__ gate_up, int64_t ld,
+__global__ void __launch_bounds__(kThreads, 3) silu_kernel(const T* __restrict__ gate_up, int64_t ld,
                                                         uint8_t* __restrict__ data, uint8_t* __restrict__ scales,
                                                         int64_t M, int I, Divisor segs) {
   const int lane = threadIdx.x & 31;
@@ -199,19 +210,20 @@ __global__ void __launch_bounds__(kThreads) silu_kernel(const T* __restrict__ ga
   dev::griddep_launch();
   dev::griddep_wait();
   if (t.row >= M) return;
-  const uint4* gr = reinterpret_cast<const uint4*>(gate_up + t.row * ld);
+  const int v0 = t.g0 * 32 + lane;
+  const uint4* gr = reinterpret_cast<const uint4*>(gate_up + t.row * ld) + v0;
   const uint4* ur = gr + nvec;
-  uint32_t* qr = reinterpret_cast<uint32_t*>(data + t.row * (I >> 1));
+  uint32_t* qr = reinterpret_cast<uint32_t*>(data + t.row * (I >> 1)) + v0;
+  uint8_t* sw = scales + scale_word(t.row, kt, lane) + static_cast<int64_t>(t.g0) * 1024;
   uint4 graw[VPT], uraw[VPT];
 #pragma unroll
   for (int j = 0; j < VPT; ++j) {
-    const int vi = (t.g0 + j) * 32 + lane;
-    graw[j] = vi < nvec ? __ldcs(gr + vi) : make_uint4(0, 0, 0, 0);
-    uraw[j] = vi < nvec ? __ldcs(ur + vi) : make_uint4(0, 0, 0, 0);
+    const bool in = v0 + 32 * j < nvec;
+    graw[j] = in ? __ldcs(gr + 32 * j) : make_uint4(0, 0, 0, 0);
+    uraw[j] = in ? __ldcs(ur + 32 * j) : make_uint4(0, 0, 0, 0);
   }
 #pragma unroll
   for (int j = 0; j < VPT; ++j) {
-    const int vi = (t.g0 + j) * 32 + lane;
     if ((t.g0 + j) * 32 >= nvec) break;
     Vec8 y;
     {
@@ -221,8 +233,8 @@ __global__ void __launch_bounds__(kThreads) silu_kernel(const T* __restrict__ ga
       if (far_gate<T>(graw[j])) y = silu_far<T>(graw[j], uraw[j], y);
     }
     const float amax = quad_max(amax8(y));
-    int byte = scale_byte(abs_bits(amax * (1.0f - kSiluDelta)));
-    if (byte != scale_byte(abs_bits(amax * (1.0f + kSiluDelta)))) {
+    int byte;
+    if (scale_open(amax, kSiluDelta, byte)) {
       // next to a power of two: all four lanes of the block come here
       double d = silu_amax_exact<T>(graw[j], uraw[j]);
       const uint32_t quad = 15u << (lane & 28);
@@ -240,8 +252,8 @@ __global__ void __launch_bounds__(kThreads) silu_kernel(const T* __restrict__ ga
       const uint32_t hi = pack8_scaled(y, f * (1.0f + kSiluDelta));
       if (w != hi) w = silu_codes_exact<T>(graw[j], uraw[j], byte, w, hi);
     }
-    if (vi < nvec) qr[vi] = w;
-    store_scales(scales, t.row, 2 * (t.g0 + j), kt, lane, byte);
+    if (v0 + 32 * j < nvec) qr[32 * j] = w;
+    store_scales(sw + 1024 * j, lane, byte);
   }
 }
 
@@ -322,7 +334,7 @@ __device__ __forceinline__ Vec8 norm_input(const uint4& xr, const uint4& rr) {
 }
 
 template <typename T, int VPT, int MAX_THREADS, bool ADD>
-__global__ void __launch_bounds__(MAX_THREADS)
+__global__ void __launch_bounds__(MAX_THREADS, MAX_THREADS <= 256 ? 3 : 1)
     rmsnorm_kernel(const T* __restrict__ x, int64_t ldx, T* residual, int64_t ldr, const T* __restrict__ weight,
                    float eps, uint8_t* __restrict__ data, uint8_t* __restrict__ scales, int K) {
   __shared__ double part[MAX_THREADS / 32];
@@ -377,6 +389,8 @@ __global__ void __launch_bounds__(MAX_THREADS)
   // a row whose mean square nears the ends of fp32's range is taken in 64 bits
   const bool far = !(mean > 1e-30 && mean < 1e30);
   const float r = 1.0f / sqrtf(static_cast<float>(mean));
+  uint8_t* sw = scales + scale_word(row, kt, lane);
+  uint32_t* qr = reinterpret_cast<uint32_t*>(data + row * (K >> 1));
 #pragma unroll
   for (int j = 0; j < VPT; ++j) {
     const int base = (threadIdx.x & ~31) + j * blockDim.x;
@@ -392,8 +406,8 @@ __global__ void __launch_bounds__(MAX_THREADS)
     float am = amax8(y);
     if (vi >= nvec) am = 0.0f;  // a lane beyond the row: 0 times an infinite r is no value of the block
     const float amax = quad_max(am);
-    int byte = scale_byte(abs_bits(amax * (1.0f - kNormDelta)));
-    if (byte != scale_byte(abs_bits(amax * (1.0f + kNormDelta)))) {
+    int byte;
+    if (scale_open(amax, kNormDelta, byte)) {
       double d = norm_amax_exact<T>(xa[j], ra[j], wraw, n);
       const uint32_t quad = 15u << (lane & 28);
 #pragma unroll
@@ -410,8 +424,8 @@ __global__ void __launch_bounds__(MAX_THREADS)
       const uint32_t hi = pack8_scaled(y, f * (1.0f + kNormDelta));
       if (code != hi) code = norm_codes_exact<T>(xa[j], ra[j], wraw, n, byte, code, hi);
     }
-    if (vi < nvec) reinterpret_cast<uint32_t*>(data + row * (K >> 1))[vi] = code;
-    store_scales(scales, row, 2 * (base >> 5), kt, lane, byte);
+    if (vi < nvec) qr[vi] = code;
+    store_scales(sw + base * 32, lane, byte);
   }
 }
 
@@ -438,18 +452,20 @@ __global__ void __launch_bounds__(kThreads) dequant_kernel(const uint8_t* __rest
   dev::griddep_launch();
   dev::griddep_wait();
   if (t.row >= M) return;
-  const uint32_t* qr = reinterpret_cast<const uint32_t*>(data + t.row * (K >> 1));
+  const int v0 = t.g0 * 32 + lane;
+  const uint32_t* qr = reinterpret_cast<const uint32_t*>(data + t.row * (K >> 1)) + v0;
+  const uint8_t* sr = scales + scale_word(t.row, kt, lane) + ((lane >> 2) & 3) + static_cast<int64_t>(t.g0) * 1024;
+  O* dst = out + t.row * K + static_cast<int64_t>(v0) * 8;
   uint32_t w[VPT], s[VPT];
 #pragma unroll
   for (int j = 0; j < VPT; ++j) {
-    const int vi = (t.g0 + j) * 32 + lane;
-    w[j] = vi < nvec ? qr[vi] : 0u;
-    s[j] = vi < nvec ? scales[scale_offset(t.row, vi >> 4, kt) + ((vi >> 2) & 3)] : 0u;
+    const bool in = v0 + 32 * j < nvec;
+    w[j] = in ? __ldcs(qr + 32 * j) : 0u;
+    s[j] = in ? sr[1024 * j] : 0u;
   }
 #pragma unroll
   for (int j = 0; j < VPT; ++j) {
-    const int vi = (t.g0 + j) * 32 + lane;
-    if (vi >= nvec) break;
+    if (v0 + 32 * j >= nvec) break;
     // 2^(s - 127): a subnormal for s = 0, NaN for s = 255
     const float f = s[j] == kNanScale ? __uint_as_float(0x7fffffffu)
                     : s[j] == 0       ? __uint_as_float(0x00400000u)
@@ -463,7 +479,7 @@ __global__ void __launch_bounds__(kThreads) dequant_kernel(const uint8_t* __rest
           : "r"((w[j] >> (8 * b)) & 255u));
       v.p[b] = __fmul2_rn(__half22float2(reinterpret_cast<const __half2&>(h)), make_float2(f, f));
     }
-    store8(out + t.row * K + static_cast<int64_t>(vi) * 8, v);
+    store8(dst + 256 * j, v);
   }
 }
 
@@ -514,44 +530,35 @@ int run_quant(const void* x, int64_t ldx, uint8_t* data, uint8_t* scales, int64_
 
 template <typename T>
 int run_silu(const void* gu, int64_t ld, uint8_t* data, uint8_t* scales, int64_t M, int64_t I, cudaStream_t s) {
-  const int vpt = pick_vpt(M, I) == 4 ? 2 : 1;
+  const int vpt = pick_vpt(M, I);
   uint32_t segs;
   unsigned grid;
   if (int rc = grid_of("mxfp4_silu_mul_quant", M, I, vpt, &segs, &grid)) return rc;
-  auto kern = vpt == 2 ? silu_kernel<T, 2> : silu_kernel<T, 1>;
+  auto kern = vpt == 4 ? silu_kernel<T, 4> : silu_kernel<T, 1>;
   W8A8_CUDA_TRY(launch_pdl(kern, dim3(grid), dim3(kThreads), 0, s, static_cast<const T*>(gu), ld, data, scales, M,
                            static_cast<int>(I), Divisor(segs)));
   return W8A8_OK;
 }
 
 // Threads and vectors per thread of a row: with few rows one vector per thread
-// (the shortest chain), with many up to six, so that a CTA is small and an SM
-// holds many rows at different stages.
+// (the shortest chain), with many four, so that a CTA is small and an SM holds
+// many rows at different stages.
 template <typename T, bool ADD>
 int run_norm(const void* x, int64_t ldx, void* residual, int64_t ldr, const void* weight, float eps, uint8_t* data,
              uint8_t* scales, int64_t M, int64_t K, cudaStream_t s) {
   const int nvec = static_cast<int>(K / 8);
   const bool many = M >= 2 * sm_count();
-  int vpt = (nvec + 1023) / 1024;
-  if (many) vpt = nvec <= 32 ? 1 : nvec <= 6 * 256 ? 6 : vpt;
-  if (many && nvec > 32 && nvec <= 6 * 256) {  // the fewest warps that hold the row, their vectors evened out
-    const int warps = (nvec + 6 * 32 - 1) / (6 * 32);
-    vpt = (nvec + warps * 32 - 1) / (warps * 32);
-  }
+  const int vpt = many || nvec > 2048 ? 4 : nvec > 1024 ? 2 : 1;
   const int threads = ((nvec + vpt - 1) / vpt + 31) / 32 * 32;
 #define MXFP4_NORM(V, THREADS)                                                                                      \
   W8A8_CUDA_TRY(launch_pdl(rmsnorm_kernel<T, V, THREADS, ADD>, dim3(static_cast<unsigned>(M)), dim3(threads), 0, s, \
                            static_cast<const T*>(x), ldx, static_cast<T*>(residual), ldr,                           \
                            static_cast<const T*>(weight), eps, data, scales, static_cast<int>(K)))
-  if (threads > 256) {
-    if (vpt <= 1) MXFP4_NORM(1, 1024); else if (vpt <= 2) MXFP4_NORM(2, 1024); else MXFP4_NORM(4, 1024);
-  } else if (vpt <= 1) {
-    MXFP4_NORM(1, 256);
-  } else if (vpt <= 4) {
-    MXFP4_NORM(4, 256);
-  } else {
-    MXFP4_NORM(6, 256);
-  }
+  if (vpt == 1) MXFP4_NORM(1, 1024);
+  else if (vpt == 2) MXFP4_NORM(2, 1024);
+  else if (threads <= 256) MXFP4_NORM(4, 256);
+  else if (threads <= 512) MXFP4_NORM(4, 512);
+  else MXFP4_NORM(4, 1024);
 #undef MXFP4_NORM
   return W8A8_OK;
 }

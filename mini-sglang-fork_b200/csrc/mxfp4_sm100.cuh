@@ -86,30 +86,14 @@ struct MxGemmArgs {
   long long timeout_ns;
   int M, N, K;       // N: output columns (I with the SiLU epilogue)
   int kblocks;       // 256-value k blocks
-  int ttiles;        // token tiles of the weight-stationary kernel
+  int ttiles, tiles;  // weight-stationary kernel: token tiles, output tiles
 };
 
-// 16 columns of fp32 TMEM
-__device__ __forceinline__ void tmem_ld16f(uint32_t taddr, float (&v)[16]) {
-  uint32_t r[16];
-  asm volatile(
-      "tcgen05.ld.sync.aligned.32x32b.x16.b32 "
-      "{%0, %1, %2, %3, %4, %5, %6, %7, %8, %9, %10, %11, %12, %13, %14, %15}, [%16];"
-      : "=r"(r[0]), "=r"(r[1]), "=r"(r[2]), "=r"(r[3]), "=r"(r[4]), "=r"(r[5]), "=r"(r[6]), "=r"(r[7]), "=r"(r[8]),
-        "=r"(r[9]), "=r"(r[10]), "=r"(r[11]), "=r"(r[12]), "=r"(r[13]), "=r"(r[14]), "=r"(r[15])
-      : "r"(taddr));
-  asm volatile("tcgen05.wait::ld.sync.aligned;"
-               : "+r"(r[0]), "+r"(r[1]), "+r"(r[2]), "+r"(r[3]), "+r"(r[4]), "+r"(r[5]), "+r"(r[6]), "+r"(r[7]),
-                 "+r"(r[8]), "+r"(r[9]), "+r"(r[10]), "+r"(r[11]), "+r"(r[12]), "+r"(r[13]), "+r"(r[14]), "+r"(r[15])
-               :
-               : "memory");
-#pragma unroll
-  for (int j = 0; j < 16; ++j) v[j] = __uint_as_float(r[j]);
-}
-
-__device__ __forceinline__ float ld_dsmem(uint32_t cluster_addr) {
-  float v;
-  asm volatile("ld.shared::cluster.f32 %0, [%1];" : "=f"(v) : "r"(cluster_addr) : "memory");
+__device__ __forceinline__ float4 ld_dsmem4(uint32_t cluster_addr) {
+  float4 v;
+  asm volatile("ld.shared::cluster.v4.f32 {%0, %1, %2, %3}, [%4];"
+               : "=f"(v.x), "=f"(v.y), "=f"(v.z), "=f"(v.w)
+               : "r"(cluster_addr));
   return v;
 }
 
@@ -119,14 +103,64 @@ __device__ __forceinline__ uint32_t cluster_size() {
   return r;
 }
 
+// Asks for a tile to be brought into L2; reads nothing, so it may run ahead of
+// the kernel that is still writing other memory (or even that tile: L2 is
+// where both meet).
+__device__ __forceinline__ void tma_prefetch_2d(const void* tmap, int32_t x, int32_t y) {
+  asm volatile("cp.async.bulk.prefetch.tensor.2d.L2.global.tile [%0, {%1, %2}];" ::"l"(
+                   reinterpret_cast<uint64_t>(tmap)),
+               "r"(x), "r"(y)
+               : "memory");
+}
+
+// silu(gate) * up of 32 features (block `j` of 128-feature tile `ft`) of one
+// output row, as one MXFP4 block.  Here the sums themselves carry fp32's
+// rounding, so the product is quantised as it comes, in one conversion.
+template <typename O>
+__device__ __forceinline__ void silu_block(const MxGemmArgs& g, const float (&gate)[32], const float (&up)[32],
+                                           int64_t row, int ft, int j) {
+  const int f0 = ft * 128 + 32 * j;
+  Vec8 y[4];
+#pragma unroll
+  for (int e = 0; e < 16; ++e) {
+    float2 gv = make_float2(gate[2 * e], gate[2 * e + 1]);
+    float2 uv = make_float2(up[2 * e], up[2 * e + 1]);
+    if (g.bias) {
+      const O* b = static_cast<const O*>(g.bias) + f0 + 2 * e;
+      gv = __fadd2_rn(gv, make_float2(to_float(b[0]), to_float(b[1])));
+      uv = __fadd2_rn(uv, make_float2(to_float(b[g.N]), to_float(b[g.N + 1])));
+    }
+    y[e >> 2].p[e & 3] = silu_mul_fast(gv, uv);
+  }
+  const float m = max3_abs(max3_abs(amax8(y[0]), amax8(y[1]), amax8(y[2])), amax8(y[3]), 0.0f);
+  const int byte = scale_byte(abs_bits(m));
+  const float f = inv_scale(byte);
+  uint32_t w[4];
+#pragma unroll
+  for (int e = 0; e < 4; ++e) w[e] = byte == kNanScale ? 0u : pack8_scaled(y[e], f);
+  if (row < g.M) {
+    const int64_t kt = k_tiles(g.N);
+    *reinterpret_cast<uint4*>(g.q + row * (g.N >> 1) + (f0 >> 1)) = make_uint4(w[0], w[1], w[2], w[3]);
+    uint8_t* s = g.qs + scale_offset(row, ft, kt) + j;
+    *s = static_cast<uint8_t>(byte);
+    if ((ft + 1) * 128 == g.N && ft + 1 < kt) s[kTileBytes] = 0;  // the padding tile
+  }
+}
+
 // ------------------------------------------------- weight-stationary kernel
-// One CTA computes 128 output columns (weight rows, on the MMA's 128-row side)
-// for T tokens; with the SiLU epilogue 128 gate rows and the 128 up rows that
-// belong to them, in two accumulators.  A cluster of S CTAs splits K: each
-// leaves its fp32 partial sums in its own shared memory and, after a cluster
-// barrier, CTA r adds the S shares of tokens r, r + S, ... in rank order
-// through distributed shared memory and writes them, so the sum's order is
-// fixed and nothing is left in memory between calls.
+// For up to 128 tokens per tile.  One CTA computes 128 output columns (weight
+// rows, on the MMA's 128-row side) for T tokens; with the SiLU epilogue 128
+// gate rows and the 128 up rows that belong to them, in two accumulators.
+// The weights are read once, at the rate of HBM, which is what bounds it; the
+// ring (about 200 KB, the SM's whole shared memory) is there to keep enough of
+// them in flight.
+//
+// With enough tiles the CTAs are persistent and the accumulators doubled, so
+// that a tile's epilogue overlaps the next one's loads and MMAs.  With few, a
+// cluster of S CTAs splits K: each leaves its fp32 sums in its own shared
+// memory and, after a cluster barrier, CTA r adds the S shares of tokens r,
+// r + S, ... in rank order through distributed shared memory and writes them.
+// The order of the sum is fixed, and nothing is left in memory between calls.
 template <int T, bool SILU>
 struct MxRowTraits {
   static constexpr int kTiles = SILU ? 2 : 1;  // weight tiles (gate, up)
@@ -135,65 +169,48 @@ struct MxRowTraits {
   static constexpr int kSf = 1024;             // scale bytes of 128 rows per k block
   static constexpr int kStageBytes = kTiles * (kW + kSf) + kX + kSf;
   static constexpr int kSfCols = 8 * (kTiles + 1);  // TMEM columns of a stage's scales
-  static constexpr int kStages = SILU ? (T <= 32 ? 3 : T == 64 ? 4 : 4) : (T <= 32 ? 3 : T == 64 ? 4 : 3);
+  static constexpr int kStages = SILU ? (T == 16 ? 5 : T == 128 ? 3 : 4) : (T <= 32 ? 10 : T == 64 ? 8 : 6);
+  static constexpr int kChunk = T < 32 ? T : 32;  // columns that the epilogue takes at a time
   static constexpr int kAccCols = kTiles * T;
-  static constexpr int kColsNeeded = kAccCols + kStages * kSfCols;
-  static constexpr int kTmemCols = kColsNeeded <= 64 ? 64 : kColsNeeded <= 128 ? 128 : kColsNeeded <= 256 ? 256 : 512;
+  static constexpr int kAccs = 2 * kAccCols + kStages * kSfCols <= 512 ? 2 : 1;
+  static constexpr int kColsNeeded = kAccs * kAccCols + kStages * kSfCols;
+  static constexpr int kTmemCols = kColsNeeded <= 128 ? 128 : kColsNeeded <= 256 ? 256 : 512;
   static constexpr int kBarrierBytes = 256;
-  static constexpr int kUsedBytes = 1024 + kStages * kStageBytes + kBarrierBytes;
-  // At least the share of the SM's 228 KB that the kernel takes of its 512 TMEM
-  // columns (less the 1 KB that every CTA gets anyway): then whatever mix of
-  // this library's CTAs an SM holds, their TMEM allocations fit together, and
-  // no CTA of a cluster waits for columns that a CTA waiting for it holds.
-  static constexpr int kShare = kTmemCols * 456 - 1024;
-  static constexpr int kSmemBytes = kUsedBytes > kShare ? kUsedBytes : kShare;
+  static constexpr int kStagingBytes = SILU ? 4 * 2 * kChunk * 128 : 0;  // per epilogue warp: gate, up
+  static constexpr int kSmemBytes = 1024 + kStages * kStageBytes + kBarrierBytes + kStagingBytes;
   static_assert(kColsNeeded <= 512, "TMEM");
   static_assert(kSmemBytes <= 227 * 1024, "shared memory");
+  // More than half of the SM's shared memory: no second CTA of this library
+  // that holds TMEM fits beside it, so no CTA of a cluster waits for TMEM that
+  // a CTA waiting for it holds.
+  static_assert(kSmemBytes > 114 * 1024, "one CTA per SM");
   static_assert(kTiles * T * 128 * 4 <= kStages * kStageBytes, "the partial sums reuse the ring");
 };
 
 constexpr int kRowThreads = 192;  // producer, MMA, four epilogue warps
 
-// One output value (or, SiLU, one block of 32 outputs over the warp) for
-// output column `col` = this lane's, token `t` (uniform over the warp).
-template <typename O, bool SILU>
-__device__ __forceinline__ void emit(const MxGemmArgs& a, int t, int col, int lane, float g, float u, float bg,
-                                     float bu) {
-  if constexpr (!SILU) {
-    if (col < a.N) {
-      O* c = static_cast<O*>(a.out) + static_cast<int64_t>(t) * a.N + col;
-      if constexpr (sizeof(O) == 2) {
-        const uint32_t p = pack2<O>(g + bg, 0.0f);
-        *reinterpret_cast<uint16_t*>(c) = static_cast<uint16_t>(p);
-      }
-    }
-  } else {
-    // the warp's 32 columns are one block of the result (I % 128 == 0)
-    const float y = silu_mul_fast(g + bg, u + bu);
-    const uint32_t m = __reduce_max_sync(0xffffffffu, abs_bits(y));
-    const int byte = scale_byte(m);
-    uint32_t w = byte == kNanScale ? 0u : code_of(y * inv_scale(byte)) << (4 * (lane & 7));
-    w |= __shfl_xor_sync(0xffffffffu, w, 1);
-    w |= __shfl_xor_sync(0xffffffffu, w, 2);
-    w |= __shfl_xor_sync(0xffffffffu, w, 4);
-    const int c0 = col - lane;
-    if ((lane & 7) == 0)
-      *reinterpret_cast<uint32_t*>(a.q + static_cast<int64_t>(t) * (a.N >> 1) + ((c0 + lane) >> 1)) = w;
-    if (lane == 0) {
-      const int64_t kt = k_tiles(a.N);
-      uint8_t* s = a.qs + scale_offset(t, c0 >> 7, kt) + ((c0 >> 5) & 3);
-      *s = static_cast<uint8_t>(byte);
-      if ((c0 >> 7) + 1 == (a.N >> 7) && ((a.N >> 7) & 1)) s[kTileBytes] = 0;  // the padding tile
-    }
-  }
+// Word offset of column n of token t in a [token][128] fp32 array whose 16-byte
+// pieces are XORed with the token: a warp writes 32 columns of one token, or
+// reads the same piece of 8 tokens, without bank conflicts.
+__device__ __forceinline__ uint32_t part_word(int t, int n) {
+  return static_cast<uint32_t>(t * 128 + ((((n >> 2) ^ (t & 7)) << 2) | (n & 3)));
+}
+
+template <int CH>
+__device__ __forceinline__ void tmem_ld_chunk(uint32_t taddr, float (&v)[32]) {
+  uint32_t r[32];
+  dev::tmem_ld<CH>(taddr, r);
+  dev::tmem_wait_ld(r);
+#pragma unroll
+  for (int j = 0; j < CH; ++j) v[j] = __uint_as_float(r[j]);
 }
 
 template <typename O, int T, bool SILU>
-__global__ void __launch_bounds__(kRowThreads) mx_row_kernel(const __grid_constant__ CUtensorMap tm_w,
-                                                             const __grid_constant__ CUtensorMap tm_ws,
-                                                             const __grid_constant__ CUtensorMap tm_x,
-                                                             const __grid_constant__ CUtensorMap tm_xs,
-                                                             const MxGemmArgs args) {
+__global__ void __launch_bounds__(kRowThreads, 1) mx_row_kernel(const __grid_constant__ CUtensorMap tm_w,
+                                                                const __grid_constant__ CUtensorMap tm_ws,
+                                                                const __grid_constant__ CUtensorMap tm_x,
+                                                                const __grid_constant__ CUtensorMap tm_xs,
+                                                                const MxGemmArgs args) {
   using P = MxRowTraits<T, SILU>;
   extern __shared__ __align__(1024) uint8_t smem_raw[];
   uint8_t* smem = reinterpret_cast<uint8_t*>((reinterpret_cast<uintptr_t>(smem_raw) + 1023) & ~uintptr_t(1023));
@@ -205,18 +222,19 @@ __global__ void __launch_bounds__(kRowThreads) mx_row_kernel(const __grid_consta
   uint64_t* bars = reinterpret_cast<uint64_t*>(s_xs + P::kStages * P::kSf);
   uint64_t* full = bars;
   uint64_t* empty = bars + P::kStages;
-  uint64_t* acc_full = bars + 2 * P::kStages;
-  uint32_t* tmem_slot = reinterpret_cast<uint32_t*>(acc_full + 1);
+  uint64_t* acc_full = bars + 2 * P::kStages;  // [2]
+  uint64_t* acc_empty = acc_full + 2;          // [2]
+  uint64_t* drain = acc_empty + 2;
+  uint32_t* tmem_slot = reinterpret_cast<uint32_t*>(drain + 1);
   volatile int* abort_flag = reinterpret_cast<volatile int*>(tmem_slot + 1);
-  float* part = reinterpret_cast<float*>(smem);  // [tile][token][128], after the ring is done
+  float* part = reinterpret_cast<float*>(smem);  // [gate / up][token][128], after the ring is done (S > 1)
 
   const int warp = threadIdx.x >> 5;
   const int lane = threadIdx.x & 31;
   const int S = static_cast<int>(cluster_size());
   const int rank = static_cast<int>(dev::cluster_rank());
-  const int tile = blockIdx.x / S;
-  const int tt = tile % args.ttiles;
-  const int wt = tile / args.ttiles;
+  const int first = blockIdx.x / S;
+  const int step = gridDim.x / S;  // (S > 1: one tile per cluster)
   const int kb0 = static_cast<int>(static_cast<int64_t>(rank) * args.kblocks / S);
   const int kb1 = static_cast<int>(static_cast<int64_t>(rank + 1) * args.kblocks / S);
   const long long tmo = args.timeout_ns;
@@ -226,7 +244,11 @@ __global__ void __launch_bounds__(kRowThreads) mx_row_kernel(const __grid_consta
       dev::mbar_init(dev::smem_u32(full + s), 1);
       dev::mbar_init(dev::smem_u32(empty + s), 1);
     }
-    dev::mbar_init(dev::smem_u32(acc_full), 1);
+    for (int s = 0; s < 2; ++s) {
+      dev::mbar_init(dev::smem_u32(acc_full + s), 1);
+      dev::mbar_init(dev::smem_u32(acc_empty + s), 4);  // the epilogue warps
+    }
+    dev::mbar_init(dev::smem_u32(drain), 1);
     *abort_flag = 0;
     dev::fence_mbar_init();
     dev::prefetch_tmap(&tm_w);
@@ -238,37 +260,55 @@ __global__ void __launch_bounds__(kRowThreads) mx_row_kernel(const __grid_consta
     dev::tmem_alloc(dev::smem_u32(tmem_slot), P::kTmemCols);
     dev::tmem_relinquish();
   }
+  dev::griddep_launch();
+  if (warp == 0 && first < args.tiles) {
+    // the first stages' weights into L2 while the previous kernel ends
+    if (elect_one()) {
+      for (int kb = kb0; kb < min(kb1, kb0 + P::kStages); ++kb)
+#pragma unroll
+        for (int h = 0; h < P::kTiles; ++h) {
+          const int w0 = first / args.ttiles * 128 + h * args.N;
+          tma_prefetch_2d(&tm_w, kb * 128, w0);
+          tma_prefetch_2d(&tm_ws, kb * 256, w0 >> 7);
+        }
+    }
+    __syncwarp();
+  }
   dev::tc_fence_before();
   __syncthreads();
   dev::tc_fence_after();
   const uint32_t tmem = __shfl_sync(0xffffffffu, *tmem_slot, 0);  // (the same in every lane, and known to be)
-  dev::griddep_launch();
   dev::griddep_wait();  // any operand may be the previous kernel's output
 
   if (warp == 0) {
     // ------------------------------------------------------------ producer
     int stage = 0;
     uint32_t phase = 0, issued_mask = 0, issued_phase = 0;
-    for (int kb = kb0; kb < kb1; ++kb) {
-      if (!warp_wait(dev::smem_u32(empty + stage), phase ^ 1u, abort_flag, args.err, tmo)) break;
-      if (elect_one()) {
-        const uint32_t bar = dev::smem_u32(full + stage);
-        dev::mbar_expect_tx(bar, P::kStageBytes);
+    bool ok = true;
+    for (int tile = first; ok && tile < args.tiles; tile += step) {
+      const int tt = tile % args.ttiles, wt = tile / args.ttiles;
+      for (int kb = kb0; kb < kb1; ++kb) {
+        ok = warp_wait(dev::smem_u32(empty + stage), phase ^ 1u, abort_flag, args.err, tmo);
+        if (!ok) break;
+        if (elect_one()) {
+          const uint32_t bar = dev::smem_u32(full + stage);
+          dev::mbar_expect_tx(bar, P::kStageBytes);
 #pragma unroll
-        for (int h = 0; h < P::kTiles; ++h) {
-          const int w0 = wt * 128 + h * args.N;  // gate rows, then up rows
-          dev::tma_load_2d(dev::smem_u32(s_w + (stage * P::kTiles + h) * P::kW), &tm_w, bar, kb * 128, w0);
-          dev::tma_load_2d(dev::smem_u32(s_ws + (stage * P::kTiles + h) * P::kSf), &tm_ws, bar, kb * 256, w0 >> 7);
+          for (int h = 0; h < P::kTiles; ++h) {
+            const int w0 = wt * 128 + h * args.N;  // gate rows, then up rows
+            dev::tma_load_2d(dev::smem_u32(s_w + (stage * P::kTiles + h) * P::kW), &tm_w, bar, kb * 128, w0);
+            dev::tma_load_2d(dev::smem_u32(s_ws + (stage * P::kTiles + h) * P::kSf), &tm_ws, bar, kb * 256, w0 >> 7);
+          }
+          dev::tma_load_2d(dev::smem_u32(s_x + stage * P::kX), &tm_x, bar, kb * 128, tt * T);
+          dev::tma_load_2d(dev::smem_u32(s_xs + stage * P::kSf), &tm_xs, bar, kb * 256, (tt * T) >> 7);
         }
-        dev::tma_load_2d(dev::smem_u32(s_x + stage * P::kX), &tm_x, bar, kb * 128, tt * T);
-        dev::tma_load_2d(dev::smem_u32(s_xs + stage * P::kSf), &tm_xs, bar, kb * 256, (tt * T) >> 7);
-      }
-      __syncwarp();
-      issued_mask |= 1u << stage;
-      issued_phase = (issued_phase & ~(1u << stage)) | (phase << stage);
-      if (++stage == P::kStages) {
-        stage = 0;
-        phase ^= 1u;
+        __syncwarp();
+        issued_mask |= 1u << stage;
+        issued_phase = (issued_phase & ~(1u << stage)) | (phase << stage);
+        if (++stage == P::kStages) {
+          stage = 0;
+          phase ^= 1u;
+        }
       }
     }
     if (lane == 0)
@@ -279,92 +319,189 @@ __global__ void __launch_bounds__(kRowThreads) mx_row_kernel(const __grid_consta
   } else if (warp == 1) {
     // ----------------------------------------------------------------- MMA
     int stage = 0;
-    uint32_t phase = 0;
-    for (int kb = kb0; kb < kb1; ++kb) {
-      if (!warp_wait(dev::smem_u32(full + stage), phase, abort_flag, args.err, tmo)) break;
+    uint32_t phase = 0, i = 0;
+    bool ok = true;
+    for (int tile = first; ok && tile < args.tiles; tile += step, ++i) {
+      const uint32_t acc = i % P::kAccs, use = i / P::kAccs;
+      if (!warp_wait(dev::smem_u32(acc_empty + acc), (use & 1u) ^ 1u, abort_flag, args.err, tmo)) break;
       dev::tc_fence_after();
-      if (elect_one()) {
-        // each stage has its own scale columns: free again once the MMAs that
-        // read them have arrived on `empty`
-        const uint32_t sf = tmem + P::kAccCols + stage * P::kSfCols;
+      const uint32_t d = tmem + acc * P::kAccCols;
+      for (int kb = kb0; kb < kb1; ++kb) {
+        ok = warp_wait(dev::smem_u32(full + stage), phase, abort_flag, args.err, tmo);
+        if (!ok) break;
+        dev::tc_fence_after();
+        if (elect_one()) {
+          // each stage has its own scale columns: free again once the MMAs that
+          // read them have arrived on `empty`
+          const uint32_t sf = tmem + P::kAccs * P::kAccCols + stage * P::kSfCols;
 #pragma unroll
-        for (int c = 0; c < 2; ++c) {
-          cp_scales(sf + 4 * c, sdesc_scales(dev::smem_u32(s_xs + stage * P::kSf + c * kTileBytes)));
+          for (int c = 0; c < 2; ++c) {
+            cp_scales(sf + 4 * c, sdesc_scales(dev::smem_u32(s_xs + stage * P::kSf + c * kTileBytes)));
 #pragma unroll
-          for (int h = 0; h < P::kTiles; ++h)
-            cp_scales(sf + 8 * (h + 1) + 4 * c,
-                      sdesc_scales(dev::smem_u32(s_ws + (stage * P::kTiles + h) * P::kSf + c * kTileBytes)));
+            for (int h = 0; h < P::kTiles; ++h)
+              cp_scales(sf + 8 * (h + 1) + 4 * c,
+                        sdesc_scales(dev::smem_u32(s_ws + (stage * P::kTiles + h) * P::kSf + c * kTileBytes)));
+          }
+          const uint64_t dx = dev::sdesc_k_sw128(dev::smem_u32(s_x + stage * P::kX));
+          const int steps = min(4, (args.K - kb * 256 + 63) / 64);  // beyond K: nothing to add
+#pragma unroll
+          for (int k = 0; k < 4; ++k) {
+            if (k >= steps) break;
+            constexpr uint32_t ids[2] = {idesc_mxf4(128, T, 0), idesc_mxf4(128, T, 2)};
+#pragma unroll
+            for (int h = 0; h < P::kTiles; ++h) {
+              const uint64_t dw = dev::sdesc_k_sw128(dev::smem_u32(s_w + (stage * P::kTiles + h) * P::kW));
+              mma_mxf4(d + h * T, dw + 2 * k, dx + 2 * k, ids[k & 1], sf + 8 * (h + 1) + 4 * (k >> 1),
+                       sf + 4 * (k >> 1), (kb > kb0 || k > 0) ? 1u : 0u);
+            }
+          }
+          dev::tc_commit(dev::smem_u32(empty + stage));
         }
-        const uint64_t dx = dev::sdesc_k_sw128(dev::smem_u32(s_x + stage * P::kX));
-        const int steps = min(4, (args.K - kb * 256 + 63) / 64);  // beyond K: nothing to add
-#pragma unroll
-        for (int k = 0; k < 4; ++k) {
-          if (k >= steps) break;
-          constexpr uint32_t ids[2] = {idesc_mxf4(128, T, 0), idesc_mxf4(128, T, 2)};
+        __syncwarp();
+        if (++stage == P::kStages) {
+          stage = 0;
+          phase ^= 1u;
+        }
+      }
+      if (!ok) break;
+      if (elect_one()) dev::tc_commit(dev::smem_u32(acc_full + acc));
+      __syncwarp();
+    }
+    if (elect_one()) dev::tc_commit(dev::smem_u32(drain));
+    if (lane == 0 && !dev::mbar_wait_drain(dev::smem_u32(drain), 0, tmo))
+      if (args.err) atomicOr(args.err, kErrGemmDrain);
+  } else {
+    // ------------------------------------------------------------ epilogue
+    const int q = warp & 3;  // TMEM lane quarter of this warp: 32 of the tile's columns
+    const int n = q * 32 + lane;
+    const uint32_t lanes = static_cast<uint32_t>(q * 32) << 16;
+    float* stg = reinterpret_cast<float*>(reinterpret_cast<uint8_t*>(bars) + P::kBarrierBytes +
+                                          q * (P::kStagingBytes / 4));
+    uint32_t i = 0;
+    for (int tile = first; tile < args.tiles; tile += step, ++i) {
+      const int tt = tile % args.ttiles, wt = tile / args.ttiles;
+      const int tokens = min(T, args.M - tt * T);
+      const uint32_t acc = i % P::kAccs, use = i / P::kAccs;
+      // (a failed wait leaves the result unspecified; the error word says so)
+      if (!warp_wait(dev::smem_u32(acc_full + acc), use & 1u, abort_flag, args.err, tmo)) break;
+      dev::tc_fence_after();
+      const uint32_t t_acc = tmem + lanes + acc * P::kAccCols;
+      if (S > 1) {
+        for (int c = 0; c < tokens; c += P::kChunk) {
 #pragma unroll
           for (int h = 0; h < P::kTiles; ++h) {
-            const uint64_t dw = dev::sdesc_k_sw128(dev::smem_u32(s_w + (stage * P::kTiles + h) * P::kW));
-            mma_mxf4(tmem + h * T, dw + 2 * k, dx + 2 * k, ids[k & 1], sf + 8 * (h + 1) + 4 * (k >> 1),
-                     sf + 4 * (k >> 1), (kb > kb0 || k > 0) ? 1u : 0u);
+            float v[32];
+            tmem_ld_chunk<P::kChunk>(t_acc + h * T + c, v);
+#pragma unroll
+            for (int j = 0; j < P::kChunk; ++j) part[h * T * 128 + part_word(c + j, n)] = v[j];
           }
         }
-        dev::tc_commit(dev::smem_u32(empty + stage));
+        break;
       }
-      __syncwarp();
-      if (++stage == P::kStages) {
-        stage = 0;
-        phase ^= 1u;
-      }
-    }
-    if (elect_one()) dev::tc_commit(dev::smem_u32(acc_full));
-    if (lane == 0 && !dev::mbar_wait_drain(dev::smem_u32(acc_full), 0, tmo))
-      if (args.err) atomicOr(args.err, kErrGemmDrain);
-  }
-  __syncwarp();
-  const int tokens = min(T, args.M - tt * T);
-  const int q = warp & 3;  // TMEM lane quarter of this warp
-  const int n = q * 32 + lane;
-  const int col = wt * 128 + n;
-  float bg = 0.0f, bu = 0.0f;
-  if (warp >= 2) {
-    if (args.bias && col < args.N) {
-      bg = to_float(static_cast<const O*>(args.bias)[col]);
-      if constexpr (SILU) bu = to_float(static_cast<const O*>(args.bias)[args.N + col]);
-    }
-    // (a failed wait leaves the result unspecified; the error word says so)
-    dev::mbar_wait(dev::smem_u32(acc_full), 0, abort_flag, args.err, kErrGemmWait, tmo);
-    dev::tc_fence_after();
-    __syncwarp();
-    const uint32_t lanes = static_cast<uint32_t>(q * 32) << 16;
-    for (int c = 0; c < tokens; c += 16) {
-      float g[16], u[16];
-      tmem_ld16f(tmem + lanes + c, g);
-      if constexpr (SILU) tmem_ld16f(tmem + lanes + T + c, u);
-      if (S == 1) {
+      if constexpr (!SILU) {
+        const int col = wt * 128 + n;
+        const bool in = col < args.N;
+        const float bias = args.bias && in ? to_float(static_cast<const O*>(args.bias)[col]) : 0.0f;
+        O* out = static_cast<O*>(args.out) + static_cast<int64_t>(tt) * T * args.N + col;
+        for (int c = 0; c < tokens; c += P::kChunk) {
+          float v[32];
+          tmem_ld_chunk<P::kChunk>(t_acc + c, v);
 #pragma unroll
-        for (int j = 0; j < 16; ++j)
-          if (c + j < tokens) emit<O, SILU>(args, tt * T + c + j, col, lane, g[j], SILU ? u[j] : 0.0f, bg, bu);
+          for (int j = 0; j < P::kChunk; ++j)
+            if (c + j < tokens && in) {
+              const uint32_t p = pack2<O>(v[j] + bias, 0.0f);
+              *reinterpret_cast<uint16_t*>(out + static_cast<int64_t>(c + j) * args.N) = static_cast<uint16_t>(p);
+            }
+        }
       } else {
+        // a warp's 32 features are one block of the result: 32 tokens at a
+        // time are transposed through shared memory, then a lane has a block
+        for (int c = 0; c < tokens; c += P::kChunk) {
+          float g[32], u[32];
+          tmem_ld_chunk<P::kChunk>(t_acc + c, g);
+          tmem_ld_chunk<P::kChunk>(t_acc + T + c, u);
 #pragma unroll
-        for (int j = 0; j < 16; ++j) {
-          part[(c + j) * 128 + n] = g[j];
-          if constexpr (SILU) part[(T + c + j) * 128 + n] = u[j];
+          for (int j = 0; j < P::kChunk; ++j) {
+            const int w = j * 32 + ((((lane >> 2) ^ (j & 7)) << 2) | (lane & 3));
+            stg[w] = g[j];
+            stg[P::kChunk * 32 + w] = u[j];
+          }
+          __syncwarp();
+          if (lane < P::kChunk && c + lane < tokens) {
+#pragma unroll
+            for (int e = 0; e < 8; ++e) {
+              const int w = lane * 32 + ((e ^ (lane & 7)) << 2);
+              *reinterpret_cast<float4*>(g + 4 * e) = *reinterpret_cast<const float4*>(stg + w);
+              *reinterpret_cast<float4*>(u + 4 * e) = *reinterpret_cast<const float4*>(stg + P::kChunk * 32 + w);
+            }
+            silu_block<O>(args, g, u, static_cast<int64_t>(tt) * T + c + lane, wt, q);
+          }
+          __syncwarp();
         }
       }
+      dev::tc_fence_before();
+      __syncwarp();
+      if (lane == 0) dev::mbar_arrive(dev::smem_u32(acc_empty + acc));
     }
     dev::tc_fence_before();
   }
   if (S > 1) {
     dev::cluster_sync();  // every share is in its CTA's shared memory
     if (warp >= 2) {
-      for (int t = rank; t < tokens; t += S) {
-        float g = 0.0f, u = 0.0f;
-        for (int s = 0; s < S; ++s) {
-          const uint32_t base = dev::mapa(dev::smem_u32(part), static_cast<uint32_t>(s));
-          g += ld_dsmem(base + static_cast<uint32_t>(t * 128 + n) * 4);
-          if constexpr (SILU) u += ld_dsmem(base + static_cast<uint32_t>((T + t) * 128 + n) * 4);
+      const int tt = first % args.ttiles, wt = first / args.ttiles;
+      const int tokens = min(T, args.M - tt * T);
+      const int mine = (tokens - rank + S - 1) / S;  // tokens rank, rank + S, ...
+      const int et = threadIdx.x - 64;
+      const uint32_t local = dev::smem_u32(part);
+      if constexpr (!SILU) {
+        // an item: 8 columns of a token
+        for (int it = et; it < mine * 16; it += 128) {
+          const int t = rank + S * (it >> 4), n0 = (it & 15) * 8;
+          const uint32_t a0 = local + 4 * part_word(t, n0), a1 = local + 4 * part_word(t, n0 + 4);
+          float v[8] = {0, 0, 0, 0, 0, 0, 0, 0};
+#pragma unroll 4
+          for (int s = 0; s < S; ++s) {
+            const float4 x = ld_dsmem4(dev::mapa(a0, s)), y = ld_dsmem4(dev::mapa(a1, s));
+            v[0] += x.x, v[1] += x.y, v[2] += x.z, v[3] += x.w;
+            v[4] += y.x, v[5] += y.y, v[6] += y.z, v[7] += y.w;
+          }
+          const int col = wt * 128 + n0;
+          O* dst = static_cast<O*>(args.out) + (static_cast<int64_t>(tt) * T + t) * args.N + col;
+          if (args.bias) {
+            const O* b = static_cast<const O*>(args.bias) + col;
+#pragma unroll
+            for (int j = 0; j < 8; ++j)
+              if (col + j < args.N) v[j] += to_float(b[j]);
+          }
+          const uint32_t w[4] = {pack2<O>(v[0], v[1]), pack2<O>(v[2], v[3]), pack2<O>(v[4], v[5]),
+                                 pack2<O>(v[6], v[7])};
+          if ((args.N & 7) == 0) {
+            if (col < args.N) *reinterpret_cast<uint4*>(dst) = make_uint4(w[0], w[1], w[2], w[3]);
+          } else {
+#pragma unroll
+            for (int j = 0; j < 8; ++j)
+              if (col + j < args.N)
+                reinterpret_cast<uint16_t*>(dst)[j] = static_cast<uint16_t>(w[j >> 1] >> (16 * (j & 1)));
+          }
         }
-        emit<O, SILU>(args, tt * T + t, col, lane, g, u, bg, bu);
+      } else {
+        // an item: one 32-feature block of a token
+        for (int it = et; it < mine * 4; it += 128) {
+          const int t = rank + S * (it >> 2), j = it & 3;
+          float g[32], u[32];
+#pragma unroll
+          for (int e = 0; e < 32; ++e) g[e] = u[e] = 0.0f;
+          for (int s = 0; s < S; ++s) {
+#pragma unroll
+            for (int e = 0; e < 8; ++e) {
+              const uint32_t w = local + 4 * part_word(t, 32 * j + 4 * e);
+              const float4 x = ld_dsmem4(dev::mapa(w, s)), y = ld_dsmem4(dev::mapa(w + 4 * T * 128, s));
+              g[4 * e] += x.x, g[4 * e + 1] += x.y, g[4 * e + 2] += x.z, g[4 * e + 3] += x.w;
+              u[4 * e] += y.x, u[4 * e + 1] += y.y, u[4 * e + 2] += y.z, u[4 * e + 3] += y.w;
+            }
+          }
+          silu_block<O>(args, g, u, static_cast<int64_t>(tt) * T + t, wt, j);
+        }
       }
     }
     dev::cluster_sync();  // no CTA leaves while a peer still reads its share
