@@ -60,24 +60,48 @@ int active_clusters(int s, int threads, int smem, int* out) {
   return W8A8_OK;
 }
 
-// CTAs that share an output tile's K: as many as leave every tile's cluster
-// resident at once (a second wave would cost as much as the first), with two k
-// blocks each at least, at most a portable cluster's 8.
+// Launch in clusters of `cluster` CTAs, with programmatic stream serialisation.
+template <typename Kernel, typename... Args>
+int launch_cluster(Kernel kern, unsigned grid, int threads, int smem, int cluster, cudaStream_t stream,
+                   const Args&... args) {
+  cudaLaunchConfig_t cfg = {};
+  cfg.gridDim = dim3(grid);
+  cfg.blockDim = dim3(static_cast<unsigned>(threads));
+  cfg.dynamicSmemBytes = static_cast<size_t>(smem);
+  cfg.stream = stream;
+  cudaLaunchAttribute attr[2];
+  attr[0].id = cudaLaunchAttributeProgrammaticStreamSerialization;
+  attr[0].val.programmaticStreamSerializationAllowed = 1;
+  attr[1].id = cudaLaunchAttributeClusterDimension;
+  attr[1].val.clusterDim.x = static_cast<unsigned>(cluster);
+  attr[1].val.clusterDim.y = 1;
+  attr[1].val.clusterDim.z = 1;
+  cfg.attrs = attr;
+  cfg.numAttrs = 2;
+  W8A8_CUDA_TRY(cudaLaunchKernelEx(&cfg, kern, args...));
+  return W8A8_OK;
+}
+
+// Shares of K per output tile, each the work of `ctas` CTAs: as many as leave
+// every tile's cluster resident at once (a second wave would cost as much as
+// the first), `most` at most, with `least` k blocks each (measured, B200: the
+// exchange costs 2 us for 128 tokens, and more than it saves below two k
+// blocks, six with the SiLU epilogue's two sums, eight for a 256 x 256 block).
 template <auto Kern>
-int pick_split(int64_t tiles, int kblocks, int threads, int smem, int* out) {
+int pick_split(int64_t tiles, int kblocks, int threads, int smem, int ctas, int most, int least, int* out) {
   *out = 1;
-  for (int s = 2; s <= std::min(8, kblocks / 2) && tiles * s <= sm_count(); ++s) {
+  for (int s = 2; s <= std::min(most, kblocks / least) && tiles * s * ctas <= sm_count(); ++s) {
     int n = 0;
-    if (int rc = active_clusters<Kern>(s, threads, smem, &n)) return rc;
+    if (int rc = active_clusters<Kern>(s * ctas, threads, smem, &n)) return rc;
     if (tiles <= n) *out = s;
   }
   return W8A8_OK;
 }
 
-template <typename O, int T, bool SILU>
+template <typename O, int T, bool SILU, bool DEEP>
 int launch_row(const Operands& o, MxGemmArgs args, cudaStream_t stream) {
-  using P = MxRowTraits<T, SILU>;
-  constexpr auto kern = mx_row_kernel<O, T, SILU>;
+  using P = MxRowTraits<T, SILU, DEEP>;
+  constexpr auto kern = mx_row_kernel<O, T, SILU, DEEP>;
   if (int rc = allow_smem<kern>(P::kSmemBytes)) return rc;
   const int64_t wtiles = (args.N + 127) / 128;
   args.ttiles = (args.M + T - 1) / T;
@@ -90,24 +114,12 @@ int launch_row(const Operands& o, MxGemmArgs args, cudaStream_t stream) {
   W8A8_REQUIRE(tiles <= 0x7fff0000LL, W8A8_ERR_UNSUPPORTED, "mxfp4_gemm: too many output tiles");
   args.tiles = static_cast<int>(tiles);
   int split = 1;
-  if (int rc = pick_split<kern>(tiles, args.kblocks, kRowThreads, P::kSmemBytes, &split)) return rc;
-  const int64_t grid = split > 1 ? tiles * split : std::min<int64_t>(tiles, std::max(1, sm_count()));
-  cudaLaunchConfig_t cfg = {};
-  cfg.gridDim = dim3(static_cast<unsigned>(grid));
-  cfg.blockDim = dim3(kRowThreads);
-  cfg.dynamicSmemBytes = P::kSmemBytes;
-  cfg.stream = stream;
-  cudaLaunchAttribute attr[2];
-  attr[0].id = cudaLaunchAttributeProgrammaticStreamSerialization;
-  attr[0].val.programmaticStreamSerializationAllowed = 1;
-  attr[1].id = cudaLaunchAttributeClusterDimension;
-  attr[1].val.clusterDim.x = static_cast<unsigned>(split);
-  attr[1].val.clusterDim.y = 1;
-  attr[1].val.clusterDim.z = 1;
-  cfg.attrs = attr;
-  cfg.numAttrs = 2;
-  W8A8_CUDA_TRY(cudaLaunchKernelEx(&cfg, kern, tw, tws, tx, txs, args));
-  return W8A8_OK;
+  if (DEEP)
+    if (int rc = pick_split<kern>(tiles, args.kblocks, kRowThreads, P::kSmemBytes, 1, 8, SILU ? 6 : 2, &split)) return rc;
+  // (CTAs that have an SM each are persistent)
+  const int64_t grid = split > 1 ? tiles * split : DEEP ? std::min<int64_t>(tiles, std::max(1, sm_count())) : tiles;
+  return launch_cluster(kern, static_cast<unsigned>(grid), kRowThreads, P::kSmemBytes, split, stream, tw, tws, tx, txs,
+                        args);
 }
 
 template <typename O, bool SILU>
@@ -126,20 +138,30 @@ int launch_pair(const Operands& o, const MxGemmArgs& g, cudaStream_t stream) {
   if (int rc = encode_words(&tas, o.as, row_tiles(g.M), k_tiles(g.K) * kTileBytes / 4, 256)) return rc;
   if (int rc = encode_operand(&tb, o.b, o.b_rows, g.K / 2, 128)) return rc;
   if (int rc = encode_words(&tbs, o.bs, row_tiles(o.b_rows), k_tiles(g.K) * kTileBytes / 4, 256)) return rc;
-  const int pairs = static_cast<int>(std::min<int64_t>(blocks, std::max(1, sm_count() / 2)));
-  W8A8_CUDA_TRY(launch_pdl(kern, dim3(2 * pairs), dim3(PairTraits::kThreads), PairTraits::kSmemBytes, stream, ta, tas,
-                           tb, tbs, args));
-  return W8A8_OK;
+  int split = 1;
+  if (int rc = pick_split<kern>(blocks, g.kblocks, PairTraits::kThreads, PairTraits::kSmemBytes, 2, 2, 8, &split)) return rc;
+  const int64_t pairs = split > 1 ? blocks * split : std::min<int64_t>(blocks, std::max(1, sm_count() / 2));
+  return launch_cluster(kern, static_cast<unsigned>(2 * pairs), PairTraits::kThreads, PairTraits::kSmemBytes, 2 * split,
+                        stream, ta, tas, tb, tbs, args);
+}
+
+template <typename O, int T, bool SILU>
+int launch_row_any(const Operands& o, const MxGemmArgs& args, cudaStream_t stream) {
+  if constexpr (!SILU && T < 128) {
+    const int64_t tiles = static_cast<int64_t>((args.N + 127) / 128) * ((args.M + T - 1) / T);
+    if (tiles > sm_count()) return launch_row<O, T, false, false>(o, args, stream);
+  }
+  return launch_row<O, T, SILU, true>(o, args, stream);
 }
 
 template <typename O, bool SILU>
 int dispatch(const Operands& o, const MxGemmArgs& args, cudaStream_t stream) {
-  const int64_t blocks = static_cast<int64_t>((args.M + 255) / 256) * (SILU ? args.N / 128 : (args.N + 255) / 256);
-  if (args.M > 128 && 2 * blocks >= sm_count() / 2) return launch_pair<O, SILU>(o, args, stream);
-  if (args.M <= 16) return launch_row<O, 16, SILU>(o, args, stream);
-  if (args.M <= 32) return launch_row<O, 32, SILU>(o, args, stream);
-  if (args.M <= 64) return launch_row<O, 64, SILU>(o, args, stream);
-  return launch_row<O, 128, SILU>(o, args, stream);
+  if (args.M <= 16) return launch_row_any<O, 16, SILU>(o, args, stream);
+  if (args.M <= 32) return launch_row_any<O, 32, SILU>(o, args, stream);
+  if (args.M <= 64) return launch_row_any<O, 64, SILU>(o, args, stream);
+  if constexpr (!SILU)
+    if (args.M <= 128) return launch_row_any<O, 128, false>(o, args, stream);
+  return launch_pair<O, SILU>(o, args, stream);
 }
 
 int run(const char* what, const Operands& o, const void* bias, void* C, uint8_t* q, uint8_t* qs, int dtype, int64_t M,

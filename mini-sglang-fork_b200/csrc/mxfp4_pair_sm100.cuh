@@ -14,6 +14,9 @@
 // columns from 384 on.  The epilogue reads the 128 shared columns into
 // registers first and releases them; the next block's MMAs wait for those
 // only, while the rest is still being read.
+//
+// With few blocks a cluster of two pairs works on one, each on a half of K; each
+// pair finishes a half of the columns (S = 2 below; 1 otherwise).
 #pragma once
 
 #include "mxfp4_sm100.cuh"
@@ -36,7 +39,8 @@ struct PairTraits {
   static constexpr int kStagingBytes = kEpiWarps * 2048;
   static constexpr int kSmemBytes = 1024 + kStages * kStageBytes + kBarrierBytes + kStagingBytes;
   static_assert(kSmemBytes <= 227 * 1024, "shared memory");
-  static_assert(kSmemBytes > 114 * 1024, "one CTA per SM");  // as for MxRowTraits
+  static_assert(2 * 128 * 128 * 4 <= kStages * kStageBytes, "the shares reuse the ring");
+  static_assert(kSmemBytes >= 170 * 1024, "TMEM share");  // as for MxRowTraits
 };
 
 __device__ __forceinline__ void cp_scales_pair(uint32_t taddr, uint64_t sdesc) {
@@ -82,6 +86,12 @@ __device__ __forceinline__ void pair_block(const PairArgs& a, int p, int& pm, in
   tn = r / rows;
 }
 
+// Word offset of column c (a multiple of 4) of a row in a [128][32] fp32 array
+// whose 16-byte pieces are XORed with the row (part_word).
+__device__ __forceinline__ uint32_t pair_part_word(int r, int c) {
+  return static_cast<uint32_t>(r * 32 + (((c >> 2) ^ (r & 7)) << 2));
+}
+
 // Plain epilogue of 32 columns (from `col0`) of a warp's 32 rows: through the
 // warp's 2 KB of shared memory (16-byte pieces, the piece index XORed with the
 // row pair: no bank conflict either way) to rows of 64 contiguous bytes.
@@ -103,29 +113,22 @@ __device__ __forceinline__ void plain_chunk(const MxGemmArgs& g, uint32_t (&v)[3
     stg[lane * 4 + (e ^ ((lane >> 1) & 3))] = make_uint4(w[0], w[1], w[2], w[3]);
   }
   __syncwarp();
-  O* out = static_cast<O*>(g.out);
+  if ((g.N & 7) == 0) {
 #pragma unroll
-  for (int e = 0; e < 4; ++e) {
-    const int r = e * 8 + (lane >> 2), piece = lane & 3;
-    const uint4 w = stg[r * 4 + (piece ^ ((r >> 1) & 3))];
-    const int64_t row = row0 + r;
-    const int col = col0 + piece * 8;
-    if (row >= g.M || col >= g.N) continue;
-    O* dst = out + row * g.N + col;
-    if ((g.N & 7) == 0) {
-      *reinterpret_cast<uint4*>(dst) = w;
-    } else {  // rows that are not 16-byte aligned
-      const uint32_t x[4] = {w.x, w.y, w.z, w.w};
-#pragma unroll
-      for (int k = 0; k < 8; ++k)
-        if (col + k < g.N) reinterpret_cast<uint16_t*>(dst)[k] = static_cast<uint16_t>(x[k >> 1] >> (16 * (k & 1)));
+    for (int e = 0; e < 4; ++e) {
+      const int r = e * 8 + (lane >> 2), piece = lane & 3;
+      store8_row<O>(g, row0 + r, col0 + piece * 8, stg[r * 4 + (piece ^ ((r >> 1) & 3))]);
     }
+  } else if (col0 + lane < g.N) {  // rows that are not 16-byte aligned: a row at a time, a value per lane
+    O* dst = static_cast<O*>(g.out) + col0 + lane;
+    for (int r = 0; r < 32 && row0 + r < g.M; ++r)
+      dst[(row0 + r) * g.N] = reinterpret_cast<const O*>(stg + r * 4 + ((lane >> 3) ^ ((r >> 1) & 3)))[lane & 7];
   }
   __syncwarp();
 }
 
 template <typename O, bool SILU>
-__global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(PairTraits::kThreads, 1)
+__global__ void __launch_bounds__(PairTraits::kThreads, 1)
     mx_pair_kernel(const __grid_constant__ CUtensorMap tm_a, const __grid_constant__ CUtensorMap tm_as,
                    const __grid_constant__ CUtensorMap tm_b, const __grid_constant__ CUtensorMap tm_bs,
                    const PairArgs args) {
@@ -142,17 +145,24 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(PairTraits::kThreads
   uint64_t* acc_full = bars + 2 * P::kStages;  // [2]
   uint64_t* acc_free = acc_full + 2;           // the overlap of a block's accumulator has been read
   uint64_t* drain = acc_free + 1;
-  uint32_t* tmem_slot = reinterpret_cast<uint32_t*>(drain + 1);
+  uint64_t* arrived = drain + 1;  // S > 1: the other share's sums
+  uint32_t* tmem_slot = reinterpret_cast<uint32_t*>(drain + 2);
   volatile int* abort_flag = reinterpret_cast<volatile int*>(tmem_slot + 1);
   uint8_t* staging = reinterpret_cast<uint8_t*>(bars) + P::kBarrierBytes;
 
   const int warp = threadIdx.x >> 5;
   const int lane = threadIdx.x & 31;
-  const uint32_t half = dev::cluster_rank();  // 0 = leader
-  const int first = blockIdx.x >> 1;
-  const int step = gridDim.x >> 1;
+  const uint32_t rank = dev::cluster_rank();
+  const uint32_t half = rank & 1u;  // 0 = leader of its pair
+  const uint32_t leader = rank & ~1u;
+  const int S = static_cast<int>(cluster_size() >> 1);  // shares of K
+  const int share = static_cast<int>(rank >> 1);
+  const int first = blockIdx.x / (2 * S);
+  const int step = gridDim.x / (2 * S);  // (S > 1: one block per cluster)
   const int blocks = args.pairs_m * args.tiles_n;
   const MxGemmArgs& g = args.g;
+  const int kb0 = static_cast<int>(static_cast<int64_t>(share) * g.kblocks / S);
+  const int kb1 = static_cast<int>(static_cast<int64_t>(share + 1) * g.kblocks / S);
   const long long tmo = g.timeout_ns;
 
   if (threadIdx.x == 0) {
@@ -164,6 +174,7 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(PairTraits::kThreads
     dev::mbar_init(dev::smem_u32(acc_full + 1), 1);
     dev::mbar_init(dev::smem_u32(acc_free), 2 * P::kEpiWarps);  // the epilogue warps of both CTAs
     dev::mbar_init(dev::smem_u32(drain), 1);
+    dev::mbar_init(dev::smem_u32(arrived), 1);
     *abort_flag = 0;
     dev::fence_mbar_init();
     dev::prefetch_tmap(&tm_a);
@@ -195,11 +206,11 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(PairTraits::kThreads
       const int tb0 = SILU ? tn : 2 * tn;
       const int tb1 = SILU ? tn + (g.N >> 7) : 2 * tn + 1;
       const int b_row = (half ? tb1 : tb0) * 128;
-      for (int kb = 0; kb < g.kblocks; ++kb) {
+      for (int kb = kb0; kb < kb1; ++kb) {
         ok = warp_wait(dev::smem_u32(empty + stage), phase ^ 1u, abort_flag, g.err, tmo);
         if (!ok) break;
         if (elect_one()) {
-          const uint32_t bar = dev::mapa(dev::smem_u32(full + stage), 0);
+          const uint32_t bar = dev::mapa(dev::smem_u32(full + stage), leader);
           if (half == 0) dev::mbar_expect_tx(dev::smem_u32(full + stage), 2 * P::kStageBytes);
           dev::tma_load_2d_pair(dev::smem_u32(s_a + stage * P::kTile), &tm_a, bar, kb * 128, ta * 128);
           dev::tma_load_2d_pair(dev::smem_u32(s_b + stage * P::kTile), &tm_b, bar, kb * 128, b_row);
@@ -236,7 +247,7 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(PairTraits::kThreads
           break;
         dev::tc_fence_after();
         const uint32_t d = tmem + (blk & 1u) * P::kAccStep;
-        for (int kb = 0; kb < g.kblocks; ++kb) {
+        for (int kb = kb0; kb < kb1; ++kb) {
           if (!ready) {
             ok = warp_wait(dev::smem_u32(full + stage), phase, abort_flag, g.err, tmo);
             if (!ok) break;
@@ -265,10 +276,10 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(PairTraits::kThreads
               if (k >= steps) break;
               constexpr uint32_t ids[2] = {idesc_mxf4(256, 256, 0), idesc_mxf4(256, 256, 2)};
               mma_mxf4_pair(d, da + 2 * k, db + 2 * k, ids[k & 1], sfa + 4 * (k >> 1), sfb + 8 * (k >> 1),
-                            (kb > 0 || k > 0) ? 1u : 0u);
+                            (kb > kb0 || k > 0) ? 1u : 0u);
             }
-            dev::tc_commit_pair(dev::smem_u32(empty + stage));
-            dev::tc_commit_pair(dev::mapa(dev::smem_u32(empty + stage), 1));
+            dev::tc_commit_pair(dev::mapa(dev::smem_u32(empty + stage), leader));
+            dev::tc_commit_pair(dev::mapa(dev::smem_u32(empty + stage), leader + 1));
           }
           __syncwarp();
           stage = next;
@@ -276,12 +287,12 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(PairTraits::kThreads
         }
         if (!ok) break;
         if (elect_one()) {
-          dev::tc_commit_pair(dev::smem_u32(acc_full + (blk & 1u)));
-          dev::tc_commit_pair(dev::mapa(dev::smem_u32(acc_full + (blk & 1u)), 1));
+          dev::tc_commit_pair(dev::mapa(dev::smem_u32(acc_full + (blk & 1u)), leader));
+          dev::tc_commit_pair(dev::mapa(dev::smem_u32(acc_full + (blk & 1u)), leader + 1));
         }
         __syncwarp();
       }
-      if (elect_one()) dev::tc_commit_pair(dev::smem_u32(drain));
+      if (elect_one()) dev::tc_commit_pair(dev::mapa(dev::smem_u32(drain), leader));
       if (lane == 0 && !dev::mbar_wait_drain(dev::smem_u32(drain), 0, tmo))
         if (g.err) atomicOr(g.err, kErrGemmDrain);
     }
@@ -291,7 +302,7 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(PairTraits::kThreads
     const int hh = (warp - 2) >> 2;    // which of the two warps of that quarter
     const uint32_t lanes = static_cast<uint32_t>(quarter * 32) << 16;
     uint4* stg = reinterpret_cast<uint4*>(staging + (warp - 2) * 2048);
-    const uint32_t free_bar = dev::mapa(dev::smem_u32(acc_free), 0);
+    const uint32_t free_bar = dev::mapa(dev::smem_u32(acc_free), leader);
     uint32_t blk = 0;
     for (int p = first; p < blocks; p += step, ++blk) {
       int pm, tn;
@@ -303,6 +314,7 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(PairTraits::kThreads
       if (!__all_sync(0xffffffffu, ok)) break;
       dev::tc_fence_after();
       const uint32_t t = tmem + lanes + acc * P::kAccStep;
+      if (S > 1) break;  // one block, finished below
       // the shared columns: chunks of 32, 4.. 7 of accumulator 0, 0..3 of
       // accumulator 1; this warp's are hh and hh + 2 of the four
       const uint32_t shared_t = t + (acc ? 0 : 128), own_t = t + (acc ? 128 : 0);
@@ -346,8 +358,87 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(PairTraits::kThreads
     dev::tc_fence_before();
   }
 
+  if (S > 1) {
+    // Two pairs, each with a half of K.  CTA (share s, half) writes the s-th
+    // half of its rows' columns (SiLU: of the features): chunks of 32 columns,
+    // [4 chunks][128 rows][32] words.  The other share's four go to its CTA of
+    // the same rows, and that CTA's come here.
+    constexpr int kChunkWords = 128 * 32;
+    constexpr uint32_t kBytes = 4 * kChunkWords * 4;
+    float* out = reinterpret_cast<float*>(smem);
+    float* in = out + 4 * kChunkWords;
+    if (threadIdx.x == 64) dev::mbar_expect_tx(dev::smem_u32(arrived), kBytes);
+    dev::cluster_sync();  // every pair's MMAs are done: the rings may be written
+    if (warp >= 2) {
+      const int quarter = warp & 3, hh = (warp - 2) >> 2;
+      const int row = quarter * 32 + lane;
+      const uint32_t t = tmem + (static_cast<uint32_t>(quarter * 32) << 16);
+      // chunk i (0..3) of share s: columns, or features i & 1 of gate (i < 2) and up
+      const auto column = [&](int s, int i) { return SILU ? 128 * (i >> 1) + 64 * s + 32 * (i & 1) : 128 * s + 32 * i; };
+      dev::tc_fence_after();
+#pragma unroll 1
+      for (int i = hh; i < 4; i += 2) {
+        uint32_t v[32];
+        dev::tmem_ld32(t + column(share ^ 1, i), v);
+        dev::tmem_wait_ld(v);
+#pragma unroll
+        for (int e = 0; e < 8; ++e)
+          *reinterpret_cast<uint4*>(out + i * kChunkWords + pair_part_word(row, 4 * e)) =
+              make_uint4(v[4 * e], v[4 * e + 1], v[4 * e + 2], v[4 * e + 3]);
+      }
+      fence_async_smem();
+      dev::named_bar_sync(1, 32 * P::kEpiWarps);
+      if (threadIdx.x == 64) {
+        const uint32_t peer = rank ^ 2u;
+        dsmem_copy(dev::mapa(dev::smem_u32(in), peer), dev::smem_u32(out), kBytes, dev::mapa(dev::smem_u32(arrived), peer));
+      }
+      __syncwarp();
+      // this CTA's own chunk i plus the other share's (share 0's first)
+      const auto sum = [&](int i, uint32_t (&v)[32]) {
+#pragma unroll
+        for (int e = 0; e < 8; ++e) {
+          const float4 x = *reinterpret_cast<const float4*>(in + i * kChunkWords + pair_part_word(row, 4 * e));
+          const float p[4] = {x.x, x.y, x.z, x.w};
+#pragma unroll
+          for (int k = 0; k < 4; ++k) v[4 * e + k] = __float_as_uint(__uint_as_float(v[4 * e + k]) + p[k]);
+        }
+      };
+      int pm, tn;
+      pair_block(args, first, pm, tn);
+      const int row0 = (2 * pm + static_cast<int>(half)) * 128 + quarter * 32;
+      uint32_t v[32], w[32];
+      if (warp_wait(dev::smem_u32(arrived), 0, abort_flag, g.err, tmo)) {
+        if constexpr (SILU) {  // this warp: feature block hh of the share's two
+          dev::tmem_ld32(t + column(share, hh), v);
+          dev::tmem_ld32(t + column(share, 2 + hh), w);
+          dev::tmem_wait_ld(v);
+          dev::tmem_wait_ld(w);
+          sum(hh, v);
+          sum(2 + hh, w);
+          float gate[32], up[32];
+#pragma unroll
+          for (int e = 0; e < 32; ++e) {
+            gate[e] = __uint_as_float(v[e]);
+            up[e] = __uint_as_float(w[e]);
+          }
+          silu_block<O>(g, gate, up, row0 + lane, tn, 2 * share + hh);
+        } else {
+#pragma unroll 1
+          for (int i = hh; i < 4; i += 2) {
+            dev::tmem_ld32(t + column(share, i), v);
+            dev::tmem_wait_ld(v);
+            sum(i, v);
+            plain_chunk<O>(g, v, reinterpret_cast<uint4*>(staging + (warp - 2) * 2048), lane, row0,
+                           tn * 256 + column(share, i));
+          }
+        }
+      }
+      dev::tc_fence_before();
+    }
+  }
+
   __syncthreads();
-  dev::cluster_sync();  // the pair is done with both CTAs' TMEM and shared memory
+  dev::cluster_sync();  // the cluster is done with every CTA's TMEM and shared memory
   if (warp == 1) {
     dev::tc_fence_after();
     dev::tmem_dealloc2(tmem, 512);

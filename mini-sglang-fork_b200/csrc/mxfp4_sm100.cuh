@@ -89,12 +89,19 @@ struct MxGemmArgs {
   int ttiles, tiles;  // weight-stationary kernel: token tiles, output tiles
 };
 
-__device__ __forceinline__ float4 ld_dsmem4(uint32_t cluster_addr) {
-  float4 v;
-  asm volatile("ld.shared::cluster.v4.f32 {%0, %1, %2, %3}, [%4];"
-               : "=f"(v.x), "=f"(v.y), "=f"(v.z), "=f"(v.w)
-               : "r"(cluster_addr));
-  return v;
+// Copies `bytes` (a multiple of 16) of this CTA's shared memory into another
+// CTA's, counted on that CTA's mbarrier (`dst` and `bar` are cluster addresses
+// of the same CTA).
+__device__ __forceinline__ void dsmem_copy(uint32_t dst, uint32_t src, uint32_t bytes, uint32_t bar) {
+  asm volatile(
+      "cp.async.bulk.shared::cluster.shared::cta.mbarrier::complete_tx::bytes [%0], [%1], %2, [%3];" ::"r"(dst),
+      "r"(src), "r"(bytes), "r"(bar)
+      : "memory");
+}
+
+// Makes this thread's writes to its shared memory visible to bulk copies.
+__device__ __forceinline__ void fence_async_smem() {
+  asm volatile("fence.proxy.async.shared::cta;" ::: "memory");
 }
 
 __device__ __forceinline__ uint32_t cluster_size() {
@@ -111,6 +118,21 @@ __device__ __forceinline__ void tma_prefetch_2d(const void* tmap, int32_t x, int
                    reinterpret_cast<uint64_t>(tmap)),
                "r"(x), "r"(y)
                : "memory");
+}
+
+// Eight output values from column `col` (a multiple of 8) of a row.
+template <typename O>
+__device__ __forceinline__ void store8_row(const MxGemmArgs& g, int64_t row, int col, const uint4& w) {
+  if (row >= g.M || col >= g.N) return;
+  O* dst = static_cast<O*>(g.out) + row * g.N + col;
+  if ((g.N & 7) == 0) {
+    *reinterpret_cast<uint4*>(dst) = w;
+  } else {  // rows that are not 16-byte aligned
+    const uint32_t x[4] = {w.x, w.y, w.z, w.w};
+#pragma unroll
+    for (int k = 0; k < 8; ++k)
+      if (col + k < g.N) reinterpret_cast<uint16_t*>(dst)[k] = static_cast<uint16_t>(x[k >> 1] >> (16 * (k & 1)));
+  }
 }
 
 // silu(gate) * up of 32 features (block `j` of 128-feature tile `ft`) of one
@@ -152,16 +174,20 @@ __device__ __forceinline__ void silu_block(const MxGemmArgs& g, const float (&ga
 // rows, on the MMA's 128-row side) for T tokens; with the SiLU epilogue 128
 // gate rows and the 128 up rows that belong to them, in two accumulators.
 // The weights are read once, at the rate of HBM, which is what bounds it; the
-// ring (about 200 KB, the SM's whole shared memory) is there to keep enough of
-// them in flight.
+// ring (about 200 KB of an SM's shared memory, in one CTA or in two) is there
+// to keep enough of them in flight.
 //
-// With enough tiles the CTAs are persistent and the accumulators doubled, so
-// that a tile's epilogue overlaps the next one's loads and MMAs.  With few, a
-// cluster of S CTAs splits K: each leaves its fp32 sums in its own shared
-// memory and, after a cluster barrier, CTA r adds the S shares of tokens r,
-// r + S, ... in rank order through distributed shared memory and writes them.
-// The order of the sum is fixed, and nothing is left in memory between calls.
-template <int T, bool SILU>
+// With more tiles than SMs, CTAs are small enough for two or three on an SM and
+// one computes while others start or end (51200 x 5120, one token: 22.9 us; one
+// persistent CTA per SM with the same ring: 24.5).  With fewer tiles a CTA
+// takes the SM for itself, and with at most half as many, a
+// cluster of S CTAs splits K: CTA r writes an S-th of the tokens, and every CTA
+// sends it its fp32 sums of those by a bulk copy between shared memories, the
+// fast way there (gate_up 1536 x 4096, 64 tokens, eight shares: 11.5 us; 22.5
+// with loads from the peers' memory, 32.8 with stores to it).  r adds them up
+// in the order of the shares, so the result does not depend on timing, and
+// nothing is left in memory between calls.
+template <int T, bool SILU, bool DEEP>
 struct MxRowTraits {
   static constexpr int kTiles = SILU ? 2 : 1;  // weight tiles (gate, up)
   static constexpr int kW = 128 * 128;         // bytes of a weight tile's k block
@@ -169,32 +195,29 @@ struct MxRowTraits {
   static constexpr int kSf = 1024;             // scale bytes of 128 rows per k block
   static constexpr int kStageBytes = kTiles * (kW + kSf) + kX + kSf;
   static constexpr int kSfCols = 8 * (kTiles + 1);  // TMEM columns of a stage's scales
-  static constexpr int kStages = SILU ? (T == 16 ? 5 : T == 128 ? 3 : 4) : (T <= 32 ? 10 : T == 64 ? 8 : 6);
+  static constexpr int kStages = SILU   ? (T == 16 ? 5 : 4)
+                                 : DEEP ? (T <= 32 ? 10 : T == 64 ? 8 : 6)
+                                        : (T <= 32 ? 3 : 4);
   static constexpr int kChunk = T < 32 ? T : 32;  // columns that the epilogue takes at a time
   static constexpr int kAccCols = kTiles * T;
-  static constexpr int kAccs = 2 * kAccCols + kStages * kSfCols <= 512 ? 2 : 1;
+  static constexpr int kAccs = (SILU || DEEP) && 2 * kAccCols + kStages * kSfCols <= 512 ? 2 : 1;
   static constexpr int kColsNeeded = kAccs * kAccCols + kStages * kSfCols;
-  static constexpr int kTmemCols = kColsNeeded <= 128 ? 128 : kColsNeeded <= 256 ? 256 : 512;
+  static constexpr int kTmemCols = kColsNeeded <= 64 ? 64 : kColsNeeded <= 128 ? 128 : kColsNeeded <= 256 ? 256 : 512;
   static constexpr int kBarrierBytes = 256;
   static constexpr int kStagingBytes = SILU ? 4 * 2 * kChunk * 128 : 0;  // per epilogue warp: gate, up
   static constexpr int kSmemBytes = 1024 + kStages * kStageBytes + kBarrierBytes + kStagingBytes;
   static_assert(kColsNeeded <= 512, "TMEM");
   static_assert(kSmemBytes <= 227 * 1024, "shared memory");
-  // More than half of the SM's shared memory: no second CTA of this library
-  // that holds TMEM fits beside it, so no CTA of a cluster waits for TMEM that
-  // a CTA waiting for it holds.
-  static_assert(kSmemBytes > 114 * 1024, "one CTA per SM");
-  static_assert(kTiles * T * 128 * 4 <= kStages * kStageBytes, "the partial sums reuse the ring");
+  // At most three CTAs with at most 128 TMEM columns each share an SM, and one
+  // with more leaves no room for another.  So every allocation succeeds at
+  // once, and no CTA of a cluster waits for TMEM that a CTA waiting for it
+  // holds.
+  static_assert(kTmemCols <= 128 ? kSmemBytes >= 60 * 1024 : kSmemBytes >= 170 * 1024, "TMEM share");
+  // The ring holds a CTA's own shares for its peers and theirs for it.
+  static_assert(!DEEP || 2 * kTiles * (T + 8) * 512 <= kStages * kStageBytes, "the shares reuse the ring");
 };
 
 constexpr int kRowThreads = 192;  // producer, MMA, four epilogue warps
-
-// Word offset of column n of token t in a [token][128] fp32 array whose 16-byte
-// pieces are XORed with the token: a warp writes 32 columns of one token, or
-// reads the same piece of 8 tokens, without bank conflicts.
-__device__ __forceinline__ uint32_t part_word(int t, int n) {
-  return static_cast<uint32_t>(t * 128 + ((((n >> 2) ^ (t & 7)) << 2) | (n & 3)));
-}
 
 template <int CH>
 __device__ __forceinline__ void tmem_ld_chunk(uint32_t taddr, float (&v)[32]) {
@@ -205,13 +228,13 @@ __device__ __forceinline__ void tmem_ld_chunk(uint32_t taddr, float (&v)[32]) {
   for (int j = 0; j < CH; ++j) v[j] = __uint_as_float(r[j]);
 }
 
-template <typename O, int T, bool SILU>
+template <typename O, int T, bool SILU, bool DEEP>
 __global__ void __launch_bounds__(kRowThreads, 1) mx_row_kernel(const __grid_constant__ CUtensorMap tm_w,
                                                                 const __grid_constant__ CUtensorMap tm_ws,
                                                                 const __grid_constant__ CUtensorMap tm_x,
                                                                 const __grid_constant__ CUtensorMap tm_xs,
                                                                 const MxGemmArgs args) {
-  using P = MxRowTraits<T, SILU>;
+  using P = MxRowTraits<T, SILU, DEEP>;
   extern __shared__ __align__(1024) uint8_t smem_raw[];
   uint8_t* smem = reinterpret_cast<uint8_t*>((reinterpret_cast<uintptr_t>(smem_raw) + 1023) & ~uintptr_t(1023));
   // [stage] weight tiles, [stage] tokens, then the scales
@@ -225,9 +248,9 @@ __global__ void __launch_bounds__(kRowThreads, 1) mx_row_kernel(const __grid_con
   uint64_t* acc_full = bars + 2 * P::kStages;  // [2]
   uint64_t* acc_empty = acc_full + 2;          // [2]
   uint64_t* drain = acc_empty + 2;
-  uint32_t* tmem_slot = reinterpret_cast<uint32_t*>(drain + 1);
+  uint32_t* tmem_slot = reinterpret_cast<uint32_t*>(drain + 2);
   volatile int* abort_flag = reinterpret_cast<volatile int*>(tmem_slot + 1);
-  float* part = reinterpret_cast<float*>(smem);  // [gate / up][token][128], after the ring is done (S > 1)
+  uint64_t* arrived = drain + 1;  // S > 1: the peers' shares
 
   const int warp = threadIdx.x >> 5;
   const int lane = threadIdx.x & 31;
@@ -249,6 +272,7 @@ __global__ void __launch_bounds__(kRowThreads, 1) mx_row_kernel(const __grid_con
       dev::mbar_init(dev::smem_u32(acc_empty + s), 4);  // the epilogue warps
     }
     dev::mbar_init(dev::smem_u32(drain), 1);
+    dev::mbar_init(dev::smem_u32(arrived), 1);
     *abort_flag = 0;
     dev::fence_mbar_init();
     dev::prefetch_tmap(&tm_w);
@@ -261,7 +285,7 @@ __global__ void __launch_bounds__(kRowThreads, 1) mx_row_kernel(const __grid_con
     dev::tmem_relinquish();
   }
   dev::griddep_launch();
-  if (warp == 0 && first < args.tiles) {
+  if (DEEP && warp == 0) {
     // the first stages' weights into L2 while the previous kernel ends
     if (elect_one()) {
       for (int kb = kb0; kb < min(kb1, kb0 + P::kStages); ++kb)
@@ -386,18 +410,7 @@ __global__ void __launch_bounds__(kRowThreads, 1) mx_row_kernel(const __grid_con
       if (!warp_wait(dev::smem_u32(acc_full + acc), use & 1u, abort_flag, args.err, tmo)) break;
       dev::tc_fence_after();
       const uint32_t t_acc = tmem + lanes + acc * P::kAccCols;
-      if (S > 1) {
-        for (int c = 0; c < tokens; c += P::kChunk) {
-#pragma unroll
-          for (int h = 0; h < P::kTiles; ++h) {
-            float v[32];
-            tmem_ld_chunk<P::kChunk>(t_acc + h * T + c, v);
-#pragma unroll
-            for (int j = 0; j < P::kChunk; ++j) part[h * T * 128 + part_word(c + j, n)] = v[j];
-          }
-        }
-        break;
-      }
+      if (S > 1) break;  // one tile, finished below
       if constexpr (!SILU) {
         const int col = wt * 128 + n;
         const bool in = col < args.N;
@@ -445,69 +458,92 @@ __global__ void __launch_bounds__(kRowThreads, 1) mx_row_kernel(const __grid_con
     }
     dev::tc_fence_before();
   }
-  if (S > 1) {
-    dev::cluster_sync();  // every share is in its CTA's shared memory
+  if (DEEP && S > 1) {
+    const int tt = first % args.ttiles, wt = first / args.ttiles;
+    const int tokens = min(T, args.M - tt * T);
+    const auto begin = [&](int s) { return tokens * s / S; };  // tokens [begin(s), begin(s + 1)) are s's
+    const int t0 = begin(rank), count = begin(rank + 1) - t0;
+    // in the ring: [token][gate / up][128] sums of this CTA, then from each
+    // share (in rank order, its own place left empty) the same of its tokens
+    constexpr int kTokenWords = P::kTiles * 128;
+    float* own = reinterpret_cast<float*>(smem);
+    float* in = own + T * kTokenWords;
+    if (threadIdx.x == 64 && count > 0) dev::mbar_expect_tx(dev::smem_u32(arrived), (S - 1) * count * kTokenWords * 4);
+    dev::cluster_sync();  // every CTA's MMAs are done: its ring may be written
     if (warp >= 2) {
-      const int tt = first % args.ttiles, wt = first / args.ttiles;
-      const int tokens = min(T, args.M - tt * T);
-      const int mine = (tokens - rank + S - 1) / S;  // tokens rank, rank + S, ...
+      const int q = warp & 3, n = q * 32 + lane;
+      const uint32_t t_acc = tmem + (static_cast<uint32_t>(q * 32) << 16);
       const int et = threadIdx.x - 64;
-      const uint32_t local = dev::smem_u32(part);
+      dev::tc_fence_after();
+      for (int c = 0; c < tokens; c += P::kChunk)
+#pragma unroll
+        for (int h = 0; h < P::kTiles; ++h) {
+          float v[32];
+          tmem_ld_chunk<P::kChunk>(t_acc + h * T + c, v);
+#pragma unroll
+          for (int j = 0; j < P::kChunk; ++j)
+            own[(c + j) * kTokenWords + h * 128 + ((((n >> 2) ^ ((c + j) & 7)) << 2) | (n & 3))] = v[j];
+        }
+      dev::tc_fence_before();
+      fence_async_smem();
+      dev::named_bar_sync(1, 128);
+      if (et < S && et != rank) {
+        const int to = begin(et), many = begin(et + 1) - to;
+        if (many > 0)
+          dsmem_copy(dev::mapa(dev::smem_u32(in) + static_cast<uint32_t>(rank * many * kTokenWords) * 4, et),
+                     dev::smem_u32(own + to * kTokenWords), static_cast<uint32_t>(many * kTokenWords) * 4,
+                     dev::mapa(dev::smem_u32(arrived), et));
+      }
+      __syncwarp();
+      if (count > 0) warp_wait(dev::smem_u32(arrived), 0, abort_flag, args.err, tmo);
+      const int64_t row0 = static_cast<int64_t>(tt) * T;
+      // 16 bytes of the s-th share of token t (of this CTA's), word w
+      const auto piece = [&](int s, int t, int w) {
+        const float* p = s == rank ? own + t * kTokenWords : in + (s * count + t - t0) * kTokenWords;
+        return *reinterpret_cast<const float4*>(p + (w & ~127) + ((((w & 127) >> 2) ^ (t & 7)) << 2));
+      };
       if constexpr (!SILU) {
         // an item: 8 columns of a token
-        for (int it = et; it < mine * 16; it += 128) {
-          const int t = rank + S * (it >> 4), n0 = (it & 15) * 8;
-          const uint32_t a0 = local + 4 * part_word(t, n0), a1 = local + 4 * part_word(t, n0 + 4);
+        for (int it = et; it < count * 16; it += 128) {
+          const int t = t0 + (it >> 4), n0 = (it & 15) * 8;
           float v[8] = {0, 0, 0, 0, 0, 0, 0, 0};
-#pragma unroll 4
           for (int s = 0; s < S; ++s) {
-            const float4 x = ld_dsmem4(dev::mapa(a0, s)), y = ld_dsmem4(dev::mapa(a1, s));
+            const float4 x = piece(s, t, n0), y = piece(s, t, n0 + 4);
             v[0] += x.x, v[1] += x.y, v[2] += x.z, v[3] += x.w;
             v[4] += y.x, v[5] += y.y, v[6] += y.z, v[7] += y.w;
           }
           const int col = wt * 128 + n0;
-          O* dst = static_cast<O*>(args.out) + (static_cast<int64_t>(tt) * T + t) * args.N + col;
           if (args.bias) {
             const O* b = static_cast<const O*>(args.bias) + col;
 #pragma unroll
             for (int j = 0; j < 8; ++j)
               if (col + j < args.N) v[j] += to_float(b[j]);
           }
-          const uint32_t w[4] = {pack2<O>(v[0], v[1]), pack2<O>(v[2], v[3]), pack2<O>(v[4], v[5]),
-                                 pack2<O>(v[6], v[7])};
-          if ((args.N & 7) == 0) {
-            if (col < args.N) *reinterpret_cast<uint4*>(dst) = make_uint4(w[0], w[1], w[2], w[3]);
-          } else {
-#pragma unroll
-            for (int j = 0; j < 8; ++j)
-              if (col + j < args.N)
-                reinterpret_cast<uint16_t*>(dst)[j] = static_cast<uint16_t>(w[j >> 1] >> (16 * (j & 1)));
-          }
+          store8_row<O>(args, row0 + t, col,
+                        make_uint4(pack2<O>(v[0], v[1]), pack2<O>(v[2], v[3]), pack2<O>(v[4], v[5]), pack2<O>(v[6], v[7])));
         }
       } else {
         // an item: one 32-feature block of a token
-        for (int it = et; it < mine * 4; it += 128) {
-          const int t = rank + S * (it >> 2), j = it & 3;
+        for (int it = et; it < count * 4; it += 128) {
+          const int t = t0 + (it >> 2), j = it & 3;
           float g[32], u[32];
 #pragma unroll
           for (int e = 0; e < 32; ++e) g[e] = u[e] = 0.0f;
           for (int s = 0; s < S; ++s) {
 #pragma unroll
             for (int e = 0; e < 8; ++e) {
-              const uint32_t w = local + 4 * part_word(t, 32 * j + 4 * e);
-              const float4 x = ld_dsmem4(dev::mapa(w, s)), y = ld_dsmem4(dev::mapa(w + 4 * T * 128, s));
+              const float4 x = piece(s, t, 32 * j + 4 * e), y = piece(s, t, 128 + 32 * j + 4 * e);
               g[4 * e] += x.x, g[4 * e + 1] += x.y, g[4 * e + 2] += x.z, g[4 * e + 3] += x.w;
               u[4 * e] += y.x, u[4 * e + 1] += y.y, u[4 * e + 2] += y.z, u[4 * e + 3] += y.w;
             }
           }
-          silu_block<O>(args, g, u, static_cast<int64_t>(tt) * T + t, wt, j);
+          silu_block<O>(args, g, u, row0 + t, wt, j);
         }
       }
     }
-    dev::cluster_sync();  // no CTA leaves while a peer still reads its share
-  } else {
-    __syncthreads();
+    dev::cluster_sync();  // the copies out of this CTA have been taken
   }
+  __syncthreads();
   if (warp == 1) {
     dev::tc_fence_after();
     dev::tmem_dealloc(tmem, P::kTmemCols);
