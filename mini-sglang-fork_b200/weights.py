@@ -21,6 +21,11 @@ and yields this rank's (name, tensor) pairs, sharded and merged:
   then sharded -- so every rank's shard carries the same scales the unsharded
   weight had.
 
+MXFP4 (``mxfp4_weight_stream``): the same sharding and merging of packed 4-bit
+weights ``[N, K/2]`` and their E8M0 scales ``[N, K/32]`` (split on dim 1 with
+the weight: K/32 must divide by the ranks), the merged scales laid out at the
+end in the tiles of ``ops.mxfp4_scale_shape``.
+
 Quantisation at load runs the library's CUDA quantiser on the weight rows
 (``ops.quant_per_token``: per-row absmax == per-output-channel for a
 [N, K] weight) on ``device``; there is no CPU quantiser in the product.
@@ -116,6 +121,22 @@ def _merge_info(key: str):
     return None
 
 
+def _merged(buf: Dict[str, Dict[str, torch.Tensor]], key: str,
+            value: torch.Tensor) -> Optional[Tuple[str, torch.Tensor]]:
+    """``(key, value)`` when it belongs to no merge group; the merged tensor
+    when it completes one; None while one waits in ``buf``."""
+    info = _merge_info(key)
+    if info is None:
+        return key, value
+    merged_key, slot, slots = info
+    group = buf.setdefault(merged_key, {})
+    group[slot] = value
+    if not all(s in group for s in slots):
+        return None
+    del buf[merged_key]
+    return merged_key, torch.cat([group[s] for s in slots], dim=0)
+
+
 def expert_stack_info(key: str) -> Optional[Tuple[str, int]]:
     """``(packed key, expert index)`` of an expert-scoped key, else None."""
     m = _EXPERT.match(key)
@@ -185,17 +206,9 @@ def w8a8_weight_stream(items: Iterable[Tuple[str, torch.Tensor]], rank: int, wor
         else:
             produced = [(name, shard_tensor(name, tensor, rank, world, num_kv_heads))]
         for key, value in produced:
-            value = _cast(key, value, dtype)
-            info = _merge_info(key)
-            if info is None:
-                yield from out(key, value)
-                continue
-            merged_key, slot, slots = info
-            group = merge_buf.setdefault(merged_key, {})
-            group[slot] = value
-            if all(s in group for s in slots):
-                del merge_buf[merged_key]
-                yield from out(merged_key, torch.cat([group[s] for s in slots], dim=0))
+            done = _merged(merge_buf, key, _cast(key, value, dtype))
+            if done is not None:
+                yield from out(*done)
     if merge_buf:
         raise _lib.W8A8Error(_lib.ERR_INVALID_ARG, f"incomplete merge groups in checkpoint: {sorted(merge_buf)}")
     if expert_buf:
@@ -211,3 +224,67 @@ def load_w8a8_state_dict(items: Iterable[Tuple[str, torch.Tensor]], rank: int, w
     model's ``load_state_dict`` in place of the engine's
     ``{k: v.to(dtype) for k, v in load_weight(...)}`` (M/engine/engine.py:139-146)."""
     return dict(w8a8_weight_stream(items, rank, world, num_kv_heads, quantise, device, dtype, num_experts))
+
+
+def mxfp4_quantiser(device: torch.device) -> Quantiser:
+    """MXFP4 quantisation of a [N, K] weight on ``device``: (packed codes
+    [N, K/2], E8M0 bytes [N, K/32]), both uint8."""
+    def quantise(w: torch.Tensor) -> Tuple[torch.Tensor, torch.Tensor]:
+        if w.dim() != 2:
+            raise _lib.W8A8Error(_lib.ERR_INVALID_ARG, f"weight must be 2-D, got {tuple(w.shape)}")
+        t = w.dtype if w.dtype in (torch.bfloat16, torch.float16) else torch.bfloat16
+        q = ops.mxfp4_quant(w.to(device=device, dtype=t).contiguous())
+        return q.data, ops.mxfp4_plain_scales(q)
+    return quantise
+
+
+def mxfp4_weight_stream(items: Iterable[Tuple[str, torch.Tensor]], rank: int, world: int,
+                        num_kv_heads: Optional[int], quantise: Optional[Quantiser] = None,
+                        device: Optional[torch.device] = None,
+                        dtype: torch.dtype = torch.bfloat16) -> Iterator[Tuple[str, torch.Tensor]]:
+    """Shard and merge a checkpoint stream for ``rank`` of ``world`` into the
+    state dict of the MXFP4 layers (module docstring).  A floating projection
+    weight is quantised unsharded (``quantise``: the CUDA quantiser on
+    ``device`` by default); a packed one (``.weight`` uint8 [N, K/2] with
+    ``.weight_scale`` uint8 [N, K/32]) passes through.  Other floating tensors
+    are cast to ``dtype``.  Experts have no MXFP4 layer and are refused."""
+    if not (0 <= rank < world):
+        raise _lib.W8A8Error(_lib.ERR_INVALID_ARG, f"rank {rank} not in [0, {world})")
+    merge_buf: Dict[str, Dict[str, torch.Tensor]] = {}
+    for name, tensor in items:
+        if name.startswith(_SKIP_PREFIXES):
+            continue
+        name = name.removeprefix("language_model.")
+        if _EXPERT.match(name):
+            raise _lib.W8A8Error(_lib.ERR_UNSUPPORTED, f"{name}: mixture-of-experts weights have no MXFP4 layer")
+        if is_linear_weight(name) and tensor.is_floating_point():
+            if quantise is None:  # created on first use: packed checkpoints need no CUDA here
+                quantise = mxfp4_quantiser(device if device is not None
+                                           else torch.device("cuda", torch.cuda.current_device()))
+            produced = list(zip((name, name + "_scale"), quantise(tensor)))
+        else:
+            produced = [(name, tensor)]
+        for key, value in produced:
+            scale = key.endswith(".weight_scale")
+            if scale and (value.dtype != torch.uint8 or value.dim() != 2):
+                raise _lib.W8A8Error(_lib.ERR_INVALID_ARG,
+                                     f"{key}: MXFP4 scales must be uint8 [N, K/32], got {value.dtype} {tuple(value.shape)}")
+            if scale and any(s in key for s in _SPLIT_DIM_1) and value.shape[1] % world:
+                raise _lib.W8A8Error(_lib.ERR_INVALID_ARG,
+                                     f"{key}: {value.shape[1]} blocks of 32 do not divide by {world} ranks")
+            value = shard_tensor(key, value, rank, world, num_kv_heads)
+            done = _merged(merge_buf, key, value.to(dtype) if value.is_floating_point() else value)
+            if done is not None:
+                key, value = done
+                yield key, ops.mxfp4_tile_scales(value) if scale else value.contiguous()
+    if merge_buf:
+        raise _lib.W8A8Error(_lib.ERR_INVALID_ARG, f"incomplete merge groups in checkpoint: {sorted(merge_buf)}")
+
+
+def load_mxfp4_state_dict(items: Iterable[Tuple[str, torch.Tensor]], rank: int, world: int,
+                          num_kv_heads: Optional[int], quantise: Optional[Quantiser] = None,
+                          device: Optional[torch.device] = None,
+                          dtype: torch.dtype = torch.bfloat16) -> Dict[str, torch.Tensor]:
+    """``dict(mxfp4_weight_stream(...))``: the state dict to hand to a model
+    built of the MXFP4 layers."""
+    return dict(mxfp4_weight_stream(items, rank, world, num_kv_heads, quantise, device, dtype))
