@@ -207,10 +207,12 @@ __device__ __forceinline__ float to_float<__nv_bfloat16>(__nv_bfloat16 x) { retu
 template <>
 __device__ __forceinline__ float to_float<__half>(__half x) { return __half2float(x); }
 
-// silu(g) * u in fp32 on the ex2 and rcp units.  For g in [-40, inf) the
-// relative error is below 2^-18: the argument -g log2(e) carries at most
-// 58 (2^-24 + 2^-25.9) absolute error, i.e. 3e-6 relative in exp, ex2 and rcp
-// about 2^-22 each, and three roundings.  Below that see the callers.
+// silu(g) * u in fp32 on the ex2 and rcp units, as (g u) / (1 + exp(-g)).  For
+// g in [-40, inf) the relative error is below 2^-18: the argument -g log2(e)
+// carries at most 58 (2^-24 + 2^-25) absolute error, i.e. 3.6e-6 relative in
+// exp, ex2 and rcp about 2^-22 each, and three roundings.  (g u taken first
+// keeps subnormal gates exact where a large up lifts them; where it overflows
+// although the quotient would not, the result is not finite.)
 __device__ __forceinline__ float ex2_approx(float x) {
   float y;
   asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(y) : "f"(x));
@@ -226,7 +228,7 @@ __device__ __forceinline__ float2 silu_mul_fast(float2 g, float2 u) {
   constexpr float c = -1.4426950408889634f;
   const float2 t = __fmul2_rn(g, make_float2(c, c));
   const float2 d = __fadd2_rn(make_float2(ex2_approx(t.x), ex2_approx(t.y)), make_float2(1.0f, 1.0f));
-  return __fmul2_rn(__fmul2_rn(g, make_float2(rcp_approx(d.x), rcp_approx(d.y))), u);
+  return __fmul2_rn(__fmul2_rn(g, u), make_float2(rcp_approx(d.x), rcp_approx(d.y)));
 }
 
 __device__ __forceinline__ float silu_mul_fast(float g, float u) {

@@ -95,7 +95,7 @@ def silu_mul(gate: torch.Tensor, up: torch.Tensor) -> torch.Tensor:
 
 def rmsnorm(x: torch.Tensor, weight: torch.Tensor, eps: float, residual: Optional[torch.Tensor] = None):
     """``(y fp64, new residual in x's type or None)``."""
-    v = x.double() + (0 if residual is None else residual.double())
+    v = x.double() if residual is None else (x.float() + residual.float()).double()  # the fp32 sum
     y = v / torch.sqrt(v.square().mean(-1, keepdim=True) + eps) * weight.double()
     res = None if residual is None else (x.float() + residual.float()).to(x.dtype)
     return y, res
