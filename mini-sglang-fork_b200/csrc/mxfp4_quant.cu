@@ -265,6 +265,18 @@ __device__ __noinline__ uint2 norm_exact(Vec8 v, uint4 wr, NormRow n, int lane) 
   });
 }
 
+// Sum over the CTA, in every thread and in an order that does not vary.
+__device__ __forceinline__ double block_sum(double x, double* part, int warps) {
+#pragma unroll
+  for (int o = 16; o > 0; o >>= 1) x += __shfl_xor_sync(0xffffffffu, x, o);
+  if (warps == 1) return x;
+  if ((threadIdx.x & 31) == 0) part[threadIdx.x >> 5] = x;
+  __syncthreads();
+  x = 0.0;
+  for (int i = 0; i < warps; ++i) x += part[i];
+  return x;
+}
+
 template <typename T, int VPT, int MAX_THREADS, bool ADD>
 __global__ void __launch_bounds__(MAX_THREADS)
     rmsnorm_kernel(const T* __restrict__ x, int64_t ldx, T* residual, int64_t ldr, const T* __restrict__ weight,
@@ -316,28 +328,23 @@ __global__ void __launch_bounds__(MAX_THREADS)
 #pragma unroll
     for (int e = 0; e < 4; e += 2) {
       const float2 q = __ffma2_rn(v[j].p[e + 1], v[j].p[e + 1], __fmul2_rn(v[j].p[e], v[j].p[e]));
-      const float s = q.x + q.y;
-      if (s > 1e30f || s < 1e-30f) {  // squares near the ends of fp32's range
-        for (int i = 0; i < 2; ++i)
-          ss += static_cast<double>(v[j].p[e + i].x) * v[j].p[e + i].x +
-                static_cast<double>(v[j].p[e + i].y) * v[j].p[e + i].y;
-      } else {
-        ss += s;
-      }
+      ss += q.x + q.y;
     }
   }
-#pragma unroll
-  for (int o = 16; o > 0; o >>= 1) ss += __shfl_xor_sync(0xffffffffu, ss, o);
-  if (warps > 1) {
-    if (lane == 0) part[threadIdx.x >> 5] = ss;
-    __syncthreads();
+  ss = block_sum(ss, part, warps);
+  const double mean = ss * (1.0 / K) + static_cast<double>(eps);
+  // A row whose mean square nears the ends of fp32's range, where squares
+  // overflow or lose digits, is summed again and finished in 64 bits.
+  const bool far = !(mean > 1e-25 && mean < 1e25);
+  if (far) {
     ss = 0.0;
-    for (int i = 0; i < warps; ++i) ss += part[i];
+    for (int j = 0; j < VPT; ++j)
+      for (int e = 0; e < 4; ++e)
+        ss += static_cast<double>(v[j].p[e].x) * v[j].p[e].x + static_cast<double>(v[j].p[e].y) * v[j].p[e].y;
+    __syncthreads();  // `part` has been read
+    ss = block_sum(ss, part, warps);
   }
   const NormRow n = {ss, K, eps};
-  const double mean = ss * (1.0 / K) + static_cast<double>(eps);
-  // a row whose mean square nears the ends of fp32's range is taken in 64 bits
-  const bool far = !(mean > 1e-30 && mean < 1e30);
   const float r = 1.0f / sqrtf(static_cast<float>(mean));
   const float2 r2 = make_float2(r, r);
   uint8_t* sw = scales + scale_word(row, kt, lane);
@@ -491,6 +498,7 @@ int run_norm(const void* x, int64_t ldx, void* residual, int64_t ldr, const void
                            static_cast<const T*>(weight), eps, data, scales, static_cast<int>(K)))
   if (vpt == 1) MXFP4_NORM(1, 1024);
   else if (vpt == 2) MXFP4_NORM(2, 1024);
+  else if (threads <= 256) MXFP4_NORM(4, 256);
   else if (threads <= 512) MXFP4_NORM(4, 512);
   else MXFP4_NORM(4, 1024);
 #undef MXFP4_NORM
