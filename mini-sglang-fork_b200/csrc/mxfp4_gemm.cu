@@ -31,8 +31,9 @@ struct Operands {
   int64_t b_rows;  // rows of B: N, or 2I
 };
 
-// Clusters of s CTAs of `Kern` (one CTA per SM) that the device holds at once:
-// fewer than SMs / s, since a cluster lives in one group of SMs.
+// Clusters of s CTAs of `Kern` that the device holds at once with one CTA per
+// SM, which is what the query assumes of kernels that allocate TMEM: fewer than
+// SMs / s, since a cluster lives in one group of SMs.
 template <auto Kern>
 int active_clusters(int s, int threads, int smem, int* out) {
   static std::mutex mu;
@@ -88,12 +89,12 @@ int launch_cluster(Kernel kern, unsigned grid, int threads, int smem, int cluste
 // exchange costs 2 us for 128 tokens, and more than it saves below two k
 // blocks, six with the SiLU epilogue's two sums, eight for a 256 x 256 block).
 template <auto Kern>
-int pick_split(int64_t tiles, int kblocks, int threads, int smem, int ctas, int most, int least, int* out) {
+int pick_split(int64_t tiles, int kblocks, int threads, int smem, int per_sm, int ctas, int most, int least, int* out) {
   *out = 1;
-  for (int s = 2; s <= std::min(most, kblocks / least) && tiles * s * ctas <= sm_count(); ++s) {
+  for (int s = 2; s <= std::min(most, kblocks / least) && tiles * s * ctas <= per_sm * sm_count(); ++s) {
     int n = 0;
     if (int rc = active_clusters<Kern>(s * ctas, threads, smem, &n)) return rc;
-    if (tiles <= n) *out = s;
+    if (tiles <= per_sm * n) *out = s;
   }
   return W8A8_OK;
 }
@@ -115,9 +116,8 @@ int launch_row(const Operands& o, MxGemmArgs args, cudaStream_t stream) {
   args.tiles = static_cast<int>(tiles);
   int split = 1;
   if (DEEP)
-    if (int rc = pick_split<kern>(tiles, args.kblocks, kRowThreads, P::kSmemBytes, 1, 8, SILU ? 6 : 2, &split)) return rc;
-  // (CTAs that have an SM each are persistent)
-  const int64_t grid = split > 1 ? tiles * split : DEEP ? std::min<int64_t>(tiles, std::max(1, sm_count())) : tiles;
+    if (int rc = pick_split<kern>(tiles, args.kblocks, kRowThreads, P::kSmemBytes, P::kPerSm, 1, 8, SILU ? 6 : 2, &split)) return rc;
+  const int64_t grid = split > 1 ? tiles * split : P::kPersistent ? std::min<int64_t>(tiles, std::max(1, sm_count())) : tiles;
   return launch_cluster(kern, static_cast<unsigned>(grid), kRowThreads, P::kSmemBytes, split, stream, tw, tws, tx, txs,
                         args);
 }
@@ -139,7 +139,7 @@ int launch_pair(const Operands& o, const MxGemmArgs& g, cudaStream_t stream) {
   if (int rc = encode_operand(&tb, o.b, o.b_rows, g.K / 2, 128)) return rc;
   if (int rc = encode_words(&tbs, o.bs, row_tiles(o.b_rows), k_tiles(g.K) * kTileBytes / 4, 256)) return rc;
   int split = 1;
-  if (int rc = pick_split<kern>(blocks, g.kblocks, PairTraits::kThreads, PairTraits::kSmemBytes, 2, 2, 8, &split)) return rc;
+  if (int rc = pick_split<kern>(blocks, g.kblocks, PairTraits::kThreads, PairTraits::kSmemBytes, 1, 2, 2, 8, &split)) return rc;
   const int64_t pairs = split > 1 ? blocks * split : std::min<int64_t>(blocks, std::max(1, sm_count() / 2));
   return launch_cluster(kern, static_cast<unsigned>(2 * pairs), PairTraits::kThreads, PairTraits::kSmemBytes, 2 * split,
                         stream, ta, tas, tb, tbs, args);

@@ -174,14 +174,15 @@ __device__ __forceinline__ void silu_block(const MxGemmArgs& g, const float (&ga
 // rows, on the MMA's 128-row side) for T tokens; with the SiLU epilogue 128
 // gate rows and the 128 up rows that belong to them, in two accumulators.
 // The weights are read once, at the rate of HBM, which is what bounds it; the
-// ring (about 200 KB of an SM's shared memory, in one CTA or in two) is there
-// to keep enough of them in flight.
+// ring (about 200 KB of an SM's shared memory, in one CTA or in several) is
+// there to keep enough of them in flight.
 //
-// With more tiles than SMs, CTAs are small enough for two or three on an SM and
-// one computes while others start or end (51200 x 5120, one token: 22.9 us; one
-// persistent CTA per SM with the same ring: 24.5).  With fewer tiles a CTA
-// takes the SM for itself, and with at most half as many, a
-// cluster of S CTAs splits K: CTA r writes an S-th of the tokens, and every CTA
+// Up to 32 tokens, two CTAs share an SM, so that one starts (its weights asked
+// for in L2) while the other ends; three with more tiles than SMs (51200 x
+// 5120, one token: 23.2 us; one persistent CTA per SM with the same ring:
+// 24.5).  With few tiles a cluster of S CTAs splits K (5120 x 25600, one token:
+// 14.0 us with six shares, two CTAs per SM; 15.0 with three shares, one per SM;
+// 29.6 without): CTA r writes an S-th of the tokens, and every CTA
 // sends it its fp32 sums of those by a bulk copy between shared memories, the
 // fast way there (gate_up 1536 x 4096, 64 tokens, eight shares: 11.5 us; 22.5
 // with loads from the peers' memory, 32.8 with stores to it).  r adds them up
@@ -196,11 +197,13 @@ struct MxRowTraits {
   static constexpr int kStageBytes = kTiles * (kW + kSf) + kX + kSf;
   static constexpr int kSfCols = 8 * (kTiles + 1);  // TMEM columns of a stage's scales
   static constexpr int kStages = SILU   ? (T == 16 ? 5 : 4)
-                                 : DEEP ? (T <= 32 ? 10 : T == 64 ? 8 : 6)
+                                 : DEEP ? (T <= 32 ? 5 : T == 64 ? 8 : 6)
                                         : (T <= 32 ? 3 : 4);
   static constexpr int kChunk = T < 32 ? T : 32;  // columns that the epilogue takes at a time
   static constexpr int kAccCols = kTiles * T;
-  static constexpr int kAccs = (SILU || DEEP) && 2 * kAccCols + kStages * kSfCols <= 512 ? 2 : 1;
+  // CTAs that take tile after tile have two accumulators where TMEM allows
+  static constexpr bool kPersistent = SILU || T == 128;
+  static constexpr int kAccs = kPersistent && 2 * kAccCols + kStages * kSfCols <= 512 ? 2 : 1;
   static constexpr int kColsNeeded = kAccs * kAccCols + kStages * kSfCols;
   static constexpr int kTmemCols = kColsNeeded <= 64 ? 64 : kColsNeeded <= 128 ? 128 : kColsNeeded <= 256 ? 256 : 512;
   static constexpr int kBarrierBytes = 256;
@@ -208,6 +211,7 @@ struct MxRowTraits {
   static constexpr int kSmemBytes = 1024 + kStages * kStageBytes + kBarrierBytes + kStagingBytes;
   static_assert(kColsNeeded <= 512, "TMEM");
   static_assert(kSmemBytes <= 227 * 1024, "shared memory");
+  static constexpr int kPerSm = 228 * 1024 / (kSmemBytes + 1024);  // CTAs on an SM
   // At most three CTAs with at most 128 TMEM columns each share an SM, and one
   // with more leaves no room for another.  So every allocation succeeds at
   // once, and no CTA of a cluster waits for TMEM that a CTA waiting for it
