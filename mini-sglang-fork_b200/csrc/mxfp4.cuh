@@ -90,17 +90,6 @@ __device__ __forceinline__ uint32_t pack8_scaled(const Vec8& v, float f) {
   return w;
 }
 
-// The E2M1 code of one value (already scaled).
-__device__ __forceinline__ uint32_t code_of(float t) {
-  uint32_t w;
-  asm("{\n\t.reg .b8 b0;\n\t"
-      "cvt.rn.satfinite.e2m1x2.f32 b0, %2, %1;\n\t"
-      "cvt.u32.u8 %0, b0;\n\t}"
-      : "=r"(w)
-      : "f"(t), "f"(0.0f));
-  return w;
-}
-
 // ---- 64-bit forms, for the values next to a border
 // E2M1 code of t (already divided by the block's scale).
 __device__ inline uint32_t code_of(double t) {
@@ -231,8 +220,13 @@ __device__ __forceinline__ float2 silu_mul_fast(float2 g, float2 u) {
   return __fmul2_rn(__fmul2_rn(g, u), make_float2(rcp_approx(d.x), rcp_approx(d.y)));
 }
 
-__device__ __forceinline__ float silu_mul_fast(float g, float u) {
-  return silu_mul_fast(make_float2(g, 0.0f), make_float2(u, 0.0f)).x;
+// The same with the sigmoid taken into g first, for callers without a second
+// look: finite for every finite product, and a zero once exp(-g) overflows.
+__device__ __forceinline__ float2 silu_mul_plain(float2 g, float2 u) {
+  constexpr float c = -1.4426950408889634f;
+  const float2 t = __fmul2_rn(g, make_float2(c, c));
+  const float2 d = __fadd2_rn(make_float2(ex2_approx(t.x), ex2_approx(t.y)), make_float2(1.0f, 1.0f));
+  return __fmul2_rn(__fmul2_rn(g, make_float2(rcp_approx(d.x), rcp_approx(d.y))), u);
 }
 
 }  // namespace mx

@@ -279,7 +279,7 @@ __device__ __forceinline__ double block_sum(double x, double* part, int warps) {
 
 template <typename T, int VPT, int MAX_THREADS, bool ADD>
 __global__ void __launch_bounds__(MAX_THREADS)
-    rmsnorm_kernel(const T* __restrict__ x, int64_t ldx, T* residual, int64_t ldr, const T* __restrict__ weight,
+    rmsnorm_kernel(const T* x, int64_t ldx, T* residual, int64_t ldr, const T* __restrict__ weight,
                    float eps, uint8_t* __restrict__ data, uint8_t* __restrict__ scales, int K) {
   __shared__ double part[MAX_THREADS / 32];
   const int lane = threadIdx.x & 31;

@@ -152,7 +152,7 @@ __device__ __forceinline__ void silu_block(const MxGemmArgs& g, const float (&ga
       gv = __fadd2_rn(gv, make_float2(to_float(b[0]), to_float(b[1])));
       uv = __fadd2_rn(uv, make_float2(to_float(b[g.N]), to_float(b[g.N + 1])));
     }
-    y[e >> 2].p[e & 3] = silu_mul_fast(gv, uv);
+    y[e >> 2].p[e & 3] = silu_mul_plain(gv, uv);
   }
   const float m = max3_abs(max3_abs(amax8(y[0]), amax8(y[1]), amax8(y[2])), amax8(y[3]), 0.0f);
   const int byte = scale_byte(abs_bits(m));

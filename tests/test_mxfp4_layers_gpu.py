@@ -4,9 +4,14 @@ and the calls at the edges: no rows, rows inside larger buffers, more than 2^32
 values, refused alignments."""
 from __future__ import annotations
 
+import subprocess
+import sys
+import threading
+
 import pytest
 import torch
 
+from conftest import ROOT
 from oracle import mxfp4_oracle as O
 from test_mxfp4_gpu import _gemm_bound, _gen, _operand, _same
 
@@ -183,6 +188,100 @@ def test_streams_at_once(pkg, cuda_dev):
                 got.append(d(*_inputs(m, cuda_dev, m))[0])
         torch.cuda.synchronize()
         assert all(torch.equal(a, b) for a, b in zip(got, want))
+
+
+_FIRST = """
+import importlib, sys, torch
+sys.path.insert(0, {root!r})
+p = importlib.import_module("mini-sglang-fork_b200")
+x = torch.randn(20, 4096, device="cuda").bfloat16()
+w = torch.randn(512, 4096, device="cuda").bfloat16()
+n = torch.ones(4096, device="cuda").bfloat16()
+g = torch.cuda.CUDAGraph()
+with torch.cuda.graph(g):
+    q, _ = p.mxfp4_rmsnorm_quant(x, n, 1e-6)
+    b = p.mxfp4_quant(w)
+    y = p.mxfp4_gemm(q, b)
+    z = p.mxfp4_dequant(p.mxfp4_gate_up_silu_quant(q, b))
+g.replay()
+torch.cuda.synchronize()
+q, _ = p.mxfp4_rmsnorm_quant(x, n, 1e-6)
+assert torch.equal(y, p.mxfp4_gemm(q, p.mxfp4_quant(w)))
+assert torch.equal(z, p.mxfp4_dequant(p.mxfp4_gate_up_silu_quant(q, p.mxfp4_quant(w))))
+print("captured first")
+"""
+
+
+def test_first_calls_may_be_captured(cuda_dev):
+    """A process whose first MXFP4 calls are inside a capture: whatever is set
+    up once per device does not disturb it."""
+    r = subprocess.run([sys.executable, "-c", _FIRST.format(root=ROOT)], capture_output=True, text=True, timeout=240)
+    assert r.returncode == 0 and "captured first" in r.stdout, r.stdout + r.stderr
+
+
+def test_calls_from_two_threads(pkg, cuda_dev):
+    d = _Decoder(pkg, cuda_dev)
+    want = {m: d(*_inputs(m, cuda_dev, m))[0] for m in (4, 200)}
+    torch.cuda.synchronize()
+    bad = []
+
+    def work(m):
+        with torch.cuda.stream(torch.cuda.Stream()):
+            for _ in range(20):
+                if not torch.equal(d(*_inputs(m, cuda_dev, m))[0], want[m]):
+                    bad.append(m)
+
+    threads = [threading.Thread(target=work, args=(m,)) for m in want]
+    for t in threads:
+        t.start()
+    for t in threads:
+        t.join()
+    assert not bad
+
+
+def test_residual_is_the_input(pkg, cuda_dev):
+    """The same tensor as x and residual: v = 2x, written back in place."""
+    x, _ = _inputs(9, cuda_dev, 0)
+    w = torch.ones(512, dtype=torch.bfloat16, device=cuda_dev)
+    y, r = O.rmsnorm(x.cpu(), w.cpu(), 1e-6, x.cpu())
+    q, out = pkg.mxfp4_rmsnorm_quant(x, w, 1e-6, x)
+    _same(q, *O.quant(y))
+    assert torch.equal(out.cpu(), r) and torch.equal(x.cpu(), r)
+
+
+def _far(pkg, dev, negative):
+    """Operands with gates around 2^22 and ups around 2^112; `negative`: every
+    gate below zero."""
+    k, i = 64, 128
+    a, _ = _operand(pkg, 3, k, 1.0, 0, dev)
+    w, _ = _operand(pkg, 2 * i, k, 1.0, 1, dev)
+    data, wdata = a.data.clone(), w.data.clone()
+    if negative:
+        data &= 0x77  # magnitudes
+        wdata[:i] |= 0x88
+    scale = torch.full((3, 2), 127 + 20, dtype=torch.uint8, device=dev)
+    wscale = torch.full((2 * i, 2), 127, dtype=torch.uint8, device=dev)
+    wscale[i:] = 127 + 90
+    a = pkg.MXFP4Tensor(data, pkg.ops.mxfp4_tile_scales(scale))
+    w = pkg.MXFP4Tensor(wdata, pkg.ops.mxfp4_tile_scales(wscale))
+    gu = O.decode(a.data, a.scales) @ O.decode(w.data, w.scales).T
+    return pkg.mxfp4_dequant(pkg.mxfp4_gate_up_silu_quant(a, w)).cpu(), gu[:, :i], gu[:, i:]
+
+
+def test_gated_product_far_gates(pkg, cuda_dev):
+    """Gates whose exp overflows give zeros, not NaN, next to ups that overflow
+    with them."""
+    y, g, u = _far(pkg, cuda_dev, negative=True)
+    assert (g < -200).all() and ((g * u).abs() > O.FP32_MAX).any()
+    assert (y == 0).all()
+
+
+def test_gated_product_overflow(pkg, cuda_dev):
+    """A product beyond fp32 makes its block NaN, and no block without one."""
+    y, g, u = _far(pkg, cuda_dev, negative=False)
+    over = (O.silu_mul(g, u).abs() > O.FP32_MAX).reshape(3, 4, 32).any(-1)
+    assert over.any()
+    assert torch.equal(y.isnan().reshape(3, 4, 32), over[..., None].expand(3, 4, 32))
 
 
 @pytest.mark.parametrize("m,n,k", [(1, 640, 5120), (40, 512, 8192), (100, 1024, 2048), (200, 512, 8192), (1000, 768, 256)])
