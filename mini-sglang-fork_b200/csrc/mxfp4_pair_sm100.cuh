@@ -37,7 +37,8 @@ struct PairTraits {
   static_assert(kSfCol + kStages * kSfCols <= 512, "TMEM");
   static constexpr int kBarrierBytes = 256;
   static constexpr int kStagingBytes = kEpiWarps * 2048;
-  static constexpr int kSmemBytes = 1024 + kStages * kStageBytes + kBarrierBytes + kStagingBytes;
+  static constexpr int kBiasBytes = 2 * 1024;  // of a block's 256 columns, for two blocks
+  static constexpr int kSmemBytes = 1024 + kStages * kStageBytes + kBarrierBytes + kStagingBytes + kBiasBytes;
   static_assert(kSmemBytes <= 227 * 1024, "shared memory");
   static_assert(2 * 128 * 128 * 4 <= kStages * kStageBytes, "the shares reuse the ring");
   static_assert(kSmemBytes >= 170 * 1024, "TMEM share");  // as for MxRowTraits
@@ -92,17 +93,22 @@ __device__ __forceinline__ uint32_t pair_part_word(int r, int c) {
   return static_cast<uint32_t>(r * 32 + (((c >> 2) ^ (r & 7)) << 2));
 }
 
-// Plain epilogue of 32 columns (from `col0`) of a warp's 32 rows: through the
+// Plain epilogue of 32 columns (from `col0`, their biases in shared memory at
+// `bias`) of a warp's 32 rows: through the
 // warp's 2 KB of shared memory (16-byte pieces, the piece index XORed with the
 // row pair: no bank conflict either way) to rows of 64 contiguous bytes.
 template <typename O>
-__device__ __forceinline__ void plain_chunk(const MxGemmArgs& g, uint32_t (&v)[32], uint4* stg, int lane, int64_t row0,
-                                            int col0) {
+__device__ __forceinline__ void plain_chunk(const MxGemmArgs& g, const float* bias, uint32_t (&v)[32], uint4* stg,
+                                            int lane, int64_t row0, int col0) {
   if (g.bias) {
-    const O* b = static_cast<const O*>(g.bias) + col0;
 #pragma unroll
-    for (int e = 0; e < 32; ++e)
-      if (col0 + e < g.N) v[e] = __float_as_uint(__uint_as_float(v[e]) + to_float(b[e]));
+    for (int i = 0; i < 8; ++i) {
+      const float4 b = *reinterpret_cast<const float4*>(bias + 4 * i);
+      v[4 * i] = __float_as_uint(__uint_as_float(v[4 * i]) + b.x);
+      v[4 * i + 1] = __float_as_uint(__uint_as_float(v[4 * i + 1]) + b.y);
+      v[4 * i + 2] = __float_as_uint(__uint_as_float(v[4 * i + 2]) + b.z);
+      v[4 * i + 3] = __float_as_uint(__uint_as_float(v[4 * i + 3]) + b.w);
+    }
   }
 #pragma unroll
   for (int e = 0; e < 4; ++e) {
@@ -149,6 +155,7 @@ __global__ void __launch_bounds__(PairTraits::kThreads, 1)
   uint32_t* tmem_slot = reinterpret_cast<uint32_t*>(drain + 2);
   volatile int* abort_flag = reinterpret_cast<volatile int*>(tmem_slot + 1);
   uint8_t* staging = reinterpret_cast<uint8_t*>(bars) + P::kBarrierBytes;
+  float* bias_s = reinterpret_cast<float*>(staging + P::kStagingBytes);
 
   const int warp = threadIdx.x >> 5;
   const int lane = threadIdx.x & 31;
@@ -309,9 +316,15 @@ __global__ void __launch_bounds__(PairTraits::kThreads, 1)
       pair_block(args, p, pm, tn);
       const int row0 = (2 * pm + static_cast<int>(half)) * 128 + quarter * 32;  // this warp's rows
       const uint32_t acc = blk & 1u;
-      const bool ok =
-          dev::mbar_wait(dev::smem_u32(acc_full + acc), (blk >> 1) & 1u, abort_flag, g.err, kErrGemmWait, tmo);
-      if (!__all_sync(0xffffffffu, ok)) break;
+      float* bias = bias_s + acc * 256;  // before the wait for the sums
+      if (g.bias) {
+        const int et = threadIdx.x - 64;
+        const O* b = static_cast<const O*>(g.bias);
+        const int c = SILU ? tn * 128 + (et & 127) + (et >> 7) * g.N : tn * 256 + et;
+        bias[et] = SILU || c < g.N ? to_float(b[c]) : 0.0f;
+      }
+      const bool ok = warp_wait(dev::smem_u32(acc_full + acc), (blk >> 1) & 1u, abort_flag, g.err, tmo);
+      if (g.bias ? dev::named_bar_or(1, 32 * P::kEpiWarps, !ok) : !ok) break;  // (publishes the biases)
       dev::tc_fence_after();
       const uint32_t t = tmem + lanes + acc * P::kAccStep;
       if (S > 1) break;  // one block, finished below
@@ -335,7 +348,7 @@ __global__ void __launch_bounds__(PairTraits::kThreads, 1)
             gate[e] = __uint_as_float(acc ? sh[e] : own[e]);
             up[e] = __uint_as_float(acc ? own[e] : sh[e]);
           }
-          silu_block<O>(g, gate, up, row0 + lane, tn, j);
+          silu_block(g, bias, gate, up, row0 + lane, tn, j);
         };
         dev::tmem_ld32(own_t + 32 * hh, v);
         dev::tmem_wait_ld(v);
@@ -346,13 +359,15 @@ __global__ void __launch_bounds__(PairTraits::kThreads, 1)
       } else {
         const int cs = tn * 256 + (acc ? 0 : 128) + 32 * hh, co = tn * 256 + (acc ? 128 : 0) + 32 * hh;
         dev::tmem_ld32(own_t + 32 * hh, v);  // lands while the first chunk is written
-        plain_chunk<O>(g, s0, stg, lane, row0, cs);
-        plain_chunk<O>(g, s1, stg, lane, row0, cs + 64);
+        const float* bs = bias + (cs - tn * 256);
+        const float* bo = bias + (co - tn * 256);
+        plain_chunk<O>(g, bs, s0, stg, lane, row0, cs);
+        plain_chunk<O>(g, bs + 64, s1, stg, lane, row0, cs + 64);
         dev::tmem_wait_ld(v);
         dev::tmem_ld32(own_t + 32 * hh + 64, s0);
-        plain_chunk<O>(g, v, stg, lane, row0, co);
+        plain_chunk<O>(g, bo, v, stg, lane, row0, co);
         dev::tmem_wait_ld(s0);
-        plain_chunk<O>(g, s0, stg, lane, row0, co + 64);
+        plain_chunk<O>(g, bo + 64, s0, stg, lane, row0, co + 64);
       }
     }
     dev::tc_fence_before();
@@ -421,15 +436,15 @@ __global__ void __launch_bounds__(PairTraits::kThreads, 1)
             gate[e] = __uint_as_float(v[e]);
             up[e] = __uint_as_float(w[e]);
           }
-          silu_block<O>(g, gate, up, row0 + lane, tn, 2 * share + hh);
+          silu_block(g, bias_s, gate, up, row0 + lane, tn, 2 * share + hh);
         } else {
 #pragma unroll 1
           for (int i = hh; i < 4; i += 2) {
             dev::tmem_ld32(t + column(share, i), v);
             dev::tmem_wait_ld(v);
             sum(i, v);
-            plain_chunk<O>(g, v, reinterpret_cast<uint4*>(staging + (warp - 2) * 2048), lane, row0,
-                           tn * 256 + column(share, i));
+            plain_chunk<O>(g, bias_s + column(share, i), v, reinterpret_cast<uint4*>(staging + (warp - 2) * 2048), lane,
+                           row0, tn * 256 + column(share, i));
           }
         }
       }

@@ -135,24 +135,45 @@ __device__ __forceinline__ void store8_row(const MxGemmArgs& g, int64_t row, int
   }
 }
 
+// Bias of eight columns from `col` (a multiple of 8), zero beyond column N: one
+// load where the pointer allows it.
+template <typename O>
+__device__ __forceinline__ Vec8 bias8(const void* bias, int col, int N) {
+  const O* b = static_cast<const O*>(bias) + col;
+  if ((reinterpret_cast<uintptr_t>(bias) & 15u) == 0 && col + 8 <= N) return unpack8<O>(__ldg(reinterpret_cast<const uint4*>(b)));
+  Vec8 v;
+#pragma unroll
+  for (int e = 0; e < 4; ++e)
+    v.p[e] = make_float2(col + 2 * e < N ? to_float(b[2 * e]) : 0.0f, col + 2 * e + 1 < N ? to_float(b[2 * e + 1]) : 0.0f);
+  return v;
+}
+
 // silu(gate) * up of 32 features (block `j` of 128-feature tile `ft`) of one
 // output row, as one MXFP4 block.  Here the sums themselves carry fp32's
 // rounding, so the product is quantised as it comes, in one conversion.
-template <typename O>
-__device__ __forceinline__ void silu_block(const MxGemmArgs& g, const float (&gate)[32], const float (&up)[32],
-                                           int64_t row, int ft, int j) {
+// `bias`: the tile's 128 gate and 128 up biases in shared memory.
+__device__ __forceinline__ void silu_block(const MxGemmArgs& g, const float* bias, const float (&gate)[32],
+                                           const float (&up)[32], int64_t row, int ft, int j) {
   const int f0 = ft * 128 + 32 * j;
   Vec8 y[4];
 #pragma unroll
-  for (int e = 0; e < 16; ++e) {
-    float2 gv = make_float2(gate[2 * e], gate[2 * e + 1]);
-    float2 uv = make_float2(up[2 * e], up[2 * e + 1]);
-    if (g.bias) {
-      const O* b = static_cast<const O*>(g.bias) + f0 + 2 * e;
-      gv = __fadd2_rn(gv, make_float2(to_float(b[0]), to_float(b[1])));
-      uv = __fadd2_rn(uv, make_float2(to_float(b[g.N]), to_float(b[g.N + 1])));
+  for (int i = 0; i < 4; ++i) {
+    Vec8 gv, uv;
+#pragma unroll
+    for (int e = 0; e < 4; ++e) {
+      gv.p[e] = make_float2(gate[8 * i + 2 * e], gate[8 * i + 2 * e + 1]);
+      uv.p[e] = make_float2(up[8 * i + 2 * e], up[8 * i + 2 * e + 1]);
     }
-    y[e >> 2].p[e & 3] = silu_mul_plain(gv, uv);
+    if (g.bias) {
+      const float2* bg = reinterpret_cast<const float2*>(bias + 32 * j + 8 * i);
+#pragma unroll
+      for (int e = 0; e < 4; ++e) {
+        gv.p[e] = __fadd2_rn(gv.p[e], bg[e]);
+        uv.p[e] = __fadd2_rn(uv.p[e], bg[64 + e]);
+      }
+    }
+#pragma unroll
+    for (int e = 0; e < 4; ++e) y[i].p[e] = silu_mul_plain(gv.p[e], uv.p[e]);
   }
   const float m = max3_abs(max3_abs(amax8(y[0]), amax8(y[1]), amax8(y[2])), amax8(y[3]), 0.0f);
   const int byte = scale_byte(abs_bits(m));
@@ -208,7 +229,8 @@ struct MxRowTraits {
   static constexpr int kTmemCols = kColsNeeded <= 64 ? 64 : kColsNeeded <= 128 ? 128 : kColsNeeded <= 256 ? 256 : 512;
   static constexpr int kBarrierBytes = 256;
   static constexpr int kStagingBytes = SILU ? 4 * 2 * kChunk * 128 : 0;  // per epilogue warp: gate, up
-  static constexpr int kSmemBytes = 1024 + kStages * kStageBytes + kBarrierBytes + kStagingBytes;
+  static constexpr int kBiasBytes = SILU ? 2 * 1024 : 0;                 // per accumulator: gate, up
+  static constexpr int kSmemBytes = 1024 + kStages * kStageBytes + kBarrierBytes + kStagingBytes + kBiasBytes;
   static_assert(kColsNeeded <= 512, "TMEM");
   static_assert(kSmemBytes <= 227 * 1024, "shared memory");
   static constexpr int kPerSm = 228 * 1024 / (kSmemBytes + 1024);  // CTAs on an SM
@@ -255,6 +277,7 @@ __global__ void __launch_bounds__(kRowThreads, 1) mx_row_kernel(const __grid_con
   uint32_t* tmem_slot = reinterpret_cast<uint32_t*>(drain + 2);
   volatile int* abort_flag = reinterpret_cast<volatile int*>(tmem_slot + 1);
   uint64_t* arrived = drain + 1;  // S > 1: the peers' shares
+  float* bias_s = reinterpret_cast<float*>(reinterpret_cast<uint8_t*>(bars) + P::kBarrierBytes + P::kStagingBytes);
 
   const int warp = threadIdx.x >> 5;
   const int lane = threadIdx.x & 31;
@@ -289,10 +312,11 @@ __global__ void __launch_bounds__(kRowThreads, 1) mx_row_kernel(const __grid_con
     dev::tmem_relinquish();
   }
   dev::griddep_launch();
-  if (DEEP && warp == 0) {
-    // the first stages' weights into L2 while the previous kernel ends
+  if (warp == 0) {
+    // the first weights into L2 while the previous kernel ends (five k blocks:
+    // 51200 x 5120, one token, 22.0 us against 23.2 without; twenty cost 27)
     if (elect_one()) {
-      for (int kb = kb0; kb < min(kb1, kb0 + P::kStages); ++kb)
+      for (int kb = kb0; kb < min(kb1, kb0 + 5); ++kb)
 #pragma unroll
         for (int h = 0; h < P::kTiles; ++h) {
           const int w0 = first / args.ttiles * 128 + h * args.N;
@@ -410,15 +434,27 @@ __global__ void __launch_bounds__(kRowThreads, 1) mx_row_kernel(const __grid_con
       const int tt = tile % args.ttiles, wt = tile / args.ttiles;
       const int tokens = min(T, args.M - tt * T);
       const uint32_t acc = i % P::kAccs, use = i / P::kAccs;
+      // the biases before the wait for the sums
+      const int col = wt * 128 + n;
+      float* bias = bias_s + (i & 1u) * 256;
+      float bias_n = 0.0f;
+      if (args.bias) {
+        const O* b = static_cast<const O*>(args.bias);
+        if constexpr (SILU) {
+          bias[n] = to_float(b[col]);
+          bias[128 + n] = to_float(b[args.N + col]);
+        } else if (col < args.N) {
+          bias_n = to_float(b[col]);
+        }
+      }
       // (a failed wait leaves the result unspecified; the error word says so)
-      if (!warp_wait(dev::smem_u32(acc_full + acc), use & 1u, abort_flag, args.err, tmo)) break;
+      const bool ok = warp_wait(dev::smem_u32(acc_full + acc), use & 1u, abort_flag, args.err, tmo);
+      if (SILU && args.bias ? dev::named_bar_or(1, 128, !ok) : !ok) break;  // (publishes the biases)
       dev::tc_fence_after();
       const uint32_t t_acc = tmem + lanes + acc * P::kAccCols;
       if (S > 1) break;  // one tile, finished below
       if constexpr (!SILU) {
-        const int col = wt * 128 + n;
         const bool in = col < args.N;
-        const float bias = args.bias && in ? to_float(static_cast<const O*>(args.bias)[col]) : 0.0f;
         O* out = static_cast<O*>(args.out) + static_cast<int64_t>(tt) * T * args.N + col;
         for (int c = 0; c < tokens; c += P::kChunk) {
           float v[32];
@@ -426,7 +462,7 @@ __global__ void __launch_bounds__(kRowThreads, 1) mx_row_kernel(const __grid_con
 #pragma unroll
           for (int j = 0; j < P::kChunk; ++j)
             if (c + j < tokens && in) {
-              const uint32_t p = pack2<O>(v[j] + bias, 0.0f);
+              const uint32_t p = pack2<O>(v[j] + bias_n, 0.0f);
               *reinterpret_cast<uint16_t*>(out + static_cast<int64_t>(c + j) * args.N) = static_cast<uint16_t>(p);
             }
         }
@@ -451,7 +487,7 @@ __global__ void __launch_bounds__(kRowThreads, 1) mx_row_kernel(const __grid_con
               *reinterpret_cast<float4*>(g + 4 * e) = *reinterpret_cast<const float4*>(stg + w);
               *reinterpret_cast<float4*>(u + 4 * e) = *reinterpret_cast<const float4*>(stg + P::kChunk * 32 + w);
             }
-            silu_block<O>(args, g, u, static_cast<int64_t>(tt) * T + c + lane, wt, q);
+            silu_block(args, bias, g, u, static_cast<int64_t>(tt) * T + c + lane, wt, q);
           }
           __syncwarp();
         }
@@ -518,10 +554,9 @@ __global__ void __launch_bounds__(kRowThreads, 1) mx_row_kernel(const __grid_con
           }
           const int col = wt * 128 + n0;
           if (args.bias) {
-            const O* b = static_cast<const O*>(args.bias) + col;
+            const Vec8 b = bias8<O>(args.bias, col, args.N);
 #pragma unroll
-            for (int j = 0; j < 8; ++j)
-              if (col + j < args.N) v[j] += to_float(b[j]);
+            for (int j = 0; j < 4; ++j) v[2 * j] += b.p[j].x, v[2 * j + 1] += b.p[j].y;
           }
           store8_row<O>(args, row0 + t, col,
                         make_uint4(pack2<O>(v[0], v[1]), pack2<O>(v[2], v[3]), pack2<O>(v[4], v[5]), pack2<O>(v[6], v[7])));
@@ -541,7 +576,7 @@ __global__ void __launch_bounds__(kRowThreads, 1) mx_row_kernel(const __grid_con
               u[4 * e] += y.x, u[4 * e + 1] += y.y, u[4 * e + 2] += y.z, u[4 * e + 3] += y.w;
             }
           }
-          silu_block<O>(args, g, u, row0 + t, wt, j);
+          silu_block(args, bias_s, g, u, row0 + t, wt, j);
         }
       }
     }
