@@ -505,23 +505,24 @@ class MXFP4Tensor:
     :func:`mxfp4_quant` and its fused forms, an operand of :func:`mxfp4_gemm`,
     and accepted by the MXFP4 layers in place of a 16-bit activation."""
 
-    # The operators' results keep codes and scales in one buffer (one
-    # allocation per call) and make the two views when asked for them.
-    __slots__ = ("_buf", "_data", "_scales", "_ptrs", "shape")
+    # The operators' results keep codes and scales in one buffer `_buf` (one
+    # allocation per call) and make the two views when asked for them; made from
+    # two tensors, `_buf` is the first of them.
+    __slots__ = ("_buf", "_data", "_scales", "_codes", "shape")
 
     def __init__(self, data: torch.Tensor, scales: torch.Tensor):
-        if data.dtype != torch.uint8 or data.dim() != 2 or not data.is_contiguous() or data.shape[1] % 16:
+        if data.dtype is not torch.uint8 or data.dim() != 2 or data.shape[1] % 16 or not data.is_contiguous():
             raise _lib.W8A8Error(_lib.ERR_INVALID_ARG, "MXFP4Tensor: data must be contiguous uint8 [R, K/2], K % 32 == 0")
         r, half = data.shape
-        if (scales.dtype != torch.uint8 or not scales.is_contiguous()
-                or scales.shape != mxfp4_scale_shape(r, 2 * half)):
+        if (scales.dtype is not torch.uint8 or scales.shape != ((r + 127) // 128, (half + 127) // 128 * 2, 512)
+                or not scales.is_contiguous()):
             raise _lib.W8A8Error(_lib.ERR_INVALID_ARG, f"MXFP4Tensor: scales must be contiguous uint8 tiles "
                                  f"{mxfp4_scale_shape(r, 2 * half)}, got {scales.dtype} {tuple(scales.shape)}")
-        if scales.device != data.device:
+        if scales.get_device() != data.get_device():
             raise _lib.W8A8Error(_lib.ERR_INVALID_ARG, f"MXFP4Tensor: data on {data.device}, scales on {scales.device}")
         self._buf = self._data = data
         self._scales = scales
-        self._ptrs = (data.data_ptr(), scales.data_ptr())
+        self._codes = -1
         self.shape = (r, 2 * half)
 
     @classmethod
@@ -530,14 +531,17 @@ class MXFP4Tensor:
             raise _lib.W8A8Error(_lib.ERR_INVALID_ARG,
                                  f"MXFP4: the last dimension ({k}) must be a positive multiple of 32")
         t = cls.__new__(cls)
-        codes = rows * (k // 2)
-        t._buf = torch.empty(codes + (rows + 127) // 128 * ((k + 255) // 256) * 1024, dtype=torch.uint8,
-                             device=like.device)
-        p = t._buf.data_ptr()
+        t._codes = codes = rows * (k // 2)
+        t._buf = like.new_empty(codes + (rows + 127) // 128 * ((k + 255) // 256) * 1024, dtype=torch.uint8)
         t._data = t._scales = None
-        t._ptrs = (p, p + codes)
         t.shape = (rows, k)
         return t
+
+    def _ptrs(self) -> Tuple[int, int]:
+        """Addresses of the codes and the scales (of this moment: a caller's
+        tensors may be given other storage)."""
+        p = self._buf.data_ptr()
+        return p, p + self._codes if self._codes >= 0 else self._scales.data_ptr()
 
     @property
     def data(self) -> torch.Tensor:
@@ -561,7 +565,7 @@ class MXFP4Tensor:
         """Marks the memory as in use on another stream (as
         ``torch.Tensor.record_stream``)."""
         self._buf.record_stream(stream)
-        if self._scales is not None and self._buf is self._data:
+        if self._codes < 0:
             self._scales.record_stream(stream)
 
 
@@ -588,24 +592,27 @@ def _mx_call(what: str, fn, t: torch.Tensor, *args) -> None:
     """Launches ``fn(*args, stream)`` on ``t``'s device and that device's
     current stream, whichever device is current."""
     idx = t.get_device()
-    if idx == torch.cuda.current_device():
+    if idx == torch._C._cuda_getDevice():
         status = fn(*args, torch._C._cuda_getCurrentRawStream(idx))
     else:
         with torch.cuda.device(idx):
             status = fn(*args, torch._C._cuda_getCurrentRawStream(idx))
-    if status != _lib.OK:
+    if status:
         _lib.check(status, what)
 
 
 def _check_mx_input(name: str, what: str, x: torch.Tensor) -> int:
     """A 2-D 16-bit CUDA activation with unit column stride; its dtype code.
     (A row stride of 0 or below K, as an expanded or overlapping view has, is
-    refused: only separate rows are read and, for a residual, written.)"""
-    _require_cuda(name, x)
-    if x.dtype not in (torch.bfloat16, torch.float16) or x.dim() != 2 or (x.shape[1] > 1 and x.stride(1) != 1):
+    refused by the library: only separate rows are read and, for a residual,
+    written.)"""
+    if not x.is_cuda:
+        _require_cuda(name, x)
+    code = _MX_DTYPE.get(x.dtype, 2)
+    if code > 1 or x.dim() != 2 or (x.stride(1) != 1 and x.shape[1] > 1):
         raise _lib.W8A8Error(_lib.ERR_INVALID_ARG,
                              f"{name}: {what} must be a 2-D bf16 or fp16 tensor with unit column stride")
-    return _MX_DTYPE[x.dtype]
+    return code
 
 
 def _row_stride(x: torch.Tensor) -> int:
@@ -622,7 +629,7 @@ def mxfp4_quant(x: torch.Tensor) -> MXFP4Tensor:
     dt = _check_mx_input("mxfp4_quant", "x", x)
     m, k = x.shape
     q = MXFP4Tensor._empty(m, k, x)
-    _mx_call("mxfp4_quant", _lib.load().mxfp4_quant, x, x.data_ptr(), _row_stride(x), dt, *q._ptrs, m, k)
+    _mx_call("mxfp4_quant", _lib.load().mxfp4_quant, x, x.data_ptr(), _row_stride(x), dt, *q._ptrs(), m, k)
     return q
 
 
@@ -633,8 +640,8 @@ def mxfp4_dequant(q: MXFP4Tensor, dtype: torch.dtype = torch.bfloat16) -> torch.
         raise _lib.W8A8Error(_lib.ERR_INVALID_ARG, f"mxfp4_dequant: bf16, fp16 or fp32, not {dtype}")
     _require_cuda("mxfp4_dequant", q._buf)
     m, k = q.shape
-    out = torch.empty(m, k, dtype=dtype, device=q.device)
-    _mx_call("mxfp4_dequant", _lib.load().mxfp4_dequant, out, *q._ptrs, out.data_ptr(), _MX_DTYPE[dtype], m, k)
+    out = q._buf.new_empty((m, k), dtype=dtype)
+    _mx_call("mxfp4_dequant", _lib.load().mxfp4_dequant, out, *q._ptrs(), out.data_ptr(), _MX_DTYPE[dtype], m, k)
     return out
 
 
@@ -649,7 +656,7 @@ def mxfp4_silu_and_mul_quant(gate_up: torch.Tensor) -> MXFP4Tensor:
     i = two_i // 2
     q = MXFP4Tensor._empty(m, i, gate_up)
     _mx_call("mxfp4_silu_and_mul_quant", _lib.load().mxfp4_silu_mul_quant, gate_up, gate_up.data_ptr(),
-             _row_stride(gate_up), dt, *q._ptrs, m, i)
+             _row_stride(gate_up), dt, *q._ptrs(), m, i)
     return q
 
 
@@ -672,21 +679,25 @@ def mxfp4_rmsnorm_quant(x: torch.Tensor, weight: torch.Tensor, eps: float,
     _one_device("mxfp4_rmsnorm_quant", x, weight, residual)
     q = MXFP4Tensor._empty(m, k, x)
     _mx_call("mxfp4_rmsnorm_quant", _lib.load().mxfp4_rmsnorm_quant, x, x.data_ptr(), _row_stride(x), _ptr(residual),
-             _row_stride(residual) if residual is not None else k, weight.data_ptr(), float(eps), dt, *q._ptrs, m, k)
+             _row_stride(residual) if residual is not None else k, weight.data_ptr(), float(eps), dt, *q._ptrs(), m, k)
     return q, residual if residual is not None else x
 
 
 def _check_mx_gemm(name: str, a: MXFP4Tensor, w: MXFP4Tensor, bias: Optional[torch.Tensor],
-                   dtype: torch.dtype) -> None:
-    if dtype not in (torch.bfloat16, torch.float16):
+                   dtype: torch.dtype) -> int:
+    """Checks of a product's operands; the dtype code."""
+    code = _MX_DTYPE.get(dtype, 2)
+    if code > 1:
         raise _lib.W8A8Error(_lib.ERR_INVALID_ARG, f"{name}: bf16 or fp16, not {dtype}")
     if a.shape[1] != w.shape[1]:
         raise _lib.W8A8Error(_lib.ERR_INVALID_ARG, f"{name}: shape mismatch A{tuple(a.shape)} B{tuple(w.shape)}")
-    if bias is not None and (bias.dtype != dtype or bias.shape != (w.shape[0],) or not bias.is_contiguous()):
+    if bias is not None and (bias.dtype is not dtype or bias.shape != (w.shape[0],) or not bias.is_contiguous()):
         raise _lib.W8A8Error(_lib.ERR_INVALID_ARG, f"{name}: bias must be contiguous {dtype} [{w.shape[0]}]")
-    _require_cuda(name, a._buf, w._buf, bias)
-    if a.device != w.device or (bias is not None and bias.device != a.device):
+    idx = a._buf.get_device()
+    if idx < 0 or w._buf.get_device() != idx or (bias is not None and bias.get_device() != idx):
+        _require_cuda(name, a._buf, w._buf, bias)
         _one_device(name, a._buf, w._buf, bias)
+    return code
 
 
 def mxfp4_gemm(a: MXFP4Tensor, w: MXFP4Tensor, bias: Optional[torch.Tensor] = None,
@@ -696,17 +707,17 @@ def mxfp4_gemm(a: MXFP4Tensor, w: MXFP4Tensor, bias: Optional[torch.Tensor] = No
     bias has it too, and ``out`` when given)."""
     if out is not None:
         out_dtype = out.dtype
-    _check_mx_gemm("mxfp4_gemm", a, w, bias, out_dtype)
+    code = _check_mx_gemm("mxfp4_gemm", a, w, bias, out_dtype)
     m, k = a.shape
     n = w.shape[0]
     if out is None:
-        out = torch.empty(m, n, dtype=out_dtype, device=a.device)
+        out = a._buf.new_empty((m, n), dtype=out_dtype)
     else:
         _require_cuda("mxfp4_gemm", out)
         _one_device("mxfp4_gemm", a._buf, out)
         _check_2d("mxfp4_gemm out", out, out_dtype, (m, n))
-    _mx_call("mxfp4_gemm", _lib.load().mxfp4_gemm, out, *a._ptrs, *w._ptrs, _ptr(bias), out.data_ptr(),
-             _MX_DTYPE[out_dtype], m, n, k)
+    _mx_call("mxfp4_gemm", _lib.load().mxfp4_gemm, out, *a._ptrs(), *w._ptrs(), _ptr(bias), out.data_ptr(),
+             code, m, n, k)
     return out
 
 
@@ -718,7 +729,7 @@ def mxfp4_gate_up_silu_quant(a: MXFP4Tensor, w: MXFP4Tensor, bias: Optional[torc
     [M, 2I] product reaches memory; otherwise :func:`mxfp4_gemm` (rounding to
     ``dtype``) and :func:`mxfp4_silu_and_mul_quant` run.  ``dtype`` is also the
     bias's type.  I % 32 == 0."""
-    _check_mx_gemm("mxfp4_gate_up_silu_quant", a, w, bias, dtype)
+    code = _check_mx_gemm("mxfp4_gate_up_silu_quant", a, w, bias, dtype)
     m, k = a.shape
     i, odd = divmod(w.shape[0], 2)
     if odd or i % 32:
@@ -727,8 +738,8 @@ def mxfp4_gate_up_silu_quant(a: MXFP4Tensor, w: MXFP4Tensor, bias: Optional[torc
     if i % 128:
         return mxfp4_silu_and_mul_quant(mxfp4_gemm(a, w, bias, out_dtype=dtype))
     y = MXFP4Tensor._empty(m, i, a._buf)
-    _mx_call("mxfp4_gate_up_silu_quant", _lib.load().mxfp4_gemm_silu_quant, a._buf, *a._ptrs, *w._ptrs, _ptr(bias),
-             _MX_DTYPE[dtype], *y._ptrs, m, i, k)
+    _mx_call("mxfp4_gate_up_silu_quant", _lib.load().mxfp4_gemm_silu_quant, a._buf, *a._ptrs(), *w._ptrs(), _ptr(bias),
+             code, *y._ptrs(), m, i, k)
     return y
 
 
