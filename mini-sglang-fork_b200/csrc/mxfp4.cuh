@@ -197,11 +197,12 @@ template <>
 __device__ __forceinline__ float to_float<__half>(__half x) { return __half2float(x); }
 
 // silu(g) * u in fp32 on the ex2 and rcp units, as (g u) / (1 + exp(-g)).  For
-// g in [-40, inf) the relative error is below 2^-18: the argument -g log2(e)
-// carries at most 58 (2^-24 + 2^-25) absolute error, i.e. 3.6e-6 relative in
-// exp, ex2 and rcp about 2^-22 each, and three roundings.  (g u taken first
-// keeps subnormal gates exact where a large up lifts them; where it overflows
-// although the quotient would not, the result is not finite.)
+// g in [-40, inf) the relative error is below 2^-18 = 3.8e-6: the argument
+// t = -g log2(e), below 58, is off by its own rounding (2^-19) and by the
+// constant's (40 x 2e-8), 2.7e-6 together, which is 1.9e-6 relative in 2^t;
+// ex2 adds 2^-22, the sum, rcp and two products about 2^-22 together.  (g u
+// taken first keeps subnormal gates exact where a large up lifts them; where it
+// overflows although the quotient would not, the result is not finite.)
 __device__ __forceinline__ float ex2_approx(float x) {
   float y;
   asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(y) : "f"(x));
