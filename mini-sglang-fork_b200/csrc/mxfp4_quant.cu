@@ -246,8 +246,13 @@ __global__ void __launch_bounds__(kThreads, 5) silu_kernel(const T* __restrict__
 // One CTA per row, thread t holding vectors t + blockDim * j of v = x +
 // residual in fp32.  The sum of squares is taken in fp32 over four values and
 // in 64 bits from there (one conversion and one add per four values), so r is
-// good to fp32 and the exact path can use the same sum.  y = (v r) w in fp32:
-// errors of r (2.5e-7) and of the two products stay below 2^-20.
+// good to fp32 and the exact path can use the same sum.  y = v (r w) in fp32:
+// errors of r (2.5e-7) and of the two products stay below 2^-20.  r w may leave
+// fp32's range.  Above, y is not finite, and its block is taken in 64 bits.
+// Below, it is off by 2^-150, and y by that times |v| <= sqrt(K) rms: less than
+// 2^-45 of the block's first border (m / 32 or more) as long as the block's
+// largest magnitude m is at least 2^-92 rms; a block of less, in a row that is
+// not all zeros, is taken in 64 bits too.
 constexpr float kNormDelta = 9.5367431640625e-7f;  // 2^-20
 constexpr int kNormMaxThreads = 1024;
 
@@ -345,7 +350,9 @@ __global__ void __launch_bounds__(MAX_THREADS)
     ss = block_sum(ss, part, warps);
   }
   const NormRow n = {ss, K, eps};
-  const float r = 1.0f / sqrtf(static_cast<float>(mean));
+  const float root = sqrtf(static_cast<float>(mean));
+  const float r = 1.0f / root;
+  const float limit = ss > 0.0 ? root * 2.0194839173657902e-28f : 0.0f;  // 2^-92 rms
   const float2 r2 = make_float2(r, r);
   uint8_t* sw = scales + scale_word(row, kt, lane);
   uint32_t* qr = reinterpret_cast<uint32_t*>(data + row * (K >> 1));
@@ -357,11 +364,12 @@ __global__ void __launch_bounds__(MAX_THREADS)
     const Vec8 w = unpack8<T>(wa[j]);
     Vec8 y;
 #pragma unroll
-    for (int e = 0; e < 4; ++e) y.p[e] = __fmul2_rn(__fmul2_rn(v[j].p[e], r2), w.p[e]);
+    for (int e = 0; e < 4; ++e) y.p[e] = __fmul2_rn(v[j].p[e], __fmul2_rn(w.p[e], r2));
     uint32_t code;
     int byte;
     // (a lane beyond the row may hold 0 times an infinite r: no value of the block)
-    const bool ok = block_fast(y, quad_max(vi < nvec ? amax8(y) : 0.0f), kNormDelta, code, byte);
+    const float m = quad_max(vi < nvec ? amax8(y) : 0.0f);
+    const bool ok = block_fast(y, m, kNormDelta, code, byte) && m >= limit;
     if (quad_any(far || (!ok && vi < nvec), lane)) {
       const uint2 e = norm_exact<T>(v[j], wa[j], n, lane);
       code = e.x;

@@ -176,6 +176,38 @@ def test_rmsnorm_quant_extremes(pkg, cuda_dev):
         _same(q, *O.quant(y))
 
 
+def test_rmsnorm_quant_tiny_values_under_large_weights(pkg, cuda_dev):
+    """v / rms or weight / rms below fp32's range, lifted back into it by the other
+    factor: 1e-38 / 1e10 times 1e30 is 1e-18, in blocks of their own and next to
+    zeros, and 1e10 / 1e10 times 1e-36 stays what it is."""
+    k = 256
+    g = _gen(11)
+    x = torch.randn(8, k, generator=g)
+    x[:, :64] *= 1e10
+    x[0, 64:] *= 1e-38
+    x[1, 64:] *= 1e-30
+    x[2, 64:] *= 1e-36
+    x[3, 64:] = 0.0
+    x[4, 64:] *= 1e-38
+    x[4, 70:90] = 0.0
+    x[5, 64:] *= 1e-28
+    x[6, :32] = 0.0
+    x[7, 32:64] *= 1e-5
+    x = x.bfloat16().to(cuda_dev)
+    w = (torch.randn(k, generator=g) * 1e30).bfloat16()
+    w[:32] = 1.0
+    w[32:48] = 1e-30
+    w[48:64] = 1e-36
+    w[64:96] = 0.0
+    w[128:160] = 2.0
+    w[224:] = 1e-30
+    w = w.to(cuda_dev)
+    for res in (None, torch.zeros_like(x)):
+        y, _ = O.rmsnorm(x.cpu(), w.cpu(), 1e-6, None if res is None else res.cpu())
+        q, _ = pkg.ops.mxfp4_rmsnorm_quant(x, w, 1e-6, res)
+        _same(q, *O.quant(y))
+
+
 # --------------------------------------------------------------------- product
 @pytest.mark.parametrize("m,n,k", [(1, 128, 64), (1, 16, 32), (16, 128, 256), (1, 1, 32), (5, 130, 96), (16, 384, 1056), (17, 200, 512),
                                    (32, 256, 2080), (33, 512, 768), (64, 1000, 4096), (65, 384, 320), (128, 256, 1024),
