@@ -84,10 +84,22 @@ int mxfp4_gemm(const uint8_t* a_data, const uint8_t* a_scales, const uint8_t* b_
  * (I rows); up (I rows)] MXFP4 [2I, K], bias[2I] (nullable) of type `dtype`;
  * the result is MXFP4 of y = silu(A gate^T + bias) * (A up^T + bias), [M, I],
  * from the fp32 accumulators.  I % 128 == 0 (W8A8_ERR_UNSUPPORTED otherwise:
- * take mxfp4_gemm and mxfp4_silu_mul_quant). */
+ * take mxfp4_gemm_silu_quant_halves). */
 int mxfp4_gemm_silu_quant(const uint8_t* a_data, const uint8_t* a_scales, const uint8_t* b_data,
                           const uint8_t* b_scales, const void* bias, int dtype, uint8_t* y_data,
                           uint8_t* y_scales, int64_t M, int64_t I, int64_t K, void* stream);
+
+/* The scale tiles of [gate; up] ([2I, K], I % 32 == 0) as those of gate [I, K]
+ * and then those of up [I, K], 2 mxfp4_scale_bytes(I, K) bytes in all: where
+ * I % 128 != 0 the up rows start inside a tile, from where the tensor core
+ * cannot read them.  16-byte aligned pointers. */
+int mxfp4_half_scales(const uint8_t* scales, uint8_t* half_scales, int64_t I, int64_t K, void* stream);
+
+/* mxfp4_gemm_silu_quant for any I % 32 == 0, with the scales of B as
+ * mxfp4_half_scales lays them out. */
+int mxfp4_gemm_silu_quant_halves(const uint8_t* a_data, const uint8_t* a_scales, const uint8_t* b_data,
+                                 const uint8_t* b_half_scales, const void* bias, int dtype, uint8_t* y_data,
+                                 uint8_t* y_scales, int64_t M, int64_t I, int64_t K, void* stream);
 
 #ifdef __cplusplus
 }

@@ -95,6 +95,9 @@ MXFP4_SIGNATURES = {
     "mxfp4_rmsnorm_quant": (_c_int, [_c_vp, _c_i64, _c_vp, _c_i64, _c_vp, ctypes.c_float, _c_int, _c_vp, _c_vp,
                                      _c_i64, _c_i64, _c_vp]),
     "mxfp4_gemm": (_c_int, [_c_vp, _c_vp, _c_vp, _c_vp, _c_vp, _c_vp, _c_int, _c_i64, _c_i64, _c_i64, _c_vp]),
+    "mxfp4_half_scales": (_c_int, [_c_vp, _c_vp, _c_i64, _c_i64, _c_vp]),
+    "mxfp4_gemm_silu_quant_halves": (_c_int, [_c_vp, _c_vp, _c_vp, _c_vp, _c_vp, _c_int, _c_vp, _c_vp, _c_i64, _c_i64,
+                                              _c_i64, _c_vp]),
     "mxfp4_gemm_silu_quant": (_c_int, [_c_vp, _c_vp, _c_vp, _c_vp, _c_vp, _c_int, _c_vp, _c_vp, _c_i64, _c_i64,
                                        _c_i64, _c_vp]),
 }

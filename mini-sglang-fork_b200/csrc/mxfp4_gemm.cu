@@ -26,9 +26,43 @@ int allow_smem(int bytes) {
   return W8A8_OK;
 }
 
+// Scale tiles of [gate; up] ([2I, K]) to tiles of each half's own, zero beyond
+// row I.  A thread moves 16 bytes: rows r, r + 32, r + 64, r + 96 of a tile (r <
+// 32).  I is a multiple of 32, so these stay 32 apart, and begin `shift` groups
+// of 32 inside a source tile: they are the last words of that tile's 16 bytes
+// for r and the first of the next one's.
+__global__ void __launch_bounds__(256) half_scales_kernel(const uint4* __restrict__ src, uint4* __restrict__ dst, int64_t I,
+                                                          int64_t ktiles) {
+  dev::griddep_launch();
+  dev::griddep_wait();
+  constexpr int kPieces = kTileBytes / 16;
+  const int64_t i = static_cast<int64_t>(blockIdx.x) * 256 + threadIdx.x;
+  const int64_t rtiles = (I + 127) / 128, tile = i / kPieces;
+  const int64_t rt = tile / ktiles, kt = tile - rt * ktiles;
+  if (rt >= 2 * rtiles) return;
+  const int64_t half = rt >= rtiles, t = rt - half * rtiles;  // of the half's tiles
+  const int64_t row = half * I + t * 128;                     // of the first of its rows in the source
+  const int shift = static_cast<int>(row >> 5) & 3;
+  const int64_t at = ((row >> 7) * ktiles + kt) * kPieces + i % kPieces;
+  const int groups = static_cast<int>(min(static_cast<int64_t>(4), (I - t * 128) >> 5));  // of 32 rows that exist
+  const uint4 a = src[at];
+  const uint4 b = shift + groups > 4 ? src[at + ktiles * kPieces] : make_uint4(0, 0, 0, 0);
+  const uint32_t w[8] = {a.x, a.y, a.z, a.w, b.x, b.y, b.z, b.w};
+  uint32_t o[4];
+#pragma unroll
+  for (int g = 0; g < 4; ++g) {
+    uint32_t x = 0;
+#pragma unroll
+    for (int s = 0; s < 4; ++s) x = shift == s ? w[g + s] : x;
+    o[g] = g < groups ? x : 0u;
+  }
+  dst[i] = make_uint4(o[0], o[1], o[2], o[3]);
+}
+
 struct Operands {
   const uint8_t *a, *as, *b, *bs;
-  int64_t b_rows;  // rows of B: N, or 2I
+  int64_t b_rows;    // rows of B: N, or 2I
+  int64_t bs_tiles;  // row tiles of B's scales: of N rows, or of I rows twice
 };
 
 // Clusters of s CTAs of `Kern` that the device holds at once with one CTA per
@@ -108,7 +142,7 @@ int launch_row(const Operands& o, MxGemmArgs args, cudaStream_t stream) {
   args.ttiles = (args.M + T - 1) / T;
   CUtensorMap tw, tws, tx, txs;
   if (int rc = encode_operand(&tw, o.b, o.b_rows, args.K / 2, 128)) return rc;
-  if (int rc = encode_words(&tws, o.bs, row_tiles(o.b_rows), k_tiles(args.K) * kTileBytes / 4, 256)) return rc;
+  if (int rc = encode_words(&tws, o.bs, o.bs_tiles, k_tiles(args.K) * kTileBytes / 4, 256)) return rc;
   if (int rc = encode_operand(&tx, o.a, args.M, args.K / 2, T)) return rc;
   if (int rc = encode_words(&txs, o.as, row_tiles(args.M), k_tiles(args.K) * kTileBytes / 4, 256)) return rc;
   const int64_t tiles = wtiles * args.ttiles;
@@ -129,7 +163,7 @@ int launch_pair(const Operands& o, const MxGemmArgs& g, cudaStream_t stream) {
   PairArgs args;
   args.g = g;
   args.pairs_m = (g.M + 255) / 256;
-  args.tiles_n = SILU ? g.N / 128 : (g.N + 255) / 256;
+  args.tiles_n = SILU ? (g.N + 127) / 128 : (g.N + 255) / 256;
   const int64_t blocks = static_cast<int64_t>(args.pairs_m) * args.tiles_n;
   // (the block counter runs one grid past the last block)
   W8A8_REQUIRE(blocks <= 0x7fff0000LL, W8A8_ERR_UNSUPPORTED, "mxfp4_gemm: too many output tiles");
@@ -137,7 +171,7 @@ int launch_pair(const Operands& o, const MxGemmArgs& g, cudaStream_t stream) {
   if (int rc = encode_operand(&ta, o.a, g.M, g.K / 2, 128)) return rc;
   if (int rc = encode_words(&tas, o.as, row_tiles(g.M), k_tiles(g.K) * kTileBytes / 4, 256)) return rc;
   if (int rc = encode_operand(&tb, o.b, o.b_rows, g.K / 2, 128)) return rc;
-  if (int rc = encode_words(&tbs, o.bs, row_tiles(o.b_rows), k_tiles(g.K) * kTileBytes / 4, 256)) return rc;
+  if (int rc = encode_words(&tbs, o.bs, o.bs_tiles, k_tiles(g.K) * kTileBytes / 4, 256)) return rc;
   int split = 1;
   if (int rc = pick_split<kern>(blocks, g.kblocks, PairTraits::kThreads, PairTraits::kSmemBytes, 1, 2, 2, 8, &split)) return rc;
   const int64_t pairs = split > 1 ? blocks * split : std::min<int64_t>(blocks, std::max(1, sm_count() / 2));
@@ -174,7 +208,7 @@ int run(const char* what, const Operands& o, const void* bias, void* C, uint8_t*
   W8A8_REQUIRE(dtype == kBf16 || dtype == kFp16, W8A8_ERR_INVALID_ARG, "%s: bf16 or fp16", what);
   W8A8_REQUIRE(M <= (1LL << 27) && N <= (1LL << 27) && K <= (1LL << 27), W8A8_ERR_UNSUPPORTED, "%s: shape too large",
                what);
-  W8A8_REQUIRE(!silu || N % 128 == 0, W8A8_ERR_UNSUPPORTED, "%s: I=%lld must be a multiple of 128", what, (long long)N);
+  W8A8_REQUIRE(!silu || N % kBlock == 0, W8A8_ERR_INVALID_ARG, "%s: I=%lld must be a multiple of 32", what, (long long)N);
   W8A8_REQUIRE(W8A8_ALIGNED16(o.a) && W8A8_ALIGNED16(o.as) && W8A8_ALIGNED16(o.b) && W8A8_ALIGNED16(o.bs) &&
                    W8A8_ALIGNED16(C) && W8A8_ALIGNED16(q) && W8A8_ALIGNED16(qs) &&
                    (reinterpret_cast<uintptr_t>(bias) & 1u) == 0,
@@ -208,15 +242,48 @@ extern "C" {
 
 int mxfp4_gemm(const uint8_t* a_data, const uint8_t* a_scales, const uint8_t* b_data, const uint8_t* b_scales,
                const void* bias, void* C, int dtype, int64_t M, int64_t N, int64_t K, void* stream) {
-  return w8a8::mx::run("mxfp4_gemm", {a_data, a_scales, b_data, b_scales, N}, bias, C, nullptr, nullptr, dtype, M, N,
-                       K, false, static_cast<cudaStream_t>(stream));
+  using namespace w8a8;
+  return mx::run("mxfp4_gemm", {a_data, a_scales, b_data, b_scales, N, mx::row_tiles(N)}, bias, C, nullptr, nullptr,
+                 dtype, M, N, K, false, static_cast<cudaStream_t>(stream));
 }
 
 int mxfp4_gemm_silu_quant(const uint8_t* a_data, const uint8_t* a_scales, const uint8_t* b_data,
                           const uint8_t* b_scales, const void* bias, int dtype, uint8_t* y_data, uint8_t* y_scales,
                           int64_t M, int64_t I, int64_t K, void* stream) {
-  return w8a8::mx::run("mxfp4_gemm_silu_quant", {a_data, a_scales, b_data, b_scales, 2 * I}, bias, nullptr, y_data,
-                       y_scales, dtype, M, I, K, true, static_cast<cudaStream_t>(stream));
+  using namespace w8a8;
+  W8A8_REQUIRE(I <= 0 || I % 128 == 0, W8A8_ERR_UNSUPPORTED,
+               "mxfp4_gemm_silu_quant: I=%lld must be a multiple of 128 (mxfp4_gemm_silu_quant_halves takes the others)",
+               (long long)I);
+  return mx::run("mxfp4_gemm_silu_quant", {a_data, a_scales, b_data, b_scales, 2 * I, 2 * mx::row_tiles(I)}, bias,
+                 nullptr, y_data, y_scales, dtype, M, I, K, true, static_cast<cudaStream_t>(stream));
+}
+
+int mxfp4_gemm_silu_quant_halves(const uint8_t* a_data, const uint8_t* a_scales, const uint8_t* b_data,
+                                 const uint8_t* b_half_scales, const void* bias, int dtype, uint8_t* y_data,
+                                 uint8_t* y_scales, int64_t M, int64_t I, int64_t K, void* stream) {
+  using namespace w8a8;
+  return mx::run("mxfp4_gemm_silu_quant_halves",
+                 {a_data, a_scales, b_data, b_half_scales, 2 * I, 2 * mx::row_tiles(I)}, bias, nullptr, y_data, y_scales,
+                 dtype, M, I, K, true, static_cast<cudaStream_t>(stream));
+}
+
+int mxfp4_half_scales(const uint8_t* scales, uint8_t* half_scales, int64_t I, int64_t K, void* stream) {
+  using namespace w8a8;
+  W8A8_REQUIRE(I >= 0 && K >= 0, W8A8_ERR_INVALID_ARG, "mxfp4_half_scales: negative shape");
+  if (I == 0) return W8A8_OK;
+  W8A8_REQUIRE(I % mx::kBlock == 0 && K > 0 && K % mx::kBlock == 0, W8A8_ERR_INVALID_ARG,
+               "mxfp4_half_scales: I=%lld and K=%lld must be positive multiples of 32", (long long)I, (long long)K);
+  W8A8_REQUIRE(scales && half_scales, W8A8_ERR_INVALID_ARG, "mxfp4_half_scales: null pointer");
+  W8A8_REQUIRE(I <= (1LL << 27) && K <= (1LL << 27), W8A8_ERR_UNSUPPORTED, "mxfp4_half_scales: shape too large");
+  W8A8_REQUIRE(W8A8_ALIGNED16(scales) && W8A8_ALIGNED16(half_scales), W8A8_ERR_ALIGNMENT,
+               "mxfp4_half_scales: pointers must be 16-byte aligned");
+  const int64_t pieces = 2 * mx::row_tiles(I) * mx::k_tiles(K) * (mx::kTileBytes / 16);
+  const int64_t ctas = (pieces + 255) / 256;
+  W8A8_REQUIRE(ctas < (1LL << 31), W8A8_ERR_UNSUPPORTED, "mxfp4_half_scales: shape too large");
+  W8A8_CUDA_TRY(launch_pdl(mx::half_scales_kernel, dim3(static_cast<unsigned>(ctas)), dim3(256), 0,
+                           static_cast<cudaStream_t>(stream), reinterpret_cast<const uint4*>(scales),
+                           reinterpret_cast<uint4*>(half_scales), I, mx::k_tiles(K)));
+  return W8A8_OK;
 }
 
 }  // extern "C"

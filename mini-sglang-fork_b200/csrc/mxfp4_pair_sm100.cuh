@@ -211,8 +211,8 @@ __global__ void __launch_bounds__(PairTraits::kThreads, 1)
       const int ta = 2 * pm + static_cast<int>(half);  // 128-row tile of A
       // 128-row tiles of B: the block's two, or its gate rows and their up rows
       const int tb0 = SILU ? tn : 2 * tn;
-      const int tb1 = SILU ? tn + (g.N >> 7) : 2 * tn + 1;
-      const int b_row = (half ? tb1 : tb0) * 128;
+      const int tb1 = SILU ? tn + ((g.N + 127) >> 7) : 2 * tn + 1;
+      const int b_row = half == 0 ? tb0 * 128 : SILU ? tn * 128 + g.N : tb1 * 128;
       for (int kb = kb0; kb < kb1; ++kb) {
         ok = warp_wait(dev::smem_u32(empty + stage), phase ^ 1u, abort_flag, g.err, tmo);
         if (!ok) break;
@@ -320,8 +320,8 @@ __global__ void __launch_bounds__(PairTraits::kThreads, 1)
       if (g.bias) {
         const int et = threadIdx.x - 64;
         const O* b = static_cast<const O*>(g.bias);
-        const int c = SILU ? tn * 128 + (et & 127) + (et >> 7) * g.N : tn * 256 + et;
-        bias[et] = SILU || c < g.N ? to_float(b[c]) : 0.0f;
+        const int c = SILU ? tn * 128 + (et & 127) : tn * 256 + et;
+        bias[et] = c < g.N ? to_float(b[SILU ? c + (et >> 7) * g.N : c]) : 0.0f;
       }
       const bool ok = warp_wait(dev::smem_u32(acc_full + acc), (blk >> 1) & 1u, abort_flag, g.err, tmo);
       if (g.bias ? dev::named_bar_or(1, 32 * P::kEpiWarps, !ok) : !ok) break;  // (publishes the biases)

@@ -84,7 +84,8 @@ struct MxGemmArgs {
   uint8_t* qs;       // SiLU: scale tiles of [M, I]
   unsigned int* err;
   long long timeout_ns;
-  int M, N, K;       // N: output columns (I with the SiLU epilogue)
+  int M, N, K;       // N: output columns (I with the SiLU epilogue: B has N gate
+                     // rows and N up rows, each half with scale tiles of its own)
   int kblocks;       // 256-value k blocks
   int ttiles, tiles;  // weight-stationary kernel: token tiles, output tiles
 };
@@ -181,12 +182,13 @@ __device__ __forceinline__ void silu_block(const MxGemmArgs& g, const float* bia
   uint32_t w[4];
 #pragma unroll
   for (int e = 0; e < 4; ++e) w[e] = byte == kNanScale ? 0u : pack8_scaled(y[e], f);
-  if (row < g.M) {
+  if (row < g.M && f0 < g.N) {
     const int64_t kt = k_tiles(g.N);
     *reinterpret_cast<uint4*>(g.q + row * (g.N >> 1) + (f0 >> 1)) = make_uint4(w[0], w[1], w[2], w[3]);
-    uint8_t* s = g.qs + scale_offset(row, ft, kt) + j;
-    *s = static_cast<uint8_t>(byte);
-    if ((ft + 1) * 128 == g.N && ft + 1 < kt) s[kTileBytes] = 0;  // the padding tile
+    uint8_t* s = g.qs + scale_offset(row, ft, kt);
+    s[j] = static_cast<uint8_t>(byte);
+    if (f0 + 32 == g.N)  // the last block also writes the padding to 256 features
+      for (int b = f0 / 32 + 1; b & 7; ++b) s[(b / 4 - ft) * kTileBytes + (b & 3)] = 0;
   }
 }
 
@@ -235,9 +237,9 @@ struct MxRowTraits {
   static_assert(kSmemBytes <= 227 * 1024, "shared memory");
   static constexpr int kPerSm = 228 * 1024 / (kSmemBytes + 1024);  // CTAs on an SM
   // At most three CTAs with at most 128 TMEM columns each share an SM, and one
-  // with more leaves no room for another.  So every allocation succeeds at
-  // once, and no CTA of a cluster waits for TMEM that a CTA waiting for it
-  // holds.
+  // with more leaves no room for another (nor does an int8 GEMM, whose ring
+  // alone is 180 KB or more).  So every allocation succeeds at once, and no CTA
+  // of a cluster waits for TMEM that a CTA waiting for it holds.
   static_assert(kTmemCols <= 128 ? kSmemBytes >= 60 * 1024 : kSmemBytes >= 170 * 1024, "TMEM share");
   // The ring holds a CTA's own shares for its peers and theirs for it.
   static_assert(!DEEP || 2 * kTiles * (T + 8) * 512 <= kStages * kStageBytes, "the shares reuse the ring");
@@ -285,6 +287,7 @@ __global__ void __launch_bounds__(kRowThreads, 1) mx_row_kernel(const __grid_con
   const int rank = static_cast<int>(dev::cluster_rank());
   const int first = blockIdx.x / S;
   const int step = gridDim.x / S;  // (S > 1: one tile per cluster)
+  const int wtiles = (args.N + 127) >> 7;
   const int kb0 = static_cast<int>(static_cast<int64_t>(rank) * args.kblocks / S);
   const int kb1 = static_cast<int>(static_cast<int64_t>(rank + 1) * args.kblocks / S);
   const long long tmo = args.timeout_ns;
@@ -319,9 +322,9 @@ __global__ void __launch_bounds__(kRowThreads, 1) mx_row_kernel(const __grid_con
       for (int kb = kb0; kb < min(kb1, kb0 + 5); ++kb)
 #pragma unroll
         for (int h = 0; h < P::kTiles; ++h) {
-          const int w0 = first / args.ttiles * 128 + h * args.N;
-          tma_prefetch_2d(&tm_w, kb * 128, w0);
-          tma_prefetch_2d(&tm_ws, kb * 256, w0 >> 7);
+          const int wt = first / args.ttiles;
+          tma_prefetch_2d(&tm_w, kb * 128, wt * 128 + h * args.N);
+          tma_prefetch_2d(&tm_ws, kb * 256, wt + h * wtiles);
         }
     }
     __syncwarp();
@@ -347,9 +350,11 @@ __global__ void __launch_bounds__(kRowThreads, 1) mx_row_kernel(const __grid_con
           dev::mbar_expect_tx(bar, P::kStageBytes);
 #pragma unroll
           for (int h = 0; h < P::kTiles; ++h) {
-            const int w0 = wt * 128 + h * args.N;  // gate rows, then up rows
-            dev::tma_load_2d(dev::smem_u32(s_w + (stage * P::kTiles + h) * P::kW), &tm_w, bar, kb * 128, w0);
-            dev::tma_load_2d(dev::smem_u32(s_ws + (stage * P::kTiles + h) * P::kSf), &tm_ws, bar, kb * 256, w0 >> 7);
+            // gate rows, then up rows
+            dev::tma_load_2d(dev::smem_u32(s_w + (stage * P::kTiles + h) * P::kW), &tm_w, bar, kb * 128,
+                             wt * 128 + h * args.N);
+            dev::tma_load_2d(dev::smem_u32(s_ws + (stage * P::kTiles + h) * P::kSf), &tm_ws, bar, kb * 256,
+                             wt + h * wtiles);
           }
           dev::tma_load_2d(dev::smem_u32(s_x + stage * P::kX), &tm_x, bar, kb * 128, tt * T);
           dev::tma_load_2d(dev::smem_u32(s_xs + stage * P::kSf), &tm_xs, bar, kb * 256, (tt * T) >> 7);
@@ -441,8 +446,8 @@ __global__ void __launch_bounds__(kRowThreads, 1) mx_row_kernel(const __grid_con
       if (args.bias) {
         const O* b = static_cast<const O*>(args.bias);
         if constexpr (SILU) {
-          bias[n] = to_float(b[col]);
-          bias[128 + n] = to_float(b[args.N + col]);
+          bias[n] = col < args.N ? to_float(b[col]) : 0.0f;
+          bias[128 + n] = col < args.N ? to_float(b[args.N + col]) : 0.0f;
         } else if (col < args.N) {
           bias_n = to_float(b[col]);
         }

@@ -90,8 +90,7 @@ class LinearColParallelMerged(_LinearTPImpl):
         super().__init__(input_size, sum(output_sizes), input_size, sum(tp_output_sizes), has_bias, dtype)
 
     def forward_silu_quant(self, x: Activation) -> MXFP4Tensor:
-        """For a [gate; up] merge: MXFP4 ``silu(gate) * up``, in one kernel
-        where the local intermediate size is a multiple of 128
+        """For a [gate; up] merge: MXFP4 ``silu(gate) * up``
         (:func:`ops.mxfp4_gate_up_silu_quant`)."""
         return ops.mxfp4_gate_up_silu_quant(self._quantize_input(x), self._weight(), self.bias, self._dtype)
 

@@ -501,7 +501,8 @@ class MXFP4Tensor:
     """A microscaled 4-bit matrix ``[R, K]``: ``data [R, K/2]`` uint8 (two
     E2M1 codes per byte, even column low) and ``scales``, the E8M0 bytes of its
     32-value blocks in tiles of :func:`mxfp4_scale_shape` (row r, block c of a
-    tile at ``(r % 32) * 16 + (r // 32) * 4 + c``).  The product of
+    tile at ``(r % 32) * 16 + (r // 32) * 4 + c``; the bytes of blocks beyond K
+    are zero, those of rows beyond R are not used).  The product of
     :func:`mxfp4_quant` and its fused forms, an operand of :func:`mxfp4_gemm`,
     and accepted by the MXFP4 layers in place of a 16-bit activation."""
 
@@ -724,22 +725,26 @@ def mxfp4_gemm(a: MXFP4Tensor, w: MXFP4Tensor, bias: Optional[torch.Tensor] = No
 def mxfp4_gate_up_silu_quant(a: MXFP4Tensor, w: MXFP4Tensor, bias: Optional[torch.Tensor] = None,
                              dtype: torch.dtype = torch.bfloat16) -> MXFP4Tensor:
     """The gated half of an MLP in MXFP4: ``w [2I, K]`` is the merged [gate;
-    up] weight, the result MXFP4 ``silu(a gate^T) * (a up^T)``, ``[M, I]``.
-    With I % 128 == 0 one kernel forms it from the fp32 sums and nothing of the
-    [M, 2I] product reaches memory; otherwise :func:`mxfp4_gemm` (rounding to
-    ``dtype``) and :func:`mxfp4_silu_and_mul_quant` run.  ``dtype`` is also the
-    bias's type.  I % 32 == 0."""
+    up] weight, the result MXFP4 ``silu(a gate^T) * (a up^T)``, ``[M, I]``,
+    formed from the fp32 sums; nothing of the [M, 2I] product reaches memory.
+    ``dtype`` is the bias's type.  I % 32 == 0; where I % 128 != 0 a first, small
+    kernel lays the halves' scale tiles out apart."""
     code = _check_mx_gemm("mxfp4_gate_up_silu_quant", a, w, bias, dtype)
     m, k = a.shape
     i, odd = divmod(w.shape[0], 2)
     if odd or i % 32:
         raise _lib.W8A8Error(_lib.ERR_INVALID_ARG,
                              f"mxfp4_gate_up_silu_quant: {w.shape[0]} weight rows are not [gate; up] of a multiple of 32")
-    if i % 128:
-        return mxfp4_silu_and_mul_quant(mxfp4_gemm(a, w, bias, out_dtype=dtype))
     y = MXFP4Tensor._empty(m, i, a._buf)
-    _mx_call("mxfp4_gate_up_silu_quant", _lib.load().mxfp4_gemm_silu_quant, a._buf, *a._ptrs(), *w._ptrs(), _ptr(bias),
-             code, *y._ptrs(), m, i, k)
+    lib, (data, scales) = _lib.load(), w._ptrs()
+    if i % 128 == 0:
+        fn = lib.mxfp4_gemm_silu_quant
+    else:
+        fn = lib.mxfp4_gemm_silu_quant_halves
+        halves = a._buf.new_empty(2 * lib.mxfp4_scale_bytes(i, k), dtype=torch.uint8)
+        _mx_call("mxfp4_gate_up_silu_quant", lib.mxfp4_half_scales, a._buf, scales, halves.data_ptr(), i, k)
+        scales = halves.data_ptr()
+    _mx_call("mxfp4_gate_up_silu_quant", fn, a._buf, *a._ptrs(), data, scales, _ptr(bias), code, *y._ptrs(), m, i, k)
     return y
 
 

@@ -56,6 +56,16 @@ def test_host_validation(pkg):
     assert lib.mxfp4_gemm_silu_quant(16, 16, 16, 16, None, 0, 16, 16, 4, 96, 64, None) == L.ERR_UNSUPPORTED
     assert lib.mxfp4_gemm_silu_quant(16, 16, 16, 16, None, 0, None, 16, 4, 128, 64, None) == L.ERR_INVALID_ARG
     assert lib.mxfp4_gemm_silu_quant(None, None, None, None, None, 0, None, None, 0, 128, 64, None) == L.OK
+    assert lib.mxfp4_gemm_silu_quant_halves(16, 16, 16, 16, None, 0, 16, 16, 4, 80, 64, None) == L.ERR_INVALID_ARG
+    assert lib.mxfp4_gemm_silu_quant_halves(16, 16, 16, None, None, 0, 16, 16, 4, 96, 64, None) == L.ERR_INVALID_ARG
+    assert lib.mxfp4_gemm_silu_quant_halves(None, None, None, None, None, 0, None, None, 0, 96, 64, None) == L.OK
+    # (scales, half scales, I, K)
+    assert lib.mxfp4_half_scales(16, 16, 80, 64, None) == L.ERR_INVALID_ARG and b"multiples of 32" in msg()
+    assert lib.mxfp4_half_scales(16, 16, 96, 40, None) == L.ERR_INVALID_ARG
+    assert lib.mxfp4_half_scales(None, 16, 96, 64, None) == L.ERR_INVALID_ARG and b"null" in msg()
+    assert lib.mxfp4_half_scales(16, 24, 96, 64, None) == L.ERR_ALIGNMENT
+    assert lib.mxfp4_half_scales(16, 16, 1 << 28, 64, None) == L.ERR_UNSUPPORTED
+    assert lib.mxfp4_half_scales(None, None, 0, 64, None) == L.OK
     assert lib.mxfp4_scale_bytes(129, 288) == 2 * 4 * 512 and lib.mxfp4_scale_bytes(4, 40) == 0
 
 

@@ -281,6 +281,10 @@ def _silu_gemm_check(y, gv, uv, slack):
                                    (2000, 640, 544), (129, 4992, 96), (3000, 2048, 256)])
 @pytest.mark.parametrize("dtype", TYPES)
 def test_gate_up_silu_quant(pkg, cuda_dev, m, i, k, dtype):
+    _gate_up_check(pkg, cuda_dev, m, i, k, dtype)
+
+
+def _gate_up_check(pkg, cuda_dev, m, i, k, dtype):
     """The fused epilogue on operands whose sums are exact in fp32 (block
     scales within a few powers of two, K small: every product is a multiple of
     2^-2 of the smallest scale product and the sums stay below 2^22 of those),
@@ -299,10 +303,14 @@ def test_gate_up_silu_quant(pkg, cuda_dev, m, i, k, dtype):
 
 
 @pytest.mark.parametrize("m,i,k", [(3, 32, 64), (40, 160, 512), (300, 96, 256)])
-def test_gate_up_silu_quant_two_steps(pkg, cuda_dev, m, i, k):
-    """I % 128 != 0: the product and the SiLU quantiser, one after the other."""
-    a, _ = _operand(pkg, m, k, 1.0, m, cuda_dev)
-    w, _ = _operand(pkg, 2 * i, k, 0.05, i, cuda_dev)
-    y = pkg.ops.mxfp4_gate_up_silu_quant(a, w)
-    gu = pkg.ops.mxfp4_gemm(a, w).cpu()
-    _same(y, *O.quant(O.silu_mul(gu[:, :i], gu[:, i:])))
+def test_gate_up_silu_quant_ragged(pkg, cuda_dev, m, i, k):
+    """I % 128 != 0: the up rows start inside a scale tile and the last tile is
+    not full; held to the definition as the full tiles are."""
+    _gate_up_check(pkg, cuda_dev, m, i, k, torch.bfloat16)
+
+
+@pytest.mark.parametrize("m,i,k", [(1, 32, 32), (1, 4896, 512), (16, 224, 1056), (33, 288, 4096), (64, 5216, 288),
+                                   (65, 32, 64), (130, 416, 768), (257, 1312, 320), (1000, 10912, 256)])
+@pytest.mark.parametrize("dtype", TYPES)
+def test_gate_up_silu_quant_ragged_sizes(pkg, cuda_dev, m, i, k, dtype):
+    _gate_up_check(pkg, cuda_dev, m, i, k, dtype)
