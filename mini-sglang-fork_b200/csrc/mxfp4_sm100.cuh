@@ -55,12 +55,10 @@ __device__ __forceinline__ void mma_mxf4(uint32_t d_tmem, uint64_t adesc, uint64
 }
 
 // One lane of a converged warp.  The producer and MMA roles run their loops
-// with the whole warp and issue under this predicate: the compiler then knows
-// that one lane is active and passes the operands of TMA and tcgen05 (which
-// the hardware takes from uniform registers) directly.  Under a predicate on
-// the lane index it emits a loop over the lanes' values around every such
-// instruction; a k block of four MMAs and six scale copies then took 606 ns to
-// issue, with this 280 ns, which is the MMAs' own time.
+// with the whole warp and issue under this predicate, from which the compiler
+// knows that one lane is active.  Under a predicate on the lane index, which
+// leaves that open, a k block of four MMAs and six scale copies took 606 ns to
+// issue; with this 280 ns, which is the MMAs' own time.
 __device__ __forceinline__ bool elect_one() {
   uint32_t p;
   asm volatile(
