@@ -244,17 +244,18 @@ __global__ void __launch_bounds__(kThreads, 5) silu_kernel(const T* __restrict__
 
 // ----------------------------------------------------------------- RMSNorm
 // One CTA per row, thread t holding vectors t + blockDim * j of v = x +
-// residual in fp32.  The sum of squares is taken in fp32 over four values and
-// in 64 bits from there (one conversion and one add per four values), so r is
-// good to fp32 and the exact path can use the same sum.  y = v (r w) in fp32:
-// errors of r (2.5e-7) and of the two products stay below 2^-20.  r w may leave
+// residual in fp32.  The sum of squares is taken in 64 bits, where a square is
+// exact: blocks next to a border need it so (with fp32 sums of four squares one
+// value in 3 10^8 got the neighbouring code), and it takes no time, as the
+// 64-bit unit and the conversions run beside the rest (4097 x 5120: 29.4 us,
+// 29.3 with the fp32 sums).  y = v (r w) in fp32: errors of r (2.5e-7) and of
+// the two products stay below 2^-20.  r w may leave
 // fp32's range.  Above, y is not finite, and its block is taken in 64 bits.
 // Below, it is off by 2^-150, and y by that times |v| <= sqrt(K) rms: less than
 // 2^-45 of the block's first border (m / 32 or more) as long as the block's
 // largest magnitude m is at least 2^-92 rms; a block of less, in a row that is
 // not all zeros, is taken in 64 bits too.
 constexpr float kNormDelta = 9.5367431640625e-7f;  // 2^-20
-constexpr int kNormMaxThreads = 1024;
 
 struct NormRow {
   double ss;  // sum of v^2 over the row
@@ -327,28 +328,19 @@ __global__ void __launch_bounds__(MAX_THREADS)
       }
     }
   }
-  double ss = 0.0;
+  double s0 = 0.0, s1 = 0.0;  // two chains
 #pragma unroll
-  for (int j = 0; j < VPT; ++j) {
+  for (int j = 0; j < VPT; ++j)
 #pragma unroll
-    for (int e = 0; e < 4; e += 2) {
-      const float2 q = __ffma2_rn(v[j].p[e + 1], v[j].p[e + 1], __fmul2_rn(v[j].p[e], v[j].p[e]));
-      ss += q.x + q.y;
+    for (int e = 0; e < 4; ++e) {
+      const double a = v[j].p[e].x, b = v[j].p[e].y;
+      s0 = fma(a, a, s0);
+      s1 = fma(b, b, s1);
     }
-  }
-  ss = block_sum(ss, part, warps);
+  const double ss = block_sum(s0 + s1, part, warps);
   const double mean = ss * (1.0 / K) + static_cast<double>(eps);
-  // A row whose mean square nears the ends of fp32's range, where squares
-  // overflow or lose digits, is summed again and finished in 64 bits.
+  // rows whose mean square is beyond the fp32 form: all in 64 bits
   const bool far = !(mean > 1e-25 && mean < 1e25);
-  if (far) {
-    ss = 0.0;
-    for (int j = 0; j < VPT; ++j)
-      for (int e = 0; e < 4; ++e)
-        ss += static_cast<double>(v[j].p[e].x) * v[j].p[e].x + static_cast<double>(v[j].p[e].y) * v[j].p[e].y;
-    __syncthreads();  // `part` has been read
-    ss = block_sum(ss, part, warps);
-  }
   const NormRow n = {ss, K, eps};
   const float root = sqrtf(static_cast<float>(mean));
   const float r = 1.0f / root;

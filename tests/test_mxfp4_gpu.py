@@ -176,6 +176,25 @@ def test_rmsnorm_quant_extremes(pkg, cuda_dev):
         _same(q, *O.quant(y))
 
 
+@pytest.mark.parametrize("seed,row", [(463, 57), (688, 14), (1247, 29), (3629, 59)])
+@pytest.mark.parametrize("whole", [False, True])
+def test_rmsnorm_quant_next_to_a_border(pkg, cuda_dev, seed, row, whole):
+    """Rows in which a value is so close to a rounding border that a sum of
+    squares with fp32 additions in it gives the neighbouring code; alone and
+    among others."""
+    g = _gen(seed)
+    x = torch.randn(64, 2048, generator=g).bfloat16()
+    r = torch.randn(64, 2048, generator=g).bfloat16()
+    w = (1 + 0.3 * torch.randn(2048, generator=g)).bfloat16()
+    if whole:
+        x, r = x.repeat(8, 1), r.repeat(8, 1)
+    else:
+        x, r = x[row:row + 1].contiguous(), r[row:row + 1].contiguous()
+    y, _ = O.rmsnorm(x, w, 1e-6, r)
+    q, _ = pkg.ops.mxfp4_rmsnorm_quant(x.to(cuda_dev), w.to(cuda_dev), 1e-6, r.to(cuda_dev))
+    _same(q, *O.quant(y))
+
+
 def test_rmsnorm_quant_tiny_values_under_large_weights(pkg, cuda_dev):
     """v / rms or weight / rms below fp32's range, lifted back into it by the other
     factor: 1e-38 / 1e10 times 1e30 is 1e-18, in blocks of their own and next to

@@ -174,6 +174,42 @@ def test_decoder_layer_captured(pkg, cuda_dev):
                 assert torch.equal(u, v)
 
 
+@pytest.mark.parametrize("m", [5, 40, 300])
+def test_ragged_gated_mlp_captured(pkg, cuda_dev, m):
+    """An intermediate size that is no multiple of 128: two captured graphs of
+    one layer follow weights that are changed in place between replays, and give
+    what eager calls give, bit for bit."""
+    layer = _load(pkg, pkg.mxfp4.GatedMLP(512, 416), cuda_dev, 1)
+    other = _load(pkg, pkg.mxfp4.GatedMLP(512, 416), cuda_dev, 2)
+    xs = [torch.randn(m, 512, generator=_gen(s)).bfloat16().to(cuda_dev) for s in range(3)]
+    want = [[n.forward(x).clone() for x in xs] for n in (layer, other)]
+    assert not torch.equal(want[0][0], want[1][0])
+    graphs = []
+    for _ in range(2):
+        x, stream = xs[0].clone(), torch.cuda.Stream()
+        torch.cuda.synchronize()
+        g = torch.cuda.CUDAGraph()
+        with torch.cuda.graph(g, stream=stream):
+            out = layer.forward(x)
+        graphs.append((g, stream, x, out))
+    for n, expected in enumerate(want):
+        if n == 1:
+            torch.cuda.synchronize()
+            for mine, theirs in ((layer.gate_up_proj, other.gate_up_proj), (layer.down_proj, other.down_proj)):
+                mine.weight.copy_(theirs.weight)
+                mine.weight_scale.copy_(theirs.weight_scale)
+            torch.cuda.synchronize()
+        for s in range(3):
+            for j, (g, stream, x, out) in enumerate(graphs):
+                with torch.cuda.stream(stream):
+                    x.copy_(xs[(s + j) % 3])
+                    g.replay()
+            torch.cuda.synchronize()
+            for j, (g, stream, x, out) in enumerate(graphs):
+                assert torch.equal(out, expected[(s + j) % 3])
+
+
+
 def test_streams_at_once(pkg, cuda_dev):
     """The same weights used from four streams at once, operands made on the
     stream that uses them."""
