@@ -247,14 +247,14 @@ __global__ void __launch_bounds__(kThreads, 5) silu_kernel(const T* __restrict__
 // residual in fp32.  The sum of squares is taken in 64 bits, where a square is
 // exact: blocks next to a border need it so (with fp32 sums of four squares one
 // value in 3 10^8 got the neighbouring code), and it takes no time, as the
-// 64-bit unit and the conversions run beside the rest (4097 x 5120: 29.4 us,
-// 29.3 with the fp32 sums).  y = v (r w) in fp32: errors of r (2.5e-7) and of
-// the two products stay below 2^-20.  r w may leave
-// fp32's range.  Above, y is not finite, and its block is taken in 64 bits.
-// Below, it is off by 2^-150, and y by that times |v| <= sqrt(K) rms: less than
-// 2^-45 of the block's first border (m / 32 or more) as long as the block's
-// largest magnitude m is at least 2^-92 rms; a block of less, in a row that is
-// not all zeros, is taken in 64 bits too.
+// 64-bit unit and the conversions run beside the rest (4097 x 5120, when
+// changed: 29.4 us, 29.3 with the fp32 sums).  y = v (r w) in fp32: errors of r
+// (2.5e-7) and of the two products stay below 2^-20.  r w may leave fp32's
+// range.  Above, y is not finite, and its block is taken in 64 bits.  Below, it
+// is off by 2^-150, and y by that times |v| <= sqrt(K) rms: less than 2^-45 of
+// the block's first border (m / 32 or more) as long as the block's largest
+// magnitude m is at least 2^-92 rms; a block of less, in a row that is not all
+// zeros, is taken in 64 bits too.
 constexpr float kNormDelta = 9.5367431640625e-7f;  // 2^-20
 
 struct NormRow {
@@ -283,8 +283,8 @@ __device__ __forceinline__ double block_sum(double x, double* part, int warps) {
   return x;
 }
 
-template <typename T, int VPT, int MAX_THREADS, bool ADD>
-__global__ void __launch_bounds__(MAX_THREADS)
+template <typename T, int VPT, int MAX_THREADS, int MIN_CTAS, bool ADD>
+__global__ void __launch_bounds__(MAX_THREADS, MIN_CTAS)
     rmsnorm_kernel(const T* x, int64_t ldx, T* residual, int64_t ldr, const T* __restrict__ weight,
                    float eps, uint8_t* __restrict__ data, uint8_t* __restrict__ scales, int K) {
   __shared__ double part[MAX_THREADS / 32];
@@ -488,22 +488,26 @@ int run_silu(const void* gu, int64_t ld, uint8_t* data, uint8_t* scales, int64_t
 // Threads and vectors per thread of a row: with few rows one vector per thread
 // (the shortest chain), with many four, so that a CTA is small and an SM holds
 // rows at different stages (4097 x 5120, when chosen: 32.8 us; with two 34.8,
-// with one 69.6; 29.3 now).
+// with one 69.6).  The kernel asks for 98 registers; held to 80 and 64, so that
+// 768 to 1024 threads fit an SM, some are spilled but more rows are under way
+// (4097 x 5120: 28.1 us, 29.4 unbound; 4096 x 8192: 43.4, 52.4; 2048 x 16384:
+// 47.8, 59.7).
 template <typename T, bool ADD>
 int run_norm(const void* x, int64_t ldx, void* residual, int64_t ldr, const void* weight, float eps, uint8_t* data,
              uint8_t* scales, int64_t M, int64_t K, cudaStream_t s) {
   const int nvec = static_cast<int>(K / 8);
   const int vpt = M >= 2 * sm_count() || nvec > 2048 ? 4 : nvec > 1024 ? 2 : 1;
   const int threads = ((nvec + vpt - 1) / vpt + 31) / 32 * 32;
-#define MXFP4_NORM(V, THREADS)                                                                                      \
-  W8A8_CUDA_TRY(launch_pdl(rmsnorm_kernel<T, V, THREADS, ADD>, dim3(static_cast<unsigned>(M)), dim3(threads), 0, s, \
-                           static_cast<const T*>(x), ldx, static_cast<T*>(residual), ldr,                           \
+#define MXFP4_NORM(V, THREADS, CTAS)                                                                              \
+  W8A8_CUDA_TRY(launch_pdl(rmsnorm_kernel<T, V, THREADS, CTAS, ADD>, dim3(static_cast<unsigned>(M)), dim3(threads), \
+                           0, s, static_cast<const T*>(x), ldx, static_cast<T*>(residual), ldr,                   \
                            static_cast<const T*>(weight), eps, data, scales, static_cast<int>(K)))
-  if (vpt == 1) MXFP4_NORM(1, 1024);
-  else if (vpt == 2) MXFP4_NORM(2, 1024);
-  else if (threads <= 256) MXFP4_NORM(4, 256);
-  else if (threads <= 512) MXFP4_NORM(4, 512);
-  else MXFP4_NORM(4, 1024);
+  if (vpt == 1) MXFP4_NORM(1, 1024, 1);
+  else if (vpt == 2) MXFP4_NORM(2, 1024, 1);
+  else if (threads <= 160) MXFP4_NORM(4, 160, 5);
+  else if (threads <= 256) MXFP4_NORM(4, 256, 3);
+  else if (threads <= 512) MXFP4_NORM(4, 512, 2);
+  else MXFP4_NORM(4, 1024, 1);
 #undef MXFP4_NORM
   return W8A8_OK;
 }
