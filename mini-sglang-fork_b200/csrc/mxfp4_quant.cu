@@ -339,12 +339,15 @@ __global__ void __launch_bounds__(MAX_THREADS, MIN_CTAS)
     }
   const double ss = block_sum(s0 + s1, part, warps);
   const double mean = ss * (1.0 / K) + static_cast<double>(eps);
+  // A row with an infinity or a NaN needs no second look: r is 0 or NaN, and y
+  // zero or NaN as it is by the definition.
+  const bool finite = ss < __longlong_as_double(0x7ff0000000000000LL);
   // rows whose mean square is beyond the fp32 form: all in 64 bits
-  const bool far = !(mean > 1e-25 && mean < 1e25);
+  const bool far = finite && !(mean > 1e-25 && mean < 1e25);
   const NormRow n = {ss, K, eps};
   const float root = sqrtf(static_cast<float>(mean));
   const float r = 1.0f / root;
-  const float limit = ss > 0.0 ? root * 2.0194839173657902e-28f : 0.0f;  // 2^-92 rms
+  const float limit = finite && ss > 0.0 ? root * 2.0194839173657902e-28f : 0.0f;  // 2^-92 rms
   const float2 r2 = make_float2(r, r);
   uint8_t* sw = scales + scale_word(row, kt, lane);
   uint32_t* qr = reinterpret_cast<uint32_t*>(data + row * (K >> 1));
@@ -361,7 +364,11 @@ __global__ void __launch_bounds__(MAX_THREADS, MIN_CTAS)
     int byte;
     // (a lane beyond the row may hold 0 times an infinite r: no value of the block)
     const float m = quad_max(vi < nvec ? amax8(y) : 0.0f);
-    const bool ok = block_fast(y, m, kNormDelta, code, byte) && m >= limit;
+    bool ok = block_fast(y, m, kNormDelta, code, byte) && m >= limit;
+    if (!finite) {
+      ok = true;
+      if (byte == kNanScale) code = 0;
+    }
     if (quad_any(far || (!ok && vi < nvec), lane)) {
       const uint2 e = norm_exact<T>(v[j], wa[j], n, lane);
       code = e.x;

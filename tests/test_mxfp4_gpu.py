@@ -176,6 +176,29 @@ def test_rmsnorm_quant_extremes(pkg, cuda_dev):
         _same(q, *O.quant(y))
 
 
+@pytest.mark.parametrize("dtype", TYPES)
+@pytest.mark.parametrize("m,k", [(8, 1056), (600, 5120)])
+def test_rmsnorm_quant_rows_that_are_not_finite(pkg, cuda_dev, m, k, dtype):
+    """Infinities and NaN in some rows' input, residual and weight: zeros and NaN
+    blocks in those rows, and no other row is touched."""
+    g = _gen(m + k)
+    x, r = (torch.randn(m, k, generator=g).to(dtype) for _ in range(2))
+    x[1, 40] = float("inf")
+    x[2, 700] = float("-inf")
+    r[2, 3] = float("inf")
+    x[3, 5] = float("nan")
+    x[4, 100], r[4, 100] = float("inf"), float("-inf")
+    x[5, 64:96] = float("inf")
+    for special in (None, float("inf"), float("nan"), 0.0):
+        w = (1 + 0.1 * torch.randn(k, generator=_gen(k))).to(dtype)
+        if special is not None:
+            w[300] = special
+        y, want = O.rmsnorm(x, w, 1e-6, r)
+        q, out = pkg.ops.mxfp4_rmsnorm_quant(x.to(cuda_dev), w.to(cuda_dev), 1e-6, r.to(cuda_dev))
+        _same(q, *O.quant(y))
+        assert torch.equal(out.cpu().nan_to_num(nan=123.0), want.nan_to_num(nan=123.0))
+
+
 @pytest.mark.parametrize("seed,row", [(463, 57), (688, 14), (1247, 29), (3629, 59)])
 @pytest.mark.parametrize("whole", [False, True])
 def test_rmsnorm_quant_next_to_a_border(pkg, cuda_dev, seed, row, whole):
