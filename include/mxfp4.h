@@ -83,7 +83,9 @@ int mxfp4_gemm(const uint8_t* a_data, const uint8_t* a_scales, const uint8_t* b_
 /* gate_up GEMM with SiLU*mul and requantisation in its epilogue: B = [gate
  * (I rows); up (I rows)] MXFP4 [2I, K], bias[2I] (nullable) of type `dtype`;
  * the result is MXFP4 of y = silu(A gate^T + bias) * (A up^T + bias), [M, I],
- * from the fp32 accumulators.  I % 128 == 0 (W8A8_ERR_UNSUPPORTED otherwise:
+ * from the fp32 accumulators (the bias added in fp32), y not rounded before it
+ * is quantised: values next to a rounding border are evaluated more closely,
+ * up to 64 bits, as in mxfp4_silu_mul_quant.  I % 128 == 0 (W8A8_ERR_UNSUPPORTED otherwise:
  * take mxfp4_gemm_silu_quant_halves). */
 int mxfp4_gemm_silu_quant(const uint8_t* a_data, const uint8_t* a_scales, const uint8_t* b_data,
                           const uint8_t* b_scales, const void* bias, int dtype, uint8_t* y_data,

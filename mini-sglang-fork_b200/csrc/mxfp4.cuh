@@ -90,6 +90,23 @@ __device__ __forceinline__ uint32_t pack8_scaled(const Vec8& v, float f) {
   return w;
 }
 
+// ---- computed values (fp32, relative error below `d`): their scale and codes,
+// from both ends of that error's interval.
+// The scale of a block whose largest magnitude is m; false where the ends differ
+// or it is the NaN scale.
+__device__ __forceinline__ bool scale_fast(float m, float d, int& byte) {
+  const uint32_t l = abs_bits(m * (1.0f - d)), h = abs_bits(m * (1.0f + d));
+  byte = scale_byte(l);
+  return ((l ^ h) >> 23) == 0 && byte != kNanScale;
+}
+
+// Codes of eight values; the result has a bit set in each code whose ends differ.
+__device__ __forceinline__ uint32_t codes_fast(const Vec8& y, int byte, float d, uint32_t& w) {
+  const float f = inv_scale(byte);
+  w = pack8_scaled(y, f * (1.0f - d));
+  return w ^ pack8_scaled(y, f * (1.0f + d));
+}
+
 // ---- 64-bit forms, for the values next to a border
 // E2M1 code of t (already divided by the block's scale).
 __device__ inline uint32_t code_of(double t) {
@@ -221,13 +238,85 @@ __device__ __forceinline__ float2 silu_mul_fast(float2 g, float2 u) {
   return __fmul2_rn(__fmul2_rn(g, u), make_float2(rcp_approx(d.x), rcp_approx(d.y)));
 }
 
-// The same with the sigmoid taken into g first, for callers without a second
-// look: finite for every finite product, and a zero once exp(-g) overflows.
-__device__ __forceinline__ float2 silu_mul_plain(float2 g, float2 u) {
-  constexpr float c = -1.4426950408889634f;
-  const float2 t = __fmul2_rn(g, make_float2(c, c));
-  const float2 d = __fadd2_rn(make_float2(ex2_approx(t.x), ex2_approx(t.y)), make_float2(1.0f, 1.0f));
-  return __fmul2_rn(__fmul2_rn(g, make_float2(rcp_approx(d.x), rcp_approx(d.y))), u);
+constexpr float kSiluDelta = 3.814697265625e-6f;  // 2^-18
+
+// The same with the rounding of t and of the constant put back, 2^t (1 + ln 2
+// lo): what is left is ex2's 2^-22, rcp's 2^-23, three additions and products'
+// 2^-24 each and that of the factor with which the result is packed, 6.6e-7
+// together for g in [-40, inf): below 2^-20 = 9.5e-7.  (In results below 2^-126
+// fp32's spacing adds up to 2^-149; the smallest border is 2^-129.)
+__device__ __forceinline__ float2 silu_mul_close(float2 g, float2 u) {
+  constexpr float c = -1.44269502162933349609375f, cl = -1.925962991e-8f, ln2 = 0.693147180559945f;
+  const float2 cc = make_float2(c, c);
+  const float2 t = __fmul2_rn(g, cc);
+  float2 lo = __ffma2_rn(g, cc, make_float2(-t.x, -t.y));
+  lo = __fmul2_rn(__ffma2_rn(g, make_float2(cl, cl), lo), make_float2(ln2, ln2));
+  float2 e = make_float2(ex2_approx(t.x), ex2_approx(t.y));
+  e = __ffma2_rn(e, lo, e);
+  const float2 d = __fadd2_rn(e, make_float2(1.0f, 1.0f));
+  return __fmul2_rn(__fmul2_rn(g, u), make_float2(rcp_approx(d.x), rcp_approx(d.y)));
+}
+constexpr float kSiluCloseDelta = 9.5367431640625e-7f;  // 2^-20
+
+// silu(g) * u in 64 bits.
+__device__ inline double silu_mul_exact(float g, float u) {
+  const double x = g;
+  return x / (1.0 + exp(-x)) * static_cast<double>(u);
+}
+
+// Pairs of fp32 numbers hi + lo, about 2^-46 relative.
+__device__ __forceinline__ float2 pair_sum(float a, float b) {  // exact
+  const float s = a + b, t = s - a;
+  return make_float2(s, (a - (s - t)) + (b - t));
+}
+__device__ __forceinline__ float2 pair_mul(float2 a, float2 b) {
+  const float h = a.x * b.x;
+  return make_float2(h, fmaf(a.x, b.x, -h) + fmaf(a.x, b.y, a.y * b.x));
+}
+__device__ __forceinline__ float2 pair_add(float2 c, float2 a) {  // |c.x| >= |a.x|
+  const float s = c.x + a.x;
+  return make_float2(s, (a.x - (s - c.x)) + (a.y + c.y));
+}
+
+// 1 + exp(-g) for g >= -40 (below 1 + e^-80 as that), as a pair: the exponential is
+// 2^n e^z, with z / 8 in a Taylor polynomial and that squared three times.
+// Relative errors add up to 2^-41.
+__device__ __forceinline__ float2 one_plus_exp_neg(float g) {
+  constexpr float c = 1.44269502162933349609375f, cl = 1.925962991e-8f;  // log2(e)
+  constexpr float k = 0.0866433978080749512f, kl = -2.380817875e-10f;    // ln(2) / 8
+  constexpr float sixth = 0.16666667163372039795f, sixth_l = -4.967053731e-9f;
+  const float x = fmaxf(-g, -80.0f);
+  const float t = x * c, n = rintf(t);
+  const float2 z = pair_mul(pair_sum(t - n, fmaf(x, cl, fmaf(x, c, -t))), make_float2(k, kl));
+  float2 e = make_float2(fmaf(z.x, fmaf(z.x, fmaf(z.x, 1.0f / 5040.0f, 1.0f / 720.0f), 1.0f / 120.0f), 1.0f / 24.0f), 0.0f);
+  e = pair_add(make_float2(sixth, sixth_l), pair_mul(z, e));
+  e = pair_add(make_float2(0.5f, 0.0f), pair_mul(z, e));
+  e = pair_add(make_float2(1.0f, 0.0f), pair_mul(z, e));
+  e = pair_add(make_float2(1.0f, 0.0f), pair_mul(z, e));
+#pragma unroll
+  for (int i = 0; i < 3; ++i) e = pair_mul(e, e);
+  const float s = __int_as_float((static_cast<int>(n) + 127) << 23);  // n is in [-116, 58]
+  const float2 d = pair_sum(1.0f, e.x * s);
+  return make_float2(d.x, fmaf(e.y, s, d.y));
+}
+
+// On which side of `border` |silu(g) u| f lies (1 above, -1 below), for a value
+// within 2^-17 of it; 0 where this does not tell (within 2^-38, or factors out of
+// the range that it is made for): compares |g u| f with border (1 + exp(-g)).  It
+// takes no 64-bit instruction: while tcgen05.mma runs the first of those waits
+// for some 5000 clocks (170 otherwise).
+__device__ __forceinline__ int silu_mul_side(float g, float u, float f, float border) {
+  const float ag = fabsf(g), au = fabsf(u) * f;
+  if (!(ag > 8.67361738e-19f && g >= -40.0f && g < 1.15292150e18f && au < 3.402823466e38f)) return 0;  // 2^-60, 2^60
+  const float2 d = one_plus_exp_neg(g);
+  const float p = ag * au, pl = fmaf(ag, au, -p);
+  const float diff = fmaf(-border, d.x, p) + fmaf(-border, d.y, pl);  // (the first is exact)
+  return fabsf(diff) <= p * 3.6379788e-12f ? 0 : diff > 0.0f ? 1 : -1;  // 2^-38
+}
+
+// Border between the E2M1 magnitudes c and c + 1.
+__device__ __forceinline__ float border_above(uint32_t c) {
+  return c < 4 ? 0.25f + 0.5f * static_cast<float>(c) : c == 4 ? 2.5f : c == 5 ? 3.5f : 5.0f;
 }
 
 }  // namespace mx

@@ -349,6 +349,7 @@ __global__ void __launch_bounds__(PairTraits::kThreads, 1)
             up[e] = __uint_as_float(acc ? own[e] : sh[e]);
           }
           silu_block(g, bias, gate, up, row0 + lane, tn, j);
+          __syncwarp();  // (tcgen05.ld and the closing barriers want a converged warp)
         };
         dev::tmem_ld32(own_t + 32 * hh, v);
         dev::tmem_wait_ld(v);
@@ -437,6 +438,7 @@ __global__ void __launch_bounds__(PairTraits::kThreads, 1)
             up[e] = __uint_as_float(w[e]);
           }
           silu_block(g, bias_s, gate, up, row0 + lane, tn, 2 * share + hh);
+          __syncwarp();
         } else {
 #pragma unroll 1
           for (int i = hh; i < 4; i += 2) {

@@ -116,12 +116,8 @@ __global__ void __launch_bounds__(kThreads) quant_kernel(const T* __restrict__ x
 // block's four lanes).  False where that error could change either: then
 // block_exact gives them.
 __device__ __forceinline__ bool block_fast(const Vec8& y, float m, float d, uint32_t& w, int& byte) {
-  const uint32_t l = abs_bits(m * (1.0f - d)), h = abs_bits(m * (1.0f + d));
-  byte = scale_byte(l);
-  const float f = inv_scale(byte);
-  w = pack8_scaled(y, f * (1.0f - d));
-  const uint32_t hi = pack8_scaled(y, f * (1.0f + d));
-  return ((l ^ h) >> 23) == 0 && byte != kNanScale && w == hi;
+  const bool sure = scale_fast(m, d, byte);
+  return codes_fast(y, byte, d, w) == 0 && sure;
 }
 
 // The same from eight exact values; all four lanes of the block come here.
@@ -161,14 +157,9 @@ __device__ inline float element(const uint4& raw, int j) {
 }
 
 // -------------------------------------------------------------- SiLU * mul
-constexpr float kSiluDelta = 3.814697265625e-6f;  // 2^-18, see silu_mul_fast
-
 template <typename T>
 __device__ __noinline__ uint2 silu_exact(uint4 graw, uint4 uraw, int lane) {
-  return block_exact(lane, [&](int j) {
-    const double g = element<T>(graw, j);
-    return g / (1.0 + exp(-g)) * static_cast<double>(element<T>(uraw, j));
-  });
+  return block_exact(lane, [&](int j) { return silu_mul_exact(element<T>(graw, j), element<T>(uraw, j)); });
 }
 
 // Smallest of eight gates.  Below -40 the fast form's argument error grows (and

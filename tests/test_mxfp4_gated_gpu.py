@@ -1,0 +1,66 @@
+"""GPU: the gate_up product's epilogue, code by code: its result is the
+quantisation of the exact silu(gate) * up of its fp32 sums."""
+from __future__ import annotations
+
+import pytest
+import torch
+
+from oracle import mxfp4_oracle as O
+from test_mxfp4_gpu import _gen, _no_timeouts, _same  # noqa: F401
+
+pytestmark = pytest.mark.gpu
+
+BITS = 24
+
+
+def _sums(pkg, dev, values, m, k):
+    """Operands whose product is exactly `values` (fp32 [N]) in each of `m` rows:
+    a is 1 in the first column of every 32-value block, and a weight row has one
+    bit of its value in each of 24 blocks, spread over K from the highest down,
+    so that every partial sum is a 24-bit number."""
+    n = values.numel()
+    a = torch.zeros(m, k, dtype=torch.long)
+    a[:, ::32] = 2  # the code of 1
+    a = pkg.MXFP4Tensor(O.pack(a).to(dev), O.tile(torch.full((m, k // 32), 127)).to(dev))
+    mant, exp = torch.frexp(values.double().abs())
+    whole = (mant * 2 ** BITS).long()  # 24 bits, the highest set
+    assert torch.equal(whole.double() * torch.exp2((exp - BITS).double()), values.double().abs())
+    codes = torch.zeros(n, k, dtype=torch.long)
+    scales = torch.zeros(n, k // 32, dtype=torch.long)
+    for b in range(BITS):
+        at = b * (k // 32) // BITS
+        bit = (whole >> (BITS - 1 - b)) & 1
+        codes[:, 32 * at] = bit * torch.where(values < 0, 10, 2)
+        scales[:, at] = (exp - 1 - b + 127).clamp(min=0)
+        assert ((exp - 1 - b + 127 >= 0) | (bit == 0)).all()
+    return a, pkg.MXFP4Tensor(O.pack(codes).to(dev), O.tile(scales).to(dev))
+
+
+def _check(pkg, dev, gate, up, m, k):
+    i = gate.numel()
+    a, w = _sums(pkg, dev, torch.cat([gate, up]), m, k)
+    y = pkg.mxfp4_gate_up_silu_quant(a, w)
+    want, byte = O.quant(O.silu_mul(gate, up)[None])
+    _same(y, want.expand(m, i), byte.expand(m, -1))
+
+
+# K 768: one share of K; 4096 and 8192: several CTAs, or two SM pairs, share a block's
+SHAPES = [(1, 128, 768), (20, 160, 768), (64, 256, 1536), (100, 384, 768), (300, 416, 768),
+          (1, 256, 8192), (17, 160, 8192), (50, 128, 12288), (130, 256, 4096), (300, 352, 8192)]
+
+
+@pytest.mark.parametrize("m,i,k", SHAPES)
+def test_values_next_to_borders(pkg, cuda_dev, m, i, k):
+    """Products within fp32's rounding of a border between two codes, in a block
+    whose scale is 1 (its first product is near 6), and largest products next to
+    a power of two."""
+    g = _gen(m + i)
+    borders = torch.tensor([0.25, 0.75, 1.25, 1.75, 2.5, 3.5, 5.0])
+    for seed in range(3):
+        target = borders[torch.randint(0, 7, (i,), generator=g)]
+        target[::32] = 6.3
+        target[32::64] = 4.0  # just below or above: the block's scale hangs on it
+        target *= torch.randint(0, 2, (i,), generator=g) * 2 - 1
+        gate = torch.where(torch.rand(i, generator=g) < 0.5, 1.0, -1.0) * torch.rand(i, generator=g) * 12 + 0.01
+        up = (target.double() / O.silu_mul(gate, torch.ones(i))).float()
+        _check(pkg, cuda_dev, gate, up, m, k)
