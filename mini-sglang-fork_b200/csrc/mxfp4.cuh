@@ -258,6 +258,21 @@ __device__ __forceinline__ float2 silu_mul_close(float2 g, float2 u) {
 }
 constexpr float kSiluCloseDelta = 9.5367431640625e-7f;  // 2^-20
 
+// The same for g < -40, where the sigmoid is 2^-t (1 + 2^-t is 1 to 2^-57) and
+// neither 2^t nor its reciprocal need fit fp32 although the product with a large u
+// does: four factors 2^(-t/4), u first, so that no partial product is larger than
+// u or smaller than the result.  Their 2^-22 each and the products' 2^-24 stay
+// below 2^-18.  (Below -1000 the result is zero for every u.)
+__device__ __forceinline__ float silu_mul_far(float g, float u) {
+  constexpr float c = 1.44269502162933349609375f, cl = 1.925962991e-8f, ln2 = 0.693147180559945f;
+  const float x = fmaxf(g, -1000.0f);
+  const float t = x * c, lo = fmaf(x, cl, fmaf(x, c, -t)) * ln2;
+  const float h = ex2_approx(0.25f * t);
+  const float y = u * h * g * h * h * h;
+  return fmaf(y, lo, y);
+}
+constexpr float kSiluFar = -40.0f;
+
 // silu(g) * u in 64 bits.
 __device__ inline double silu_mul_exact(float g, float u) {
   const double x = g;
@@ -278,16 +293,17 @@ __device__ __forceinline__ float2 pair_add(float2 c, float2 a) {  // |c.x| >= |a
   return make_float2(s, (a.x - (s - c.x)) + (a.y + c.y));
 }
 
-// 1 + exp(-g) for g >= -40 (below 1 + e^-80 as that), as a pair: the exponential is
-// 2^n e^z, with z / 8 in a Taylor polynomial and that squared three times.
-// Relative errors add up to 2^-41.
-__device__ __forceinline__ float2 one_plus_exp_neg(float g) {
+// exp(-g) as 2^n times a pair (exp(80) for g beyond 80): e^z, with z / 8 in a
+// Taylor polynomial and that squared three times.  Relative errors add up to 2^-41
+// (2^-40 for g = -185, by the argument).
+__device__ __forceinline__ float2 exp_neg(float g, int& n) {
   constexpr float c = 1.44269502162933349609375f, cl = 1.925962991e-8f;  // log2(e)
   constexpr float k = 0.0866433978080749512f, kl = -2.380817875e-10f;    // ln(2) / 8
   constexpr float sixth = 0.16666667163372039795f, sixth_l = -4.967053731e-9f;
   const float x = fmaxf(-g, -80.0f);
-  const float t = x * c, n = rintf(t);
-  const float2 z = pair_mul(pair_sum(t - n, fmaf(x, cl, fmaf(x, c, -t))), make_float2(k, kl));
+  const float t = x * c, r = rintf(t);
+  n = static_cast<int>(r);
+  const float2 z = pair_mul(pair_sum(t - r, fmaf(x, cl, fmaf(x, c, -t))), make_float2(k, kl));
   float2 e = make_float2(fmaf(z.x, fmaf(z.x, fmaf(z.x, 1.0f / 5040.0f, 1.0f / 720.0f), 1.0f / 120.0f), 1.0f / 24.0f), 0.0f);
   e = pair_add(make_float2(sixth, sixth_l), pair_mul(z, e));
   e = pair_add(make_float2(0.5f, 0.0f), pair_mul(z, e));
@@ -295,20 +311,33 @@ __device__ __forceinline__ float2 one_plus_exp_neg(float g) {
   e = pair_add(make_float2(1.0f, 0.0f), pair_mul(z, e));
 #pragma unroll
   for (int i = 0; i < 3; ++i) e = pair_mul(e, e);
-  const float s = __int_as_float((static_cast<int>(n) + 127) << 23);  // n is in [-116, 58]
-  const float2 d = pair_sum(1.0f, e.x * s);
-  return make_float2(d.x, fmaf(e.y, s, d.y));
+  return e;
 }
 
-// On which side of `border` |silu(g) u| f lies (1 above, -1 below), for a value
-// within 2^-17 of it; 0 where this does not tell (within 2^-38, or factors out of
-// the range that it is made for): compares |g u| f with border (1 + exp(-g)).  It
-// takes no 64-bit instruction: while tcgen05.mma runs the first of those waits
-// for some 5000 clocks (170 otherwise).
-__device__ __forceinline__ int silu_mul_side(float g, float u, float f, float border) {
-  const float ag = fabsf(g), au = fabsf(u) * f;
-  if (!(ag > 8.67361738e-19f && g >= -40.0f && g < 1.15292150e18f && au < 3.402823466e38f)) return 0;  // 2^-60, 2^60
-  const float2 d = one_plus_exp_neg(g);
+// 2^n for n in [-126, 127].
+__device__ __forceinline__ float power2(int n) { return __int_as_float((n + 127) << 23); }
+
+// On which side of `border` |silu(g) u| / 2^scale lies (1 above, -1 below), for a
+// value within 2^-16 of it; 0 where this does not tell (within 2^-38, or factors
+// out of the range that it is made for): compares |g u| / 2^scale with border (1 +
+// exp(-g)), below kSiluFar both over 2^n.  It takes no 64-bit instruction: while
+// tcgen05.mma runs the first of those waits for some 5000 clocks (170 otherwise).
+__device__ __forceinline__ int silu_mul_side(float g, float u, int scale, float border) {
+  const float ag = fabsf(g);
+  if (!(ag > 8.67361738e-19f && g > -185.0f && g < 1.15292150e18f)) return 0;  // 2^-60, 2^60
+  int n;
+  float2 d = exp_neg(g, n);
+  int up = -scale;
+  if (g < kSiluFar) {
+    up -= n;
+  } else {
+    const float s = power2(n);  // n is in [-116, 58]
+    const float2 sum = pair_sum(1.0f, d.x * s);
+    d = make_float2(sum.x, fmaf(d.y, s, sum.y));
+  }
+  if (up < -250) return 0;
+  const float au = fabsf(u) * power2(up >> 1) * power2(up - (up >> 1));
+  if (!(au > 8.67361738e-19f && au < 3.402823466e38f)) return 0;
   const float p = ag * au, pl = fmaf(ag, au, -p);
   const float diff = fmaf(-border, d.x, p) + fmaf(-border, d.y, pl);  // (the first is exact)
   return fabsf(diff) <= p * 3.6379788e-12f ? 0 : diff > 0.0f ? 1 : -1;  // 2^-38

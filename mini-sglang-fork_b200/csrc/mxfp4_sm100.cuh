@@ -190,10 +190,10 @@ __device__ __forceinline__ float pick32(const Vec8 (&v)[4], int at) {
 // output row, as one MXFP4 block: the quantisation of the exact product of the
 // fp32 sums (plus biases), by the border check of the quantisers.  A block in
 // 10^4 has a value within the check's 2^-20 of a border; silu_mul_side places it,
-// and what that leaves open the block's 64-bit form.  (12288 x 4096: 19.4 us for
-// 256 tokens and 286 for 8192, where one conversion without a check took 18.6 and
-// 280 and gave the neighbouring code once in 4 10^7; with the second look in 64
-// bits, beside the running MMAs, 21 to 22 and 300.)
+// and what that leaves open the block's 64-bit form.  (12288 x 4096: 19.7 us for
+// 256 tokens and 290 for 8192, where one conversion without a check took 18.5 and
+// 280, gave the neighbouring code once in 4 10^7 and zeros for gates below -87;
+// with the second look in 64 bits, beside the running MMAs, 21 to 22 and 300.)
 // `bias`: the tile's 128 gate and 128 up biases in shared memory.
 __device__ __forceinline__ void silu_block(const MxGemmArgs& g, const float* bias, const float (&gate)[32],
                                            const float (&up)[32], int64_t row, int ft, int j) {
@@ -218,8 +218,24 @@ __device__ __forceinline__ void silu_block(const MxGemmArgs& g, const float* bia
     for (int e = 0; e < 4; ++e) y[i].p[e] = silu_mul_close(gv[i].p[e], uv[i].p[e]);
   }
   if (row >= g.M || f0 >= g.N) return;
+  float least_gate = 0.0f;
+#pragma unroll
+  for (int i = 0; i < 4; ++i)
+#pragma unroll
+    for (int e = 0; e < 4; ++e) least_gate = fminf(least_gate, fminf(gv[i].p[e].x, gv[i].p[e].y));
+  const bool far = least_gate < kSiluFar;
+  if (far) {
+#pragma unroll
+    for (int i = 0; i < 4; ++i)
+#pragma unroll
+      for (int e = 0; e < 4; ++e) {
+        if (gv[i].p[e].x < kSiluFar) y[i].p[e].x = silu_mul_far(gv[i].p[e].x, uv[i].p[e].x);
+        if (gv[i].p[e].y < kSiluFar) y[i].p[e].y = silu_mul_far(gv[i].p[e].y, uv[i].p[e].y);
+      }
+  }
   const float m = max3_abs(max3_abs(amax8(y[0]), amax8(y[1]), amax8(y[2])), amax8(y[3]), 0.0f);
-  const float d = m < 1e-36f ? kSiluDelta : kSiluCloseDelta;  // (results near the end of fp32's range)
+  const bool tiny = m < 1e-36f;  // results near the end of fp32's range
+  const float d = far || tiny ? kSiluDelta : kSiluCloseDelta;
   int byte;
   uint32_t w[4] = {0, 0, 0, 0}, left = 0;  // left: bit e is value e's, to be looked at again
   const auto encode = [&] {
@@ -232,7 +248,7 @@ __device__ __forceinline__ void silu_block(const MxGemmArgs& g, const float* bia
     }
   };
   bool scale_open = !scale_fast(m, d, byte);
-  bool settled = byte < 252 && d == kSiluCloseDelta;  // (else only the 64-bit form may look again)
+  bool settled = byte < 252 && !tiny;  // (else only the 64-bit form may look again)
   if (!scale_open) {
     settled = true;
     encode();
@@ -249,8 +265,8 @@ __device__ __forceinline__ void silu_block(const MxGemmArgs& g, const float* bia
     left &= left - 1;
     const uint32_t code = at < 8 ? w[0] : at < 16 ? w[1] : at < 24 ? w[2] : w[3];
     const float border = scale_open ? 8.0f : border_above(code >> nib & 7u);
-    const int side = silu_mul_side(pick32(gv, at), pick32(uv, at), inv_scale(byte), border);
-    settled = side != 0 && d == kSiluCloseDelta;
+    const int side = silu_mul_side(pick32(gv, at), pick32(uv, at), byte - 127, border);
+    settled = side != 0 && !tiny;
     if (scale_open) {
       above |= side > 0;
       if (left == 0) {

@@ -64,3 +64,29 @@ def test_values_next_to_borders(pkg, cuda_dev, m, i, k):
         gate = torch.where(torch.rand(i, generator=g) < 0.5, 1.0, -1.0) * torch.rand(i, generator=g) * 12 + 0.01
         up = (target.double() / O.silu_mul(gate, torch.ones(i))).float()
         _check(pkg, cuda_dev, gate, up, m, k)
+
+
+@pytest.mark.parametrize("m,i,k", [(1, 128, 768), (20, 160, 768), (100, 384, 768), (17, 160, 8192), (300, 352, 8192)])
+def test_far_gates(pkg, cuda_dev, m, i, k):
+    """Gates between -40 and -190, where the sigmoid leaves fp32's range, under
+    ups that lift the product back into it (up to 2^127): the values, some next to
+    a border; blocks that mix them with ordinary gates, and blocks of one gate."""
+    g = _gen(m + i)
+    borders = torch.tensor([0.25, 0.75, 1.25, 1.75, 2.5, 3.5, 5.0, 6.3, 1.0, 0.1])
+    for seed in range(6):
+        gate = -torch.rand(i, generator=g) * (45, 85, 150, 150, 150, 8)[seed] - (40.0 if seed < 5 else 84.0)
+        if seed == 3:
+            gate[::3] = torch.randn(gate[::3].numel(), generator=g) * 4 + 0.01
+        if seed >= 4:
+            gate = gate[::32].repeat_interleave(32)
+        shape = O.silu_mul(gate, torch.ones(i))
+        target = borders[torch.randint(0, 10, (i,), generator=g)].double()
+        target[::32] = 6.3
+        # each block's scale: within fp32's range, and such that every up is below 2^127
+        most = torch.floor(torch.log2(shape.abs().reshape(-1, 32).amin(1)) + 127 - 3).clamp(max=20)
+        target *= torch.exp2(torch.maximum(most - (0, 3, 6, 9, 12, 20)[seed], torch.full_like(most, -95.0))).repeat_interleave(32)
+        up = (target / shape).float().clamp(-1.7e38, 1.7e38)
+        up *= (torch.randint(0, 2, (i,), generator=g) * 2 - 1)
+        want = O.silu_mul(gate, up)
+        assert (want.abs() > 0).any() and (gate < -40).any()
+        _check(pkg, cuda_dev, gate, up, m, k)
