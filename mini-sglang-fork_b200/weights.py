@@ -226,14 +226,27 @@ def load_w8a8_state_dict(items: Iterable[Tuple[str, torch.Tensor]], rank: int, w
     return dict(w8a8_weight_stream(items, rank, world, num_kv_heads, quantise, device, dtype, num_experts))
 
 
+def _bf16_to_odd(w: torch.Tensor) -> torch.Tensor:
+    """fp32 to bf16, inexact values to the neighbour whose last bit is odd.  MXFP4
+    scales, codes and the borders between them have three significant bits or
+    fewer, an even last bit in bf16; so a value on one side of a border stays on
+    that side, and quantising the result is quantising ``w`` itself.  (An infinity
+    stays one, a NaN a NaN.)"""
+    bits = w.contiguous().view(torch.int32)
+    return ((bits >> 16) | (bits & 0xFFFF).ne(0)).to(torch.int16).view(torch.bfloat16)
+
+
 def mxfp4_quantiser(device: torch.device) -> Quantiser:
     """MXFP4 quantisation of a [N, K] weight on ``device``: (packed codes
-    [N, K/2], E8M0 bytes [N, K/32]), both uint8."""
+    [N, K/2], E8M0 bytes [N, K/32]), both uint8, the nearest to the weight's values
+    as they are in bf16, fp16 or fp32 (fp64 is rounded to fp32)."""
     def quantise(w: torch.Tensor) -> Tuple[torch.Tensor, torch.Tensor]:
         if w.dim() != 2:
             raise _lib.W8A8Error(_lib.ERR_INVALID_ARG, f"weight must be 2-D, got {tuple(w.shape)}")
-        t = w.dtype if w.dtype in (torch.bfloat16, torch.float16) else torch.bfloat16
-        q = ops.mxfp4_quant(w.to(device=device, dtype=t).contiguous())
+        w = w.to(device=device)
+        if w.dtype not in (torch.bfloat16, torch.float16):
+            w = _bf16_to_odd(w.float())
+        q = ops.mxfp4_quant(w.contiguous())
         return q.data, ops.mxfp4_plain_scales(q)
     return quantise
 

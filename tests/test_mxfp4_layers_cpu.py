@@ -120,6 +120,44 @@ def test_state_dict_contract(pkg):
         layer.load_state_dict({**good, "weight_scale": torch.zeros(48, 2, dtype=torch.uint8)})
 
 
+def _fp32_weights():
+    """fp32 values between the bf16 ones: next to every border, next to powers of
+    two (a block's scale), at both ends of the type, infinities and NaN."""
+    g = torch.Generator().manual_seed(7)
+    rows = [torch.randn(64, generator=g) * 0.02 for _ in range(60)]
+    ulp = torch.tensor([1 - 2.0 ** -20, 1 + 2.0 ** -20, 1.0, 1 - 2.0 ** -24, 1 + 2.0 ** -23])
+    borders = torch.tensor([0.25, 0.75, 1.25, 1.75, 2.5, 3.5, 5.0, 7.5, 4.0, 6.0])
+    near = (borders[:, None] * ulp).flatten()  # 50 values
+    for e in (-100, -10, 0, 3, 100):
+        for top in (4.0, 4.0 * (1 - 2.0 ** -24), 7.9999, 8.0 * (1 - 2.0 ** -24)):
+            row = torch.cat([near[:31], torch.tensor([top]), near[-31:].clamp(max=top), torch.tensor([top])])
+            rows.append(row * 2.0 ** e * (torch.randint(0, 2, (64,), generator=g) * 2 - 1))
+    bits = torch.randint(0, 2 ** 31 - 1, (200, 64), generator=g, dtype=torch.int64).to(torch.int32)
+    rows += list((bits & 0x007fffff).view(torch.float32))  # subnormals
+    rows += list(bits.view(torch.float32))  # anything, infinities' exponents among them
+    last = torch.randn(4, 64, generator=g)
+    last[0, 5], last[1, 40], last[2, 3] = float("inf"), float("nan"), torch.finfo(torch.float32).max
+    last[3, 0] = torch.tensor(0x7f800001, dtype=torch.int32).view(torch.float32)  # a NaN in its last bit alone
+    return torch.stack(rows + list(last))
+
+
+def test_fp32_checkpoint_is_quantised_as_it_is(pkg, monkeypatch):
+    """The codes and scales of an fp32 weight are the nearest to its own values, not
+    to those of its bf16 rounding."""
+    def quant(x):
+        assert x.dtype in (torch.bfloat16, torch.float16)
+        c, b = O.quant(x.double())
+        return pkg.MXFP4Tensor(O.pack(c), O.tile(b))
+
+    monkeypatch.setattr(pkg.ops, "mxfp4_quant", quant)
+    w = _fp32_weights()
+    c, b = O.quant(w.double())
+    assert not torch.equal(O.quant(w.bfloat16().double())[0], c)
+    for t in (w, w.t().contiguous().t()):
+        data, scales = pkg.weights.mxfp4_quantiser(torch.device("cpu"))(t)
+        assert torch.equal(O.unpack(data), c) and torch.equal(scales.long(), b)
+
+
 def _patch(pkg):
     """The operators' restatements in the place of the CUDA ones."""
     ops = pkg.ops
