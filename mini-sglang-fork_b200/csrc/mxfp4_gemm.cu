@@ -133,21 +133,19 @@ int pick_split(int64_t tiles, int kblocks, int threads, int smem, int per_sm, in
   return W8A8_OK;
 }
 
+// (M <= T)
 template <typename O, int T, bool SILU, bool DEEP>
 int launch_row(const Operands& o, MxGemmArgs args, cudaStream_t stream) {
   using P = MxRowTraits<T, SILU, DEEP>;
   constexpr auto kern = mx_row_kernel<O, T, SILU, DEEP>;
   if (int rc = allow_smem<kern>(P::kSmemBytes)) return rc;
-  const int64_t wtiles = (args.N + 127) / 128;
-  args.ttiles = (args.M + T - 1) / T;
+  const int64_t tiles = (args.N + 127) / 128;
+  args.tiles = static_cast<int>(tiles);
   CUtensorMap tw, tws, tx, txs;
   if (int rc = encode_operand(&tw, o.b, o.b_rows, args.K / 2, 128)) return rc;
   if (int rc = encode_words(&tws, o.bs, o.bs_tiles, k_tiles(args.K) * kTileBytes / 4, 256)) return rc;
   if (int rc = encode_operand(&tx, o.a, args.M, args.K / 2, T)) return rc;
   if (int rc = encode_words(&txs, o.as, row_tiles(args.M), k_tiles(args.K) * kTileBytes / 4, 256)) return rc;
-  const int64_t tiles = wtiles * args.ttiles;
-  W8A8_REQUIRE(tiles <= 0x7fff0000LL, W8A8_ERR_UNSUPPORTED, "mxfp4_gemm: too many output tiles");
-  args.tiles = static_cast<int>(tiles);
   int split = 1;
   if (DEEP)
     if (int rc = pick_split<kern>(tiles, args.kblocks, kRowThreads, P::kSmemBytes, P::kPerSm, 1, 8, SILU ? 6 : 2, &split)) return rc;
@@ -182,8 +180,7 @@ int launch_pair(const Operands& o, const MxGemmArgs& g, cudaStream_t stream) {
 template <typename O, int T, bool SILU>
 int launch_row_any(const Operands& o, const MxGemmArgs& args, cudaStream_t stream) {
   if constexpr (!SILU && T < 128) {
-    const int64_t tiles = static_cast<int64_t>((args.N + 127) / 128) * ((args.M + T - 1) / T);
-    if (tiles > sm_count()) return launch_row<O, T, false, false>(o, args, stream);
+    if ((args.N + 127) / 128 > sm_count()) return launch_row<O, T, false, false>(o, args, stream);
   }
   return launch_row<O, T, SILU, true>(o, args, stream);
 }

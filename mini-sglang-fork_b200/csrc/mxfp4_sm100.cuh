@@ -85,7 +85,7 @@ struct MxGemmArgs {
   int M, N, K;       // N: output columns (I with the SiLU epilogue: B has N gate
                      // rows and N up rows, each half with scale tiles of its own)
   int kblocks;       // 256-value k blocks
-  int ttiles, tiles;  // weight-stationary kernel: token tiles, output tiles
+  int tiles;         // weight-stationary kernel: 128-column tiles of the output
 };
 
 // Copies `bytes` (a multiple of 16) of this CTA's shared memory into another
@@ -302,9 +302,9 @@ __device__ __forceinline__ void silu_block(const MxGemmArgs& g, const float* bia
 }
 
 // ------------------------------------------------- weight-stationary kernel
-// For up to 128 tokens per tile.  One CTA computes 128 output columns (weight
-// rows, on the MMA's 128-row side) for T tokens; with the SiLU epilogue 128
-// gate rows and the 128 up rows that belong to them, in two accumulators.
+// For up to T (16 to 128) tokens, all of them in every tile.  One CTA computes 128
+// output columns (weight rows, on the MMA's 128-row side); with the SiLU epilogue
+// 128 gate rows and the 128 up rows that belong to them, in two accumulators.
 // The weights are read once, at the rate of HBM, which is what bounds it; the
 // ring (about 200 KB of an SM's shared memory, in one CTA or in several) is
 // there to keep enough of them in flight.
@@ -396,9 +396,9 @@ __global__ void __launch_bounds__(kRowThreads, 1) mx_row_kernel(const __grid_con
   const int rank = static_cast<int>(dev::cluster_rank());
   const int first = blockIdx.x / S;
   const int step = gridDim.x / S;  // (S > 1: one tile per cluster)
-  const int wtiles = (args.N + 127) >> 7;
   const int kb0 = static_cast<int>(static_cast<int64_t>(rank) * args.kblocks / S);
   const int kb1 = static_cast<int>(static_cast<int64_t>(rank + 1) * args.kblocks / S);
+  const int tokens = args.M;  // at most T
   const long long tmo = args.timeout_ns;
 
   if (threadIdx.x == 0) {
@@ -431,9 +431,8 @@ __global__ void __launch_bounds__(kRowThreads, 1) mx_row_kernel(const __grid_con
       for (int kb = kb0; kb < min(kb1, kb0 + 5); ++kb)
 #pragma unroll
         for (int h = 0; h < P::kTiles; ++h) {
-          const int wt = first / args.ttiles;
-          tma_prefetch_2d(&tm_w, kb * 128, wt * 128 + h * args.N);
-          tma_prefetch_2d(&tm_ws, kb * 256, wt + h * wtiles);
+          tma_prefetch_2d(&tm_w, kb * 128, first * 128 + h * args.N);
+          tma_prefetch_2d(&tm_ws, kb * 256, first + h * args.tiles);
         }
     }
     __syncwarp();
@@ -450,7 +449,6 @@ __global__ void __launch_bounds__(kRowThreads, 1) mx_row_kernel(const __grid_con
     uint32_t phase = 0, issued_mask = 0, issued_phase = 0;
     bool ok = true;
     for (int tile = first; ok && tile < args.tiles; tile += step) {
-      const int tt = tile % args.ttiles, wt = tile / args.ttiles;
       for (int kb = kb0; kb < kb1; ++kb) {
         ok = warp_wait(dev::smem_u32(empty + stage), phase ^ 1u, abort_flag, args.err, tmo);
         if (!ok) break;
@@ -461,12 +459,12 @@ __global__ void __launch_bounds__(kRowThreads, 1) mx_row_kernel(const __grid_con
           for (int h = 0; h < P::kTiles; ++h) {
             // gate rows, then up rows
             dev::tma_load_2d(dev::smem_u32(s_w + (stage * P::kTiles + h) * P::kW), &tm_w, bar, kb * 128,
-                             wt * 128 + h * args.N);
+                             tile * 128 + h * args.N);
             dev::tma_load_2d(dev::smem_u32(s_ws + (stage * P::kTiles + h) * P::kSf), &tm_ws, bar, kb * 256,
-                             wt + h * wtiles);
+                             tile + h * args.tiles);
           }
-          dev::tma_load_2d(dev::smem_u32(s_x + stage * P::kX), &tm_x, bar, kb * 128, tt * T);
-          dev::tma_load_2d(dev::smem_u32(s_xs + stage * P::kSf), &tm_xs, bar, kb * 256, (tt * T) >> 7);
+          dev::tma_load_2d(dev::smem_u32(s_x + stage * P::kX), &tm_x, bar, kb * 128, 0);
+          dev::tma_load_2d(dev::smem_u32(s_xs + stage * P::kSf), &tm_xs, bar, kb * 256, 0);
         }
         __syncwarp();
         issued_mask |= 1u << stage;
@@ -545,11 +543,9 @@ __global__ void __launch_bounds__(kRowThreads, 1) mx_row_kernel(const __grid_con
                                           q * (P::kStagingBytes / 4));
     uint32_t i = 0;
     for (int tile = first; tile < args.tiles; tile += step, ++i) {
-      const int tt = tile % args.ttiles, wt = tile / args.ttiles;
-      const int tokens = min(T, args.M - tt * T);
       const uint32_t acc = i % P::kAccs, use = i / P::kAccs;
       // the biases before the wait for the sums
-      const int col = wt * 128 + n;
+      const int col = tile * 128 + n;
       float* bias = bias_s + (i & 1u) * 256;
       float bias_n = 0.0f;
       if (args.bias) {
@@ -569,7 +565,7 @@ __global__ void __launch_bounds__(kRowThreads, 1) mx_row_kernel(const __grid_con
       if (S > 1) break;  // one tile, finished below
       if constexpr (!SILU) {
         const bool in = col < args.N;
-        O* out = static_cast<O*>(args.out) + static_cast<int64_t>(tt) * T * args.N + col;
+        O* out = static_cast<O*>(args.out) + col;
         for (int c = 0; c < tokens; c += P::kChunk) {
           float v[32];
           tmem_ld_chunk<P::kChunk>(t_acc + c, v);
@@ -601,7 +597,7 @@ __global__ void __launch_bounds__(kRowThreads, 1) mx_row_kernel(const __grid_con
               *reinterpret_cast<float4*>(g + 4 * e) = *reinterpret_cast<const float4*>(stg + w);
               *reinterpret_cast<float4*>(u + 4 * e) = *reinterpret_cast<const float4*>(stg + P::kChunk * 32 + w);
             }
-            silu_block(args, bias, g, u, static_cast<int64_t>(tt) * T + c + lane, wt, q);
+            silu_block(args, bias, g, u, c + lane, tile, q);
           }
           __syncwarp();
         }
@@ -613,8 +609,6 @@ __global__ void __launch_bounds__(kRowThreads, 1) mx_row_kernel(const __grid_con
     dev::tc_fence_before();
   }
   if (DEEP && S > 1) {
-    const int tt = first % args.ttiles, wt = first / args.ttiles;
-    const int tokens = min(T, args.M - tt * T);
     const auto begin = [&](int s) { return tokens * s / S; };  // tokens [begin(s), begin(s + 1)) are s's
     const int t0 = begin(rank), count = begin(rank + 1) - t0;
     // in the ring: [token][gate / up][128] sums of this CTA, then from each
@@ -650,7 +644,6 @@ __global__ void __launch_bounds__(kRowThreads, 1) mx_row_kernel(const __grid_con
       }
       __syncwarp();
       if (count > 0) warp_wait(dev::smem_u32(arrived), 0, abort_flag, args.err, tmo);
-      const int64_t row0 = static_cast<int64_t>(tt) * T;
       // 16 bytes of the s-th share of token t (of this CTA's), word w
       const auto piece = [&](int s, int t, int w) {
         const float* p = s == rank ? own + t * kTokenWords : in + (s * count + t - t0) * kTokenWords;
@@ -666,13 +659,13 @@ __global__ void __launch_bounds__(kRowThreads, 1) mx_row_kernel(const __grid_con
             v[0] += x.x, v[1] += x.y, v[2] += x.z, v[3] += x.w;
             v[4] += y.x, v[5] += y.y, v[6] += y.z, v[7] += y.w;
           }
-          const int col = wt * 128 + n0;
+          const int col = first * 128 + n0;
           if (args.bias) {
             const Vec8 b = bias8<O>(args.bias, col, args.N);
 #pragma unroll
             for (int j = 0; j < 4; ++j) v[2 * j] += b.p[j].x, v[2 * j + 1] += b.p[j].y;
           }
-          store8_row<O>(args, row0 + t, col,
+          store8_row<O>(args, t, col,
                         make_uint4(pack2<O>(v[0], v[1]), pack2<O>(v[2], v[3]), pack2<O>(v[4], v[5]), pack2<O>(v[6], v[7])));
         }
       } else {
@@ -690,7 +683,7 @@ __global__ void __launch_bounds__(kRowThreads, 1) mx_row_kernel(const __grid_con
               u[4 * e] += y.x, u[4 * e + 1] += y.y, u[4 * e + 2] += y.z, u[4 * e + 3] += y.w;
             }
           }
-          silu_block(args, bias_s, g, u, row0 + t, wt, j);
+          silu_block(args, bias_s, g, u, t, first, j);
         }
       }
       __syncwarp();  // (the cluster barrier wants converged warps)
