@@ -10,7 +10,8 @@ makes both from a checkpoint.  Activations are quantised per 32 values on the
 way in, or arrive as an :class:`~.ops.MXFP4Tensor` from the layer before.
 
 Row-parallel layers hold a K-shard and sum over ranks with the plugin stack's
-``all_reduce`` after the product (the fused reduce exists for W8A8 only).
+``all_reduce`` after the product (the fused reduce exists for W8A8 only).  The
+peer-memory plugin sums bf16 only: with it, fp16 row-parallel layers are refused.
 Every local input size must be a multiple of 32.
 """
 from __future__ import annotations
@@ -20,7 +21,7 @@ from typing import List, Optional, Tuple, Union
 import torch
 
 from . import _lib, ops
-from .distributed import communicator, div_even, get_tp_info
+from .distributed import PeerMemDistributedImpl, communicator, div_even, get_tp_info
 from .layers import BaseOP
 from .ops import MXFP4Tensor
 
@@ -117,6 +118,10 @@ class _RowParallel(_LinearTPImpl):
         tp_info = get_tp_info()
         self._comm = communicator()
         self._tp_size = tp_info.size
+        if tp_info.size > 1 and dtype is not torch.bfloat16 and self._comm.plugins \
+                and isinstance(self._comm.plugins[-1], PeerMemDistributedImpl):
+            raise _lib.W8A8Error(_lib.ERR_UNSUPPORTED, "MXFP4 row-parallel linear: the peer-memory all-reduce sums bf16, "
+                                 f"not {dtype}; use bf16, or another all-reduce plugin")
         super().__init__(input_size, output_size, div_even(input_size, tp_info.size), output_size, has_bias, dtype)
 
     def forward(self, x: Activation) -> torch.Tensor:

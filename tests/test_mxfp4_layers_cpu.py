@@ -158,6 +158,35 @@ def test_fp32_checkpoint_is_quantised_as_it_is(pkg, monkeypatch):
         assert torch.equal(O.unpack(data), c) and torch.equal(scales.long(), b)
 
 
+def test_fp16_row_parallel_is_refused_with_the_peer_memory_plugin(pkg):
+    """The peer-memory all-reduce sums bf16: a layer whose every forward would fail
+    there is not made; other types, plugins and a single rank are."""
+    from importlib import import_module
+
+    D = import_module(pkg.__name__ + ".distributed")
+    plugins, L, E = D.DistributedCommunicator.plugins, pkg.mxfp4, pkg.W8A8Error
+    pkg.reset_tp_info()
+    try:
+        pkg.set_tp_info(0, 2)
+        L.LinearOProj(128, 64, False, torch.float16)
+        D.DistributedCommunicator.plugins = plugins + [D.PeerMemDistributedImpl(object())]
+        for make in (lambda t: L.LinearOProj(128, 64, False, t), lambda t: L.LinearRowParallel(128, 64, False, t),
+                     lambda t: L.GatedMLP(64, 128, t)):
+            make(torch.bfloat16)
+            with pytest.raises(E, match="peer-memory"):
+                make(torch.float16)
+        L.LinearReplicated(128, 64, False, torch.float16)
+        D.DistributedCommunicator.plugins = D.DistributedCommunicator.plugins + [D.TorchDistributedImpl()]
+        L.LinearOProj(128, 64, False, torch.float16)  # the last plugin is the one in use
+        D.DistributedCommunicator.plugins = plugins + [D.PeerMemDistributedImpl(object())]
+        pkg.reset_tp_info()
+        pkg.set_tp_info(0, 1)
+        L.LinearOProj(128, 64, False, torch.float16)
+    finally:
+        D.DistributedCommunicator.plugins = plugins
+        pkg.reset_tp_info()
+
+
 def _patch(pkg):
     """The operators' restatements in the place of the CUDA ones."""
     ops = pkg.ops
