@@ -1,12 +1,13 @@
-"""GPU: the gate_up product's epilogue, code by code: its result is the
-quantisation of the exact silu(gate) * up of its fp32 sums."""
+"""GPU: the gate_up product's epilogue, code by code (its result is the
+quantisation of the exact silu(gate) * up of its fp32 sums, which these tests
+make exact), and products whose K several CTAs or SM pairs share."""
 from __future__ import annotations
 
 import pytest
 import torch
 
 from oracle import mxfp4_oracle as O
-from test_mxfp4_gpu import _gen, _no_timeouts, _same  # noqa: F401
+from test_mxfp4_gpu import _gemm_bound, _gen, _no_timeouts, _operand, _same  # noqa: F401
 
 pytestmark = pytest.mark.gpu
 
@@ -90,3 +91,50 @@ def test_far_gates(pkg, cuda_dev, m, i, k):
         want = O.silu_mul(gate, up)
         assert (want.abs() > 0).any() and (gate < -40).any()
         _check(pkg, cuda_dev, gate, up, m, k)
+
+
+def _exact_sums(a, w, av, wv):
+    """The products' sums, which fp32 holds exactly in any order: each product is
+    a multiple of the unit below, and no partial sum reaches 2^24 of them."""
+    def least(t):
+        r, k = t.shape
+        return O.untile(t.scales, r, k // 32).min().item() - 127
+
+    unit = 2.0 ** (least(a) + least(w) - 2)
+    assert (av.abs() @ wv.abs().T).max() < 2 ** 23 * unit
+    return av @ wv.T
+
+
+# K 4096 and more with few blocks: two SM pairs, or up to eight CTAs, share a block's K
+@pytest.mark.parametrize("m,i,k", [(1, 128, 4096), (16, 256, 8192), (40, 160, 12288), (64, 128, 16384), (64, 416, 8192),
+                                   (65, 128, 4096), (129, 256, 8192), (200, 416, 8192), (256, 128, 25600), (333, 96, 8192),
+                                   (500, 608, 4096)])
+@pytest.mark.parametrize("dtype", [torch.bfloat16, torch.float16])
+def test_shares_of_k(pkg, cuda_dev, m, i, k, dtype):
+    """With and without biases, the intermediate size a multiple of 128 or not."""
+    a, av = _operand(pkg, m, k, 1.0, m + k, cuda_dev)
+    w, wv = _operand(pkg, 2 * i, k, 0.05, i + k, cuda_dev)
+    full = _exact_sums(a, w, av.to(cuda_dev), wv.to(cuda_dev)).cpu()
+    bias = torch.randint(-8, 9, (2 * i,), generator=_gen(i)).to(dtype) / 16
+    for b in (None, bias):
+        gu = (full if b is None else full + b.double()).float()
+        y = pkg.mxfp4_gate_up_silu_quant(a, w, None if b is None else b.to(cuda_dev), dtype)
+        _same(y, *O.quant(O.silu_mul(gu[:, :i], gu[:, i:])))
+
+
+@pytest.mark.parametrize("m,n,k", [(129, 500, 4096), (129, 256, 25600), (200, 1000, 8192), (256, 1280, 8192), (333, 643, 4096),
+                                   (333, 640, 25600), (500, 250, 8192), (500, 2056, 4096), (1000, 130, 4128)])
+@pytest.mark.parametrize("dtype", [torch.bfloat16, torch.float16])
+def test_product_shares_of_k(pkg, cuda_dev, m, n, k, dtype):
+    """The plain product where two SM pairs share a block's K: ragged M, N and K,
+    with and without a bias."""
+    a, av = _operand(pkg, m, k, 1.0, m + k, cuda_dev, spread=1)
+    w, wv = _operand(pkg, n, k, 0.05, n + k, cuda_dev, spread=2)
+    av, wv = av.to(cuda_dev), wv.to(cuda_dev)
+    ref, mag = (av @ wv.T).cpu(), (av.abs() @ wv.abs().T).cpu()
+    bias = (0.1 * torch.randn(n, generator=_gen(n))).to(dtype)
+    for b in (None, bias):
+        want = ref if b is None else ref + b.double()
+        out = pkg.mxfp4_gemm(a, w, None if b is None else b.to(cuda_dev), out_dtype=dtype)
+        err = (out.cpu().double() - want).abs()
+        assert (err <= _gemm_bound(k, mag, want, dtype)).all()
