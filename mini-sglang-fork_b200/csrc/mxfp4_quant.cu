@@ -114,10 +114,15 @@ __global__ void __launch_bounds__(kThreads) quant_kernel(const T* __restrict__ x
 // The quantisation of a computed block: codes and scale byte of a lane's eight
 // values `y` (fp32, relative error below `d`; m: the largest magnitude over the
 // block's four lanes).  False where that error could change either: then
-// block_exact gives them.
+// block_exact gives them.  (scale_fast and codes_fast spelled out: called from
+// here they cost the SiLU kernel, which is held to 48 registers, two more spills.)
 __device__ __forceinline__ bool block_fast(const Vec8& y, float m, float d, uint32_t& w, int& byte) {
-  const bool sure = scale_fast(m, d, byte);
-  return codes_fast(y, byte, d, w) == 0 && sure;
+  const uint32_t l = abs_bits(m * (1.0f - d)), h = abs_bits(m * (1.0f + d));
+  byte = scale_byte(l);
+  const float f = inv_scale(byte);
+  w = pack8_scaled(y, f * (1.0f - d));
+  const uint32_t hi = pack8_scaled(y, f * (1.0f + d));
+  return ((l ^ h) >> 23) == 0 && byte != kNanScale && w == hi;
 }
 
 // The same from eight exact values; all four lanes of the block come here.
