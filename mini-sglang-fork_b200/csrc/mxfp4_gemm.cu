@@ -119,9 +119,17 @@ int launch_cluster(Kernel kern, unsigned grid, int threads, int smem, int cluste
 
 // Shares of K per output tile, each the work of `ctas` CTAs: as many as leave
 // every tile's cluster resident at once (a second wave would cost as much as
-// the first), `most` at most, with `least` k blocks each (measured, B200: the
-// exchange costs 2 us for 128 tokens, and more than it saves below two k
-// blocks, six with the SiLU epilogue's two sums, eight for a 256 x 256 block).
+// the first), `most` at most, with `least` k blocks each: two, six with the SiLU
+// epilogue's two sums, eight for a 256 x 256 block.  Measured (us, B200), by least:
+//   plain, least 1, 2, 3, 4:  16 x 2048 x 2048  4.6 4.1 4.6 4.6;  16 x 4096 x 2048
+//     5.2 4.7 4.8 4.8;  64 x 2048 x 2048  6.4 5.5 5.9 5.9;  but 16 x 2048 x 1024
+//     4.0 3.9 3.3 3.3 and 128 x 4096 x 2048  8.6 8.6 7.8 7.8: two shares of two
+//     blocks cost more than they save.  From 4096 x 4096 on there is no difference.
+//   SiLU, least 3, 4, 6, 8:  64 x 2816 x 4096  11.7 10.7 10.3 10.3;  64 x 2816 x 8192
+//     14.2 14.3 13.4 13.0;  16 x 1536 x 2048  6.6 6.6 5.9 5.9;  but 16 x 1536 x 4096
+//     8.1 7.4 8.4 8.5.
+//   pairs, least 4, 6, 8, 12:  512 x 4096 x 2048  9.6 7.6 7.5 7.5;  200 x 2048 x 5120
+//     10.0 10.0 10.0 10.9;  512 x 4096 x 4096  11.1 11.1 11.1 10.3.
 template <auto Kern>
 int pick_split(int64_t tiles, int kblocks, int threads, int smem, int per_sm, int ctas, int most, int least, int* out) {
   *out = 1;
@@ -177,6 +185,9 @@ int launch_pair(const Operands& o, const MxGemmArgs& g, cudaStream_t stream) {
                         stream, ta, tas, tb, tbs, args);
 }
 
+// The short ring, several CTAs on an SM, once there are more tiles than SMs; else
+// the long one, with K split.  (51200 x 5120, 400 tiles: 22.9 us with the short
+// ring for 16 tokens, 26.9 with the long one; 28.7 and 34.6 for 64.)
 template <typename O, int T, bool SILU>
 int launch_row_any(const Operands& o, const MxGemmArgs& args, cudaStream_t stream) {
   if constexpr (!SILU && T < 128) {
@@ -185,6 +196,16 @@ int launch_row_any(const Operands& o, const MxGemmArgs& args, cudaStream_t strea
   return launch_row<O, T, SILU, true>(o, args, stream);
 }
 
+// The smallest token tile that holds them all; SM pairs above 128 tokens, 64 with
+// the SiLU epilogue (us, B200):
+//   T = 16, 32, for 16 tokens:  51200 x 5120  22.9 28.1;  5120 x 5120  6.6 6.8;  gate_up
+//     12288 x 4096  12.7 13.1
+//   T = 64, 128, for 48:  51200 x 5120  28.3 31.6;  5120 x 5120  7.6 8.7;  5120 x 25600
+//     16.0 16.3;  for 64:  28.7 26.5, 8.1 8.3, 16.5 16.8
+//   T = 128, pairs, for 65:  51200 x 5120  27.0 29.9;  5120 x 25600  17.0 24.3;  for 128:
+//     29.1 31.9, 18.9 24.6;  10240 x 5120  12.5 12.7
+//   SiLU, T = 64, pairs, for 64:  2816 x 4096  10.3 11.0;  12288 x 4096  14.5 19.1;
+//     25600 x 5120  28.8 30.7
 template <typename O, bool SILU>
 int dispatch(const Operands& o, const MxGemmArgs& args, cudaStream_t stream) {
   if (args.M <= 16) return launch_row_any<O, 16, SILU>(o, args, stream);

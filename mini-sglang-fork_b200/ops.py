@@ -667,7 +667,8 @@ def mxfp4_rmsnorm_quant(x: torch.Tensor, weight: torch.Tensor, eps: float,
     residual in place, as :func:`rmsnorm_quant` does) to MXFP4, the normalised
     row not rounded in between.  Returns ``(MXFP4Tensor, residual)``; the
     residual is ``x`` itself without one.  bf16 or fp16, K % 32 == 0, K <=
-    32768."""
+    32768.  Blocks of zeros in rows that are not all zeros (padded or pruned
+    channels) are evaluated in 64 bits and take longer."""
     dt = _check_mx_input("mxfp4_rmsnorm_quant", "x", x)
     m, k = x.shape
     if weight.dtype != x.dtype or weight.shape != (k,) or not weight.is_contiguous():
@@ -726,7 +727,9 @@ def mxfp4_gate_up_silu_quant(a: MXFP4Tensor, w: MXFP4Tensor, bias: Optional[torc
                              dtype: torch.dtype = torch.bfloat16) -> MXFP4Tensor:
     """The gated half of an MLP in MXFP4: ``w [2I, K]`` is the merged [gate;
     up] weight, the result MXFP4 ``silu(a gate^T) * (a up^T)``, ``[M, I]``,
-    formed from the fp32 sums; nothing of the [M, 2I] product reaches memory.
+    formed from the fp32 sums and not rounded before it is quantised (values next
+    to a rounding border are evaluated more closely); nothing of the [M, 2I]
+    product reaches memory.
     ``dtype`` is the bias's type.  I % 32 == 0; where I % 128 != 0 a first, small
     kernel lays the halves' scale tiles out apart."""
     code = _check_mx_gemm("mxfp4_gate_up_silu_quant", a, w, bias, dtype)
