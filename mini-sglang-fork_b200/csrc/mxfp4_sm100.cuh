@@ -280,18 +280,27 @@ __device__ __forceinline__ void silu_block(const MxGemmArgs& g, const float* bia
     }
   }
   if (!settled) {
-    GatedBlock b;
+    // a gate or an up that is not finite makes a product that is not either: no
+    // need to look at that one in 64 bits
+    const float worst = max3_abs(max3_abs(amax8(gv[0]), amax8(gv[1]), amax8(gv[2])), max3_abs(amax8(gv[3]), amax8(uv[0]), amax8(uv[1])),
+                                 max3_abs(amax8(uv[2]), amax8(uv[3]), 0.0f));
+    if (worst <= 3.402823466e38f) {
+      GatedBlock b;
 #pragma unroll
-    for (int i = 0; i < 4; ++i)
+      for (int i = 0; i < 4; ++i)
 #pragma unroll
-      for (int e = 0; e < 4; ++e) {
-        *reinterpret_cast<float2*>(b.g + 8 * i + 2 * e) = gv[i].p[e];
-        *reinterpret_cast<float2*>(b.u + 8 * i + 2 * e) = uv[i].p[e];
-      }
-    gated_block_exact(b);
+        for (int e = 0; e < 4; ++e) {
+          *reinterpret_cast<float2*>(b.g + 8 * i + 2 * e) = gv[i].p[e];
+          *reinterpret_cast<float2*>(b.u + 8 * i + 2 * e) = uv[i].p[e];
+        }
+      gated_block_exact(b);
 #pragma unroll
-    for (int i = 0; i < 4; ++i) w[i] = b.w[i];
-    byte = b.byte;
+      for (int i = 0; i < 4; ++i) w[i] = b.w[i];
+      byte = b.byte;
+    } else {
+      w[0] = w[1] = w[2] = w[3] = 0;
+      byte = kNanScale;
+    }
   }
   const int64_t kt = k_tiles(g.N);
   *reinterpret_cast<uint4*>(g.q + row * (g.N >> 1) + (f0 >> 1)) = make_uint4(w[0], w[1], w[2], w[3]);

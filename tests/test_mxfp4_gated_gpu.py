@@ -93,6 +93,38 @@ def test_far_gates(pkg, cuda_dev, m, i, k):
         _check(pkg, cuda_dev, gate, up, m, k)
 
 
+@pytest.mark.parametrize("m,k", [(1, 768), (40, 768), (100, 768), (64, 8192), (300, 8192)])
+def test_gates_and_ups_that_are_not_finite(pkg, cuda_dev, m, k):
+    """Infinite and NaN sums make their blocks NaN, next to values of any size; a
+    product beyond fp32 does, one whose factors' product alone overflows does not;
+    blocks without them are not touched."""
+    i, big = 384, 2.0 ** 127
+    g = _gen(m)
+    gate, up = (torch.randn(i, generator=g) + 0.01 for _ in range(2))
+    gate[1] = gate[6 * 32] = -1000.0
+    gate[2 * 32], up[2 * 32] = 300.0, 1e37       # 3e39
+    gate[3 * 32], up[3 * 32] = -20.0, 1.5 * big  # -20 e^-20 1.5 2^127: finite
+    gate[4 * 32], up[4 * 32] = -95.0, -big
+    a, w = _sums(pkg, cuda_dev, torch.cat([gate, up]), m, k)
+    # a column that no other value uses: 4 times 2^127, or the NaN scale
+    plain = pkg.ops.mxfp4_plain_scales(w).cpu()
+    codes = O.unpack(w.data)
+    want_g, want_u = gate.clone(), up.clone()
+    free = next(c for c in range(k // 32) if c not in {b * (k // 32) // BITS for b in range(BITS)}) if k > 768 else None
+    for row, code, byte in ((6 * 32, 6, 254), (7 * 32 + 5, 14, 254), (8 * 32 + 31, 0, 255), (i + 9 * 32 + 1, 6, 254),
+                            (i + 10 * 32 + 2, 0, 255)):
+        at = 0 if free is None else free
+        codes[row] = 0  # its own value goes
+        codes[row, 32 * at] = code
+        plain[row, at] = byte
+        (want_g if row < i else want_u)[row % i] = float("nan") if byte == 255 else float("inf") * (-1 if code == 14 else 1)
+    w = pkg.MXFP4Tensor(O.pack(codes).to(cuda_dev), pkg.ops.mxfp4_tile_scales(plain).to(cuda_dev))
+    y = pkg.mxfp4_gate_up_silu_quant(a, w)
+    want, byte = O.quant(O.silu_mul(want_g, want_u)[None])
+    assert (byte[0] == 255).nonzero().flatten().tolist() == [2, 6, 7, 8, 9, 10]
+    _same(y, want.expand(m, i), byte.expand(m, -1))
+
+
 def _exact_sums(a, w, av, wv):
     """The products' sums, which fp32 holds exactly in any order: each product is
     a multiple of the unit below, and no partial sum reaches 2^24 of them."""
