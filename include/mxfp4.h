@@ -63,7 +63,9 @@ int mxfp4_dequant(const uint8_t* data, const uint8_t* scales, void* out, int dty
 /* gate_up[M, 2I] bf16 or fp16 (row stride ld) -> MXFP4 of
  * y = gate / (1 + exp(-gate)) * up, [M, I].  y is not rounded before it is
  * quantised; values that land next to a rounding border are evaluated in 64
- * bits.  I % 32 == 0, ld % 8 == 0. */
+ * bits.  So are blocks with a gate below -40 or a NaN: a call takes longer the
+ * more of those there are (4096 x 12288: 46 us; 57 and 159 us with 1 and 10 % of
+ * the blocks).  I % 32 == 0, ld % 8 == 0. */
 int mxfp4_silu_mul_quant(const void* gate_up, int64_t ld, int dtype, uint8_t* data, uint8_t* scales,
                          int64_t M, int64_t I, void* stream);
 

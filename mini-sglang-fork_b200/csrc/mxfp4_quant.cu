@@ -168,7 +168,10 @@ __device__ __noinline__ uint2 silu_exact(uint4 graw, uint4 uraw, int lane) {
 }
 
 // Smallest of eight gates.  Below -40 the fast form's argument error grows (and
-// its reciprocal flushes further down); those blocks are taken in 64 bits.
+// its reciprocal flushes further down); those blocks are taken in 64 bits, as are
+// blocks with a NaN.  (4096 x 12288: 45.6 us without any; with a gate at -50 in 1,
+// 10 and 100 % of the blocks of each row 57, 159 and 217 us, with a NaN 67, 124 and
+// 192.)
 template <typename T>
 __device__ __forceinline__ float min8(const uint4& raw);
 
